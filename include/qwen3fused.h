@@ -33,6 +33,10 @@ extern "C" {
 enum { QF_F32 = 0, QF_F16 = 1, QF_BF16 = 2 };
 enum { QF_I32 = 0, QF_I64 = 1 };
 
+/* What the rows of a paged cache hold: elements of the call's dtype, or 8-bit
+ * codes with one fp32 scale per row (see qf_kv_store_quantized). */
+enum { QF_CACHE_PLAIN = 0, QF_CACHE_E4M3 = 1, QF_CACHE_INT8 = 2 };
+
 enum {
     QF_OK = 0,
     QF_ERR_INVALID = 1,     /* null pointer, negative size, unknown tag */
@@ -48,7 +52,9 @@ enum {
     QF_FLAG_BAD_SLOT = 2,  /* slot index < 0 or >= block_size */
     QF_FLAG_BAD_TOKEN = 4, /* token id < 0 or >= vocab */
     QF_FLAG_BAD_TABLE = 8, /* logical block beyond the block table's length */
-    QF_FLAG_TIMEOUT = 16   /* a kernel gave up waiting on its own tensor-core work */
+    QF_FLAG_TIMEOUT = 16,  /* a kernel gave up waiting on its own tensor-core work */
+    QF_FLAG_BAD_TREE = 32  /* a node's parent is not an earlier node, or more drafted
+                              tokens than the call's max_tree */
 };
 
 /* ---------------------------------------------------------------------- */
@@ -268,6 +274,113 @@ int qf_paged_attention_decode_noalloc(const qf_paged_attention_args* args, cudaS
 
 /* Bytes of the fixed array qf_paged_attention_decode_noalloc uses. */
 size_t qf_paged_attention_noalloc_capacity(void);
+
+/* ---------------------------------------------------------------------- */
+/* Quantised paged KV cache: rows quantised as they are written.  No
+ * counterpart in the reference, whose caches hold the model's dtype.
+ * For the row x of token t, head h (K, and V alike), at block_mapping[t],
+ * slot_mapping[t]:
+ *   amax = max(max_d |x_d|, 2^-100);  scale = amax / Q
+ *   code_d = nearest-even(x_d * (Q / amax));  value_d = code_d * scale
+ * in fp32, Q = 448 for QF_CACHE_E4M3 (codes are e4m3 bytes), 127 for
+ * QF_CACHE_INT8 (signed bytes).  A row with an infinity or a NaN is stored as
+ * codes 0 and scale NaN: it reads back as NaN.
+ * k_src/v_src: (Hkv, T, D) of `dtype`; caches (N, Hkv, B, D) bytes; scales
+ * (N, Hkv, B) fp32; all strides in elements, any values.  The (block, slot)
+ * pairs of one call must be distinct: of two tokens sent to one slot, the row
+ * and its scale may come from different ones.  Rows of 64, 128 or 256 that
+ * start on 16-byte boundaries take the vector path. */
+int qf_kv_store_quantized(const void* k_src, const int64_t k_src_strides[3],
+                          const void* v_src, const int64_t v_src_strides[3],
+                          void* k_cache, const int64_t k_cache_strides[4],
+                          void* v_cache, const int64_t v_cache_strides[4],
+                          float* k_scale, const int64_t k_scale_strides[3],
+                          float* v_scale, const int64_t v_scale_strides[3],
+                          const void* block_mapping, const void* slot_mapping, int index_type,
+                          int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
+                          int64_t num_blocks, int64_t block_size, int dtype, int format,
+                          int32_t* status, cudaStream_t stream);
+
+/* The rows back: k_out/v_out[h, t, :] = rnd(code * scale) of the row at
+ * (block_mapping[t], slot_mapping[t]), in `dtype`.  A place outside the cache
+ * reads as a zero row and is flagged. */
+int qf_kv_load_quantized(const void* k_cache, const int64_t k_cache_strides[4],
+                         const void* v_cache, const int64_t v_cache_strides[4],
+                         const float* k_scale, const int64_t k_scale_strides[3],
+                         const float* v_scale, const int64_t v_scale_strides[3],
+                         const void* block_mapping, const void* slot_mapping, int index_type,
+                         void* k_out, const int64_t k_out_strides[3],
+                         void* v_out, const int64_t v_out_strides[3],
+                         int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
+                         int64_t num_blocks, int64_t block_size, int dtype, int format,
+                         int32_t* status, cudaStream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Attention of several new tokens per sequence over the paged cache, for the
+ * verification of a tree of drafted tokens; and decode over a quantised cache.
+ * No counterpart in the reference.  Sequence s owns query rows
+ * [cu_seqlens_q[s], cu_seqlens_q[s + 1]), its n_s drafted tokens, whose K and
+ * V are in the cache already, behind the context_lens[s] tokens before them.
+ * Query t sees every context key, and drafted key i (key context + i) iff bit
+ * i % 64 of tree_mask[t, i / 64] is set:
+ *   out[t, h] = softmax(q[t, h] . K^T * scale over the keys it sees) @ V
+ * A query that sees no key gives a zero row; so do rows outside every
+ * sequence.  cu_seqlens_q NULL: one query per sequence over its
+ * context_lens[s] keys (decode), num_tokens = num_seqs, no mask.
+ * A key that a query does not see has no part in its row, whatever the key's
+ * K and V hold (infinities and NaN too).
+ * q, out: (T, Hq, D), token and head strides, head_dim contiguous, rows of q
+ * 16-byte aligned; caches (N, Hkv, B, D) with equal strides, head_dim
+ * contiguous, rows 16-byte aligned (`cache_format` says what they hold); scales
+ * (N, Hkv, B), equal strides, for the quantised formats; block_tables int32
+ * rows; context_lens, cu_seqlens_q int32; tree_mask (T, mask_words) int64.
+ * head_dim 64, 128 or 256; any Hq / Hkv; block tables of at most 2^30 keys a row.
+ * A block index outside the cache leaves its keys out (QF_FLAG_BAD_BLOCK);
+ * context + drafts longer than the block table's row, a negative length, or
+ * cu_seqlens_q that leave [0, num_tokens] are cut (QF_FLAG_BAD_TABLE); drafted
+ * tokens past max_tree give zero rows (QF_FLAG_BAD_TREE).
+ * workspace: fp32 scratch, at least qf_paged_tree_attention_workspace_bytes
+ * (of the same arguments), 16-byte aligned, its contents of no account; NULL runs
+ * each sequence in one piece. Calls that may overlap need workspaces of their own. */
+typedef struct {
+    const void* q; int64_t q_stride_token, q_stride_head;
+    const void* k_cache; const void* v_cache; int64_t cache_strides[4];
+    const float* k_scale; const float* v_scale; int64_t scale_strides[3];
+    int64_t num_blocks, block_size;
+    const int32_t* block_tables; int64_t block_tables_row_stride, max_blocks_per_seq;
+    const int32_t* context_lens;
+    const int32_t* cu_seqlens_q;
+    const int64_t* tree_mask; int64_t mask_words;
+    int64_t num_seqs, num_tokens, max_tree, num_q_heads, num_kv_heads, head_dim;
+    float scale;
+    void* out; int64_t out_stride_token, out_stride_head;
+    void* workspace; int64_t workspace_bytes;
+    int dtype; int cache_format;
+    int32_t* status;
+} qf_paged_tree_attention_args;
+
+int qf_paged_tree_attention(const qf_paged_tree_attention_args* args, cudaStream_t stream);
+
+/* Workspace bytes that let qf_paged_tree_attention split long sequences over
+ * several CTAs (0: nothing to split).  Reads sizes, dtype and cache_format only. */
+size_t qf_paged_tree_attention_workspace_bytes(const qf_paged_tree_attention_args* args);
+
+/* sizeof(qf_paged_tree_attention_args) as compiled into the library. */
+size_t qf_paged_tree_attention_args_size(void);
+
+/* Visibility of a tree's nodes from their parents.  Sequence s owns nodes
+ * [cu_seqlens[s], cu_seqlens[s + 1]); parents[t] is the index, within the
+ * sequence, of an earlier node, or -1 for a child of the context's last token:
+ *   mask[t, i / 64] bit i % 64 = node i is t or an ancestor of t
+ *   depths[t] = number of t's ancestors
+ * so that context_lens[s] + depths[t] is the node's position.  parents: int32
+ * or int64; mask: (num_nodes, mask_words) int64, mask_words >= max_tree / 64
+ * rounded up; depths int32.  A parent that is no earlier node is read as -1, nodes past max_tree
+ * get an empty mask and depth 0 (QF_FLAG_BAD_TREE); nodes outside every sequence likewise
+ * (unflagged: a padded batch). */
+int qf_build_tree_mask(const void* parents, int index_type, const int32_t* cu_seqlens,
+                       int64_t num_seqs, int64_t num_nodes, int64_t max_tree, int64_t mask_words,
+                       int64_t* mask, int32_t* depths, int32_t* status, cudaStream_t stream);
 
 /* ---------------------------------------------------------------------- */
 /* Prefill attention over variable-length packed sequences.  Replaces

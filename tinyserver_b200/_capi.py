@@ -25,12 +25,16 @@ QF_OK, QF_ERR_INVALID, QF_ERR_UNSUPPORTED, QF_ERR_LAUNCH, QF_ERR_DEVICE = 0, 1, 
 QF_ERR_SCRATCH = 5
 QF_FLAG_BAD_BLOCK, QF_FLAG_BAD_SLOT, QF_FLAG_BAD_TOKEN, QF_FLAG_BAD_TABLE = 1, 2, 4, 8
 QF_FLAG_TIMEOUT = 16
+QF_FLAG_BAD_TREE = 32
+QF_CACHE_PLAIN, QF_CACHE_E4M3, QF_CACHE_INT8 = 0, 1, 2
 
 FLAG_NAMES = {QF_FLAG_BAD_BLOCK: "block index outside the cache",
               QF_FLAG_BAD_SLOT: "slot index outside the block",
               QF_FLAG_BAD_TOKEN: "token id outside the vocabulary",
               QF_FLAG_BAD_TABLE: "position beyond the block table",
-              QF_FLAG_TIMEOUT: "a kernel timed out waiting on its tensor-core work"}
+              QF_FLAG_TIMEOUT: "a kernel timed out waiting on its tensor-core work",
+              QF_FLAG_BAD_TREE: "a tree node's parent is no earlier node, or the tree exceeds "
+                                "max_tree"}
 
 
 class QkNormRopeArgs(ctypes.Structure):
@@ -71,6 +75,28 @@ class PagedAttentionArgs(ctypes.Structure):
         ("out", c_vp), ("out_stride_seq", c_i64), ("out_stride_head", c_i64),
         ("workspace", c_vp), ("workspace_bytes", c_i64),
         ("dtype", c_int),
+        ("status", c_vp),
+    ]
+
+
+class PagedTreeAttentionArgs(ctypes.Structure):
+    """Mirror of qf_paged_tree_attention_args (field order and types must match)."""
+
+    _fields_ = [
+        ("q", c_vp), ("q_stride_token", c_i64), ("q_stride_head", c_i64),
+        ("k_cache", c_vp), ("v_cache", c_vp), ("cache_strides", c_i64 * 4),
+        ("k_scale", c_vp), ("v_scale", c_vp), ("scale_strides", c_i64 * 3),
+        ("num_blocks", c_i64), ("block_size", c_i64),
+        ("block_tables", c_vp), ("block_tables_row_stride", c_i64),
+        ("max_blocks_per_seq", c_i64),
+        ("context_lens", c_vp), ("cu_seqlens_q", c_vp),
+        ("tree_mask", c_vp), ("mask_words", c_i64),
+        ("num_seqs", c_i64), ("num_tokens", c_i64), ("max_tree", c_i64),
+        ("num_q_heads", c_i64), ("num_kv_heads", c_i64), ("head_dim", c_i64),
+        ("scale", c_float),
+        ("out", c_vp), ("out_stride_token", c_i64), ("out_stride_head", c_i64),
+        ("workspace", c_vp), ("workspace_bytes", c_i64),
+        ("dtype", c_int), ("cache_format", c_int),
         ("status", c_vp),
     ]
 
@@ -135,6 +161,16 @@ SIGNATURES: dict[str, list] = {
     "qf_paged_attention_args_size": [],
     "qf_paged_attention_decode_noalloc": [ctypes.POINTER(PagedAttentionArgs), c_vp],
     "qf_paged_attention_noalloc_capacity": [],
+    "qf_kv_store_quantized": [c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp,
+                              I64P, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_int,
+                              c_int, c_vp, c_vp],
+    "qf_kv_load_quantized": [c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp, c_vp, c_int,
+                             c_vp, I64P, c_vp, I64P, c_i64, c_i64, c_i64, c_i64, c_i64, c_int,
+                             c_int, c_vp, c_vp],
+    "qf_paged_tree_attention": [ctypes.POINTER(PagedTreeAttentionArgs), c_vp],
+    "qf_paged_tree_attention_workspace_bytes": [ctypes.POINTER(PagedTreeAttentionArgs)],
+    "qf_paged_tree_attention_args_size": [],
+    "qf_build_tree_mask": [c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp],
     "qf_varlen_attention": [ctypes.POINTER(VarlenAttentionArgs), c_vp],
     "qf_varlen_attention_args_size": [],
     "qf_sample_tokens": [ctypes.POINTER(SampleArgs), c_vp],
@@ -149,6 +185,8 @@ RESTYPES = {"qf_last_cuda_error": ctypes.c_char_p, "qf_version": ctypes.c_char_p
             "qf_qk_norm_rope_args_size": ctypes.c_size_t,
             "qf_paged_attention_args_size": ctypes.c_size_t,
             "qf_paged_attention_workspace_bytes": ctypes.c_size_t,
+            "qf_paged_tree_attention_workspace_bytes": ctypes.c_size_t,
+            "qf_paged_tree_attention_args_size": ctypes.c_size_t,
             "qf_paged_attention_noalloc_capacity": ctypes.c_size_t,
             "qf_sample_workspace_bytes": c_i64,
             "qf_varlen_attention_args_size": ctypes.c_size_t,
@@ -181,6 +219,7 @@ def lib() -> ctypes.CDLL:
                 fn.restype = RESTYPES.get(name, c_int)
             for fn, mirror in (("qf_qk_norm_rope_args_size", QkNormRopeArgs),
                                ("qf_paged_attention_args_size", PagedAttentionArgs),
+                               ("qf_paged_tree_attention_args_size", PagedTreeAttentionArgs),
                                ("qf_varlen_attention_args_size", VarlenAttentionArgs),
                                ("qf_sample_args_size", SampleArgs)):
                 size = getattr(handle, fn)()

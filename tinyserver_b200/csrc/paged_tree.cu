@@ -1,0 +1,542 @@
+// Attention of several new tokens per sequence over the paged cache (a tree of
+// drafted tokens), and decode over a quantised cache: entry points, the fp32
+// kernel, the merge of split sequences, and the trees' visibility masks.
+//
+//   out[t, h] = softmax(q[t, h] . K^T * scale over the keys t sees) @ V
+// in one pass over the keys with a running maximum m and sum l per row
+// (scores in units of log2, so exp is 2^x).  The rows of one kv head are its
+// G = Hq / Hkv query heads of every query token, r = token * G + head: they all
+// read the same K and V, so a sequence's cache crosses HBM once per row tile.
+//
+// Which kernel:
+//  * float32: the CUDA-core kernel here (any cache format);
+//  * 16-bit: paged_tree_mma.cu (mma.sync, operands straight from global memory).
+#include <math.h>
+
+#include "qf_mma.cuh"
+#include "qf_quant.cuh"
+#include "qf_tree.cuh"
+
+namespace qf {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMmaRows = 16;
+constexpr int kMinPart = 256, kMaxPart = 1 << 30;  // keys of a partition
+
+// ---------------------------------------------------------------------------
+// fp32.  A CTA of 4 warps takes NR = 4 WR rows and steps through tiles of 32
+// keys in shared memory, as floats (codes are decoded on the way in).  WR warps
+// divide the rows, 4 / WR the keys of a tile: 4 x 1 for many rows, 1 x 4 for a
+// decode step's few.  QK: a lane owns one key and 4 rows (or 1 of each),
+// reading K by 16 bytes from rows padded to D + 4 floats and q as a broadcast;
+// PV: a lane owns D / 32 output columns.  Bound by shared-memory reads (5
+// 16-byte reads for 16 multiply-adds a lane).
+template <int FMT, int D, int WR>
+struct F32Tile {
+    static constexpr int WK = 4 / WR, NR = 4 * WR, KW = 32 / WK, KROW = D + 4;
+    static constexpr int Q = NR * D, K = 32 * KROW, V = 32 * D, PS = 4 * 4 * KW;
+    static constexpr int FLOATS = Q + K + V + PS + 4 * 4 + 32;
+    static_assert(WK * NR * D + 2 * WK * NR <= K + V, "merge area");
+};
+
+// 16 bytes' worth of a cache row as floats: 4 fp32 elements or 16 codes.
+template <int FMT>
+__device__ __forceinline__ void decode16(const uint4& v, float scale, float* f) {
+    if constexpr (FMT == QF_CACHE_PLAIN) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(word(v, i));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) codes_to_float<FMT>(word(v, i), f + 4 * i);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] *= scale;
+    }
+}
+
+template <int FMT, int D, int WR>
+__global__ void __launch_bounds__(128) tree_f32_kernel(const TreeDev a) {
+    using FT = F32Tile<FMT, D, WR>;
+    constexpr int WK = FT::WK, NR = FT::NR, KW = FT::KW, KROW = FT::KROW, PER = D / 32;
+    constexpr int EB = FMT == QF_CACHE_PLAIN ? 4 : 1, EPC = 16 / EB;
+    const int p = blockIdx.x, s = blockIdx.z;
+    const int g = blockIdx.y % a.Hkv, rg = blockIdx.y / a.Hkv;
+    const TreeSeq w = tree_seq(a, s);
+    if (p == 0 && rg == 0) zero_unowned_rows<float, D>(a, s, g, w);
+    const int rows = w.n * a.G, r0 = rg * NR;
+    if (p >= w.nparts || r0 >= rows) return;
+    const int k_begin = p * a.part, k_end = k_begin + min(w.L - k_begin, a.part);
+
+    extern __shared__ __align__(16) float fsm[];
+    float* qs = fsm;
+    float* kt = qs + FT::Q;
+    float* vt = kt + FT::K;
+    float* ps = vt + FT::V;     // [4 warps][4 rows][KW]
+    float* corr = ps + FT::PS;  // [4 warps][4 rows]
+    int* kval = reinterpret_cast<int*>(corr + 16);
+
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int wr = warp % WR, wk = warp / WR;
+    for (int i = tid; i < NR * D; i += 128) {
+        const int r = r0 + i / D, d = i % D;
+        qs[i] = r < rows ? reinterpret_cast<const float*>(a.q)[(int64_t)(w.q0 + r / a.G) * a.qt +
+                                                               (int64_t)(g * a.G + r % a.G) * a.qh + d]
+                         : 0.f;
+    }
+    const int32_t* bt = a.bt + (int64_t)s * a.bts;
+    const float sl2 = a.scale * kLog2e;
+    constexpr int NS = 4 * KW / 32;  // scores per lane
+    float m[NS], l[NS], acc[4][PER];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[i][e] = 0.f;
+
+    for (int j0 = k_begin; j0 < k_end; j0 += 32) {
+        __syncthreads();  // the tile before this one has been read
+        {
+            const int kk = tid >> 2, part = tid & 3, j = j0 + kk;
+            int64_t row = 0, srow = 0;
+            const bool ok = j < k_end && key_place(a, bt, g, j, row, srow);
+            float ksc = 1.f, vsc = 1.f;
+            if (FMT != QF_CACHE_PLAIN && ok) {
+                ksc = __ldg(a.ks + srow);
+                vsc = __ldg(a.vs + srow);
+            }
+            if (part == 0) kval[kk] = ok;
+#pragma unroll
+            for (int c = part; c < D / EPC; c += 4) {
+                float f[EPC];
+                const uint4 z = make_uint4(0, 0, 0, 0);
+                decode16<FMT>(ok ? ld_shared_ro16(a.kc + (row + c * EPC) * EB) : z, ksc, f);
+#pragma unroll
+                for (int e = 0; e < EPC; e += 4)
+                    *reinterpret_cast<float4*>(kt + kk * KROW + c * EPC + e) =
+                        make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                decode16<FMT>(ok ? ld_shared_ro16(a.vc + (row + c * EPC) * EB) : z, vsc, f);
+#pragma unroll
+                for (int e = 0; e < EPC; e += 4)
+                    *reinterpret_cast<float4*>(vt + kk * D + c * EPC + e) =
+                        make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            }
+        }
+        __syncthreads();
+        const bool draft = a.cu && j0 + 32 > w.ctx;
+        const int key = wk * KW + (NS == 4 ? lane : lane % KW);
+        float sc[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) sc[i] = 0.f;
+        const int row0 = wr * 4 + (NS == 4 ? 0 : lane / KW);  // this lane's first row in the CTA
+        const float* kr = kt + key * KROW;
+#pragma unroll 4
+        for (int d = 0; d < D; d += 4) {
+            const float4 kv = *reinterpret_cast<const float4*>(kr + d);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const float4 qv = *reinterpret_cast<const float4*>(qs + (row0 + i) * D + d);
+                sc[i] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, sc[i]))));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int r = r0 + row0 + i;
+            bool sees = kval[key] && r < rows;
+            if (draft && sees)
+                sees = (tree_bits32(a.mask + (int64_t)(w.q0 + r / a.G) * a.words, a.words,
+                                    j0 - w.ctx) >> key) & 1;
+            const float t = sees ? sc[i] * sl2 : -INFINITY;
+            float mx = t;
+#pragma unroll
+            for (int o = KW / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;
+            const float c = exp2f(m[i] - base);
+            const float pr = exp2f(t - base);
+            m[i] = mn;
+            l[i] = l[i] * c + pr;  // this lane's part of the row's sum
+            const int ri = NS == 4 ? i : lane / KW;
+            ps[(warp * 4 + ri) * KW + (NS == 4 ? lane : lane % KW)] = sees ? pr : -1.f;
+            if ((NS == 4 ? lane : lane % KW) == 0) corr[warp * 4 + ri] = c;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float c = corr[warp * 4 + i];
+#pragma unroll
+            for (int e = 0; e < PER; ++e) acc[i][e] *= c;
+        }
+        // A key that a row does not see carries p = -1 and is left out of the
+        // row: 0 times an infinity or a NaN in its V would not be 0.  (A key
+        // with no place has zeros for V; rows past the last are never stored.)
+        for (int kk = 0; kk < KW; ++kk) {
+            float v[PER];
+#pragma unroll
+            for (int e = 0; e < PER; ++e)
+                v[e] = vt[(wk * KW + kk) * D + (PER == 2 ? lane * 2 + e : (e / 4) * 128 + lane * 4 + e % 4)];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float pr = ps[(warp * 4 + i) * KW + kk];
+                if (pr >= 0.f || isnan(pr)) {
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) acc[i][e] = fmaf(pr, v[e], acc[i][e]);
+                }
+            }
+        }
+        __syncwarp();
+    }
+    // rows' sums over the lanes of a row, then the warps that share rows
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int o = KW / 2; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+    __syncthreads();
+    float* wacc = kt;  // [WK][NR][D], then max and sum [WK][NR]
+    float* wm = wacc + WK * NR * D;
+    float* wl = wm + WK * NR;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int ri = wr * 4 + (NS == 4 ? i : lane / KW);
+        if ((NS == 4 ? lane : lane % KW) == 0) {
+            wm[wk * NR + ri] = m[i];
+            wl[wk * NR + ri] = l[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+            wacc[(wk * NR + wr * 4 + i) * D +
+                 (PER == 2 ? lane * 2 + e : (e / 4) * 128 + lane * 4 + e % 4)] = acc[i][e];
+    __syncthreads();
+    for (int i = tid; i < NR * D; i += 128) {
+        const int ri = i / D, d = i % D, r = r0 + ri;
+        if (r >= rows) break;
+        float M = -INFINITY, Ls = 0.f, A = 0.f;
+#pragma unroll
+        for (int k = 0; k < WK; ++k) M = fmaxf(M, wm[k * NR + ri]);
+#pragma unroll
+        for (int k = 0; k < WK; ++k) {
+            const float f = M == -INFINITY ? 0.f : exp2f(wm[k * NR + ri] - M);
+            Ls += wl[k * NR + ri] * f;
+            A += wacc[(k * NR + ri) * D + d] * f;
+        }
+        const int64_t t = w.q0 + r / a.G, h = g * a.G + r % a.G;
+        if (w.nparts == 1) {
+            reinterpret_cast<float*>(a.out)[t * a.ot + h * a.oh + d] = Ls == 0.f ? 0.f : A / Ls;
+        } else {
+            float* o = a.ws + ((t * a.Hq + h) * a.P + p) * (D + 2);
+            o[d] = A;
+            if (d == 0) {
+                o[D] = M;
+                o[D + 1] = Ls;
+            }
+        }
+    }
+}
+
+template <int FMT, int D, int WR>
+int launch_f32(const TreeDev& a, cudaStream_t stream) {
+    constexpr auto kernel = tree_f32_kernel<FMT, D, WR>;
+    constexpr int smem = F32Tile<FMT, D, WR>::FLOATS * 4;
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return launch_failed(e);
+    const int64_t groups = ceil_div((int64_t)a.max_tree * a.G, 4 * WR);
+    if (groups * a.Hkv > 65535) return QF_ERR_UNSUPPORTED;
+    kernel<<<dim3((unsigned)a.P, (unsigned)(groups * a.Hkv), (unsigned)a.S), 128, smem, stream>>>(a);
+    return check_launch();
+}
+
+template <int FMT, int D>
+int launch_f32(const TreeDev& a, cudaStream_t stream) {
+    return a.max_tree * a.G <= 4 ? launch_f32<FMT, D, 1>(a, stream) : launch_f32<FMT, D, 4>(a, stream);
+}
+
+template <int FMT>
+int launch_f32(const TreeDev& a, int D, cudaStream_t stream) {
+    switch (D) {
+    case 64: return launch_f32<FMT, 64>(a, stream);
+    case 128: return launch_f32<FMT, 128>(a, stream);
+    default: return launch_f32<FMT, 256>(a, stream);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Join the partitions of sequences longer than one: a warp per (token, head)
+// row, partials in the workspace as (acc[D], max in log2 units, sum).
+template <typename T, int D>
+__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeDev a) {
+    pdl_wait();
+    const int h = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const TreeSeq w = tree_seq(a, blockIdx.z);
+    if (h >= a.Hq || (int)blockIdx.y >= w.n || w.nparts == 1) return;
+    const int64_t t = w.q0 + blockIdx.y;
+    const float* ws = a.ws + (t * a.Hq + h) * a.P * (D + 2);
+    float M = -INFINITY;
+    for (int p = lane; p < w.nparts; p += 32) M = fmaxf(M, ws[(int64_t)p * (D + 2) + D]);
+    M = warp_max(M);
+    constexpr int PER = D / 32;
+    float Ls = 0.f, acc[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+#pragma unroll 2
+    for (int p = 0; p < w.nparts; ++p) {
+        const float* wp = ws + (int64_t)p * (D + 2);
+        const float f = M == -INFINITY ? 0.f : exp2f(wp[D] - M);
+        Ls += wp[D + 1] * f;
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(wp + e * 32 + lane * 2);
+            acc[e] += v.x * f;
+            acc[e + 1] += v.y * f;
+        }
+    }
+    T* o = reinterpret_cast<T*>(a.out) + t * a.ot + (int64_t)h * a.oh;
+    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+        o[(e & ~1) * 32 + lane * 2 + (e & 1)] = Dt<T>::from_f(Ls == 0.f ? 0.f : acc[e] * inv);
+}
+
+template <typename T>
+int launch_merge(const TreeDev& a, int D, cudaStream_t stream) {
+    const dim3 grid((unsigned)ceil_div(a.Hq, 4), (unsigned)a.max_tree, (unsigned)a.S);
+    switch (D) {
+    case 64: return launch_pdl(tree_merge_kernel<T, 64>, grid, 128, 0, stream, a);
+    case 128: return launch_pdl(tree_merge_kernel<T, 128>, grid, 128, 0, stream, a);
+    default: return launch_pdl(tree_merge_kernel<T, 256>, grid, 128, 0, stream, a);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// A CTA per sequence, a thread per node: walk from the node to its root.  The
+// walk's indices only fall, so the mask's words come out from the last to the
+// first, each once.  Latency-bound: depth dependent reads, which the first
+// level cache answers.
+__global__ void __launch_bounds__(128)
+    build_tree_mask_kernel(const void* parents, int index_type, const int32_t* cu, int S, int T,
+                           int max_tree, int words, int64_t* mask, int32_t* depths, int32_t* status) {
+    const int s = blockIdx.x;
+    const int b = min(max(__ldg(cu + s), 0), T), e = min(max(__ldg(cu + s + 1), b), T);
+    auto empty = [&](int t0, int t1) {
+        for (int t = t0 + (int)threadIdx.x; t < t1; t += blockDim.x) {
+            for (int i = 0; i < words; ++i) mask[(int64_t)t * words + i] = 0;
+            depths[t] = 0;
+        }
+    };
+    if (s == 0) empty(0, b);
+    if (s == S - 1) empty(e, T);
+    if (e - b > max_tree) {
+        if (threadIdx.x == 0) flag(status, QF_FLAG_BAD_TREE);
+        empty(b + max_tree, e);
+    }
+    for (int i = threadIdx.x; i < min(e - b, max_tree); i += blockDim.x) {
+        int64_t* row = mask + (int64_t)(b + i) * words;
+        int node = i, depth = -1, word = words - 1;
+        uint64_t bits = 0;
+        while (node >= 0) {
+            for (; word > (node >> 6); --word) {
+                row[word] = (int64_t)bits;
+                bits = 0;
+            }
+            bits |= 1ull << (node & 63);
+            ++depth;
+            const int64_t up = load_index(parents, (int64_t)b + node, index_type);
+            if (up < -1 || up >= node) {
+                flag(status, QF_FLAG_BAD_TREE);
+                node = -1;
+            } else {
+                node = (int)up;
+            }
+        }
+        for (; word >= 0; --word) {
+            row[word] = (int64_t)bits;
+            bits = 0;
+        }
+        depths[b + i] = depth;
+    }
+}
+
+// ---------------------------------------------------------------------------
+struct TreePlan {
+    int part, P;
+    int64_t rows;  // rows of one kv head in the longest tree
+};
+
+// Keys per partition.  Splitting costs a partial of (D + 2) floats a row,
+// written and read back, so the sequences are split only until the grid has
+// some `kWaves` times as many CTAs as fit on the GPU, and never below kMinPart keys.
+TreePlan make_plan(const qf_paged_tree_attention_args& g) {
+    TreePlan p{};
+    const int64_t G = g.num_q_heads / g.num_kv_heads, nq = g.cu_seqlens_q ? g.max_tree : 1;
+    p.rows = nq * G;
+    int64_t per_cta = kMmaRows;
+    const int64_t slots = (int64_t)sm_count() * 3;
+    if (g.dtype == QF_F32) {
+        per_cta = p.rows <= 4 ? 4 : 16;
+    } else if (g.head_dim == 256 || p.rows <= 8) {
+        per_cta = 8;
+    }
+    const int64_t ctas = std::max<int64_t>(1, g.num_seqs * g.num_kv_heads * ceil_div(p.rows, per_cta));
+    const int64_t cap = std::max<int64_t>(1, g.max_blocks_per_seq * g.block_size);
+    const int64_t want = std::max<int64_t>(1, 4 * slots / ctas);  // partitions
+    int64_t part = std::max<int64_t>(kMinPart, ceil_div(ceil_div(cap, want), 128) * 128);
+    p.part = (int)std::min<int64_t>(part, kMaxPart);
+    p.P = (int)ceil_div(cap, p.part);
+    return p;
+}
+
+bool known_sizes(const qf_paged_tree_attention_args& g) {
+    return g.num_seqs > 0 && g.num_tokens > 0 && g.num_q_heads > 0 && g.num_kv_heads > 0 &&
+           g.head_dim > 0 && g.block_size > 0 && g.max_blocks_per_seq >= 0 && g.max_tree >= 0 &&
+           g.num_q_heads % g.num_kv_heads == 0 && g.block_size <= (1 << 30) &&
+           g.max_blocks_per_seq <= (1 << 30) / g.block_size;
+}
+
+int check_tree_args(const qf_paged_tree_attention_args& g) {
+    if (g.num_seqs < 0 || g.num_tokens < 0 || g.num_q_heads <= 0 || g.num_kv_heads <= 0 ||
+        g.block_size <= 0 || g.num_blocks < 0 || g.max_blocks_per_seq < 0 || g.max_tree < 0 ||
+        g.mask_words < 0)
+        return QF_ERR_INVALID;
+    if (g.num_q_heads % g.num_kv_heads) return QF_ERR_INVALID;
+    if (g.dtype != QF_F32 && g.dtype != QF_F16 && g.dtype != QF_BF16) return QF_ERR_INVALID;
+    if (g.cache_format != QF_CACHE_PLAIN && g.cache_format != QF_CACHE_E4M3 &&
+        g.cache_format != QF_CACHE_INT8)
+        return QF_ERR_INVALID;
+    if (g.head_dim != 64 && g.head_dim != 128 && g.head_dim != 256) return QF_ERR_UNSUPPORTED;
+    if (g.num_tokens == 0) return QF_OK;
+    if (g.num_seqs == 0) return QF_ERR_INVALID;  // rows that no sequence owns
+    if (!g.q || !g.k_cache || !g.v_cache || !g.context_lens || !g.out ||
+        (g.max_blocks_per_seq > 0 && !g.block_tables))
+        return QF_ERR_INVALID;
+    if (g.cu_seqlens_q) {
+        if (g.max_tree < 1 || !g.tree_mask || g.mask_words < 1) return QF_ERR_INVALID;
+        if (g.mask_words < (g.max_tree + 63) / 64) return QF_ERR_INVALID;
+    } else if (g.num_tokens != g.num_seqs) {
+        return QF_ERR_INVALID;
+    }
+    if (g.cache_format != QF_CACHE_PLAIN && (!g.k_scale || !g.v_scale)) return QF_ERR_INVALID;
+    if (!known_sizes(g) || g.num_seqs > 65535 || g.num_kv_heads > 65535 || g.max_tree > 65535 ||
+        g.mask_words > INT32_MAX || g.num_tokens > INT32_MAX || g.num_q_heads > (1 << 20))
+        return QF_ERR_UNSUPPORTED;
+    const int64_t es = g.dtype == QF_F32 ? 4 : 2, cs = g.cache_format == QF_CACHE_PLAIN ? es : 1;
+    // q rows and cache rows are read in 16-byte chunks
+    if ((g.q_stride_token * es) % 16 || (g.q_stride_head * es) % 16 || !aligned16(g.q) ||
+        (g.cache_strides[0] * cs) % 16 || (g.cache_strides[1] * cs) % 16 ||
+        (g.cache_strides[2] * cs) % 16 || g.cache_strides[3] != 1 || !aligned16(g.k_cache) ||
+        !aligned16(g.v_cache) || !aligned16(g.workspace))
+        return QF_ERR_UNSUPPORTED;
+    return QF_OK;
+}
+
+size_t plan_bytes(const qf_paged_tree_attention_args& g, const TreePlan& p) {
+    if (p.P <= 1) return 0;
+    int64_t n = 0;
+    if (__builtin_mul_overflow(g.num_tokens, g.num_q_heads, &n) ||
+        __builtin_mul_overflow(n, (int64_t)p.P, &n) ||
+        __builtin_mul_overflow(n, (g.head_dim + 2) * (int64_t)sizeof(float), &n))
+        return SIZE_MAX;
+    return (size_t)n;
+}
+
+int launch_tree_f32(const TreeDev& a, int format, int D, cudaStream_t stream) {
+    switch (format) {
+    case QF_CACHE_PLAIN: return launch_f32<QF_CACHE_PLAIN>(a, D, stream);
+    case QF_CACHE_E4M3: return launch_f32<QF_CACHE_E4M3>(a, D, stream);
+    default: return launch_f32<QF_CACHE_INT8>(a, D, stream);
+    }
+}
+
+}  // namespace
+}  // namespace qf
+
+extern "C" size_t qf_paged_tree_attention_workspace_bytes(const qf_paged_tree_attention_args* p) {
+    if (!p || !qf::known_sizes(*p)) return 0;
+    return qf::plan_bytes(*p, qf::make_plan(*p));
+}
+
+extern "C" size_t qf_paged_tree_attention_args_size(void) {
+    return sizeof(qf_paged_tree_attention_args);
+}
+
+extern "C" int qf_paged_tree_attention(const qf_paged_tree_attention_args* p, cudaStream_t stream) {
+    if (!p) return QF_ERR_INVALID;
+    const qf_paged_tree_attention_args& g = *p;
+    int rc = qf::check_tree_args(g);
+    if (rc || g.num_tokens == 0) return rc;
+    qf::TreePlan plan = qf::make_plan(g);
+    const size_t need = qf::plan_bytes(g, plan);
+    if (need > 0 && g.workspace) {
+        if (g.workspace_bytes < 0 || (size_t)g.workspace_bytes < need) return QF_ERR_INVALID;
+    } else {
+        plan.P = 1;
+        plan.part = qf::kMaxPart;
+    }
+    qf::TreeDev a{};
+    a.q = static_cast<const char*>(g.q);
+    a.qt = g.q_stride_token;
+    a.qh = g.q_stride_head;
+    a.kc = static_cast<const char*>(g.k_cache);
+    a.vc = static_cast<const char*>(g.v_cache);
+    a.c0 = g.cache_strides[0];
+    a.c1 = g.cache_strides[1];
+    a.c2 = g.cache_strides[2];
+    a.ks = g.k_scale;
+    a.vs = g.v_scale;
+    a.s0 = g.scale_strides[0];
+    a.s1 = g.scale_strides[1];
+    a.s2 = g.scale_strides[2];
+    a.N = g.num_blocks;
+    a.B = qf::FastDiv((int)g.block_size);
+    a.bt = g.block_tables;
+    a.bts = g.block_tables_row_stride;
+    a.cap = (int)(g.max_blocks_per_seq * g.block_size);
+    a.lens = g.context_lens;
+    a.cu = g.cu_seqlens_q;
+    a.mask = g.tree_mask;
+    a.words = (int)g.mask_words;
+    a.S = (int)g.num_seqs;
+    a.T = (int)g.num_tokens;
+    a.max_tree = g.cu_seqlens_q ? (int)g.max_tree : 1;
+    a.Hq = (int)g.num_q_heads;
+    a.Hkv = (int)g.num_kv_heads;
+    a.G = a.Hq / a.Hkv;
+    a.scale = g.scale;
+    a.out = static_cast<char*>(g.out);
+    a.ot = g.out_stride_token;
+    a.oh = g.out_stride_head;
+    a.ws = static_cast<float*>(g.workspace);
+    a.P = plan.P;
+    a.part = plan.part;
+    a.status = g.status;
+    const int D = (int)g.head_dim;
+    if (g.dtype == QF_F32)
+        rc = qf::launch_tree_f32(a, g.cache_format, D, stream);
+    else
+        rc = qf::launch_tree_mma(a, g.dtype, g.cache_format, D, (int)plan.rows, stream);
+    if (rc || a.P == 1) return rc;
+    switch (g.dtype) {
+    case QF_F32: return qf::launch_merge<float>(a, D, stream);
+    case QF_F16: return qf::launch_merge<__half>(a, D, stream);
+    default: return qf::launch_merge<__nv_bfloat16>(a, D, stream);
+    }
+}
+
+extern "C" int qf_build_tree_mask(const void* parents, int index_type, const int32_t* cu_seqlens,
+                                  int64_t num_seqs, int64_t num_nodes, int64_t max_tree,
+                                  int64_t mask_words, int64_t* mask, int32_t* depths, int32_t* status,
+                                  cudaStream_t stream) {
+    if (num_seqs < 0 || num_nodes < 0 || max_tree < 1 || mask_words < 1) return QF_ERR_INVALID;
+    if (index_type != QF_I32 && index_type != QF_I64) return QF_ERR_INVALID;
+    if (mask_words < (max_tree + 63) / 64) return QF_ERR_INVALID;
+    if (num_nodes == 0) return QF_OK;
+    if (num_seqs == 0 || !parents || !cu_seqlens || !mask || !depths) return QF_ERR_INVALID;
+    if (num_seqs > INT32_MAX || num_nodes > INT32_MAX || max_tree > INT32_MAX ||
+        mask_words > INT32_MAX)
+        return QF_ERR_UNSUPPORTED;
+    qf::build_tree_mask_kernel<<<(unsigned)num_seqs, 128, 0, stream>>>(
+        parents, index_type, cu_seqlens, (int)num_seqs, (int)num_nodes, (int)max_tree,
+        (int)mask_words, mask, depths, status);
+    return qf::check_launch();
+}

@@ -188,6 +188,84 @@ def _(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal,
     return torch.empty_like(q if q.stride(2) == 1 else q.contiguous())
 
 
+# ---------------------------------------------------------------------------
+# the quantised cache, and attention for drafted token trees
+@torch.library.custom_op(f"{NS}::store_kv_cache_quantized",
+                         mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"))
+def store_kv_cache_quantized(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: torch.Tensor,
+                             v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                             block_mapping: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    K.store_kv_cache_quantized(k_src, v_src, k_cache, v_cache, k_scale, v_scale, block_mapping,
+                               slot_mapping)
+
+
+@store_kv_cache_quantized.register_fake
+def _(k_src, v_src, k_cache, v_cache, k_scale, v_scale, block_mapping, slot_mapping):
+    return None
+
+
+@torch.library.custom_op(f"{NS}::load_kv_cache_quantized", mutates_args=())
+def load_kv_cache_quantized(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                            v_scale: torch.Tensor, block_mapping: torch.Tensor,
+                            slot_mapping: torch.Tensor, dtype: torch.dtype
+                            ) -> tuple[torch.Tensor, torch.Tensor]:
+    return K.load_kv_cache_quantized(k_cache, v_cache, k_scale, v_scale, block_mapping,
+                                     slot_mapping, dtype)
+
+
+@load_kv_cache_quantized.register_fake
+def _(k_cache, v_cache, k_scale, v_scale, block_mapping, slot_mapping, dtype):
+    shape = (block_mapping.numel(), k_cache.shape[1], k_cache.shape[3])
+    return (k_cache.new_empty(shape, dtype=dtype).transpose(0, 1),
+            k_cache.new_empty(shape, dtype=dtype).transpose(0, 1))
+
+
+@torch.library.custom_op(f"{NS}::paged_attention_quantized", mutates_args=())
+def paged_attention_quantized(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                              k_scale: torch.Tensor, v_scale: torch.Tensor,
+                              block_tables: torch.Tensor, block_size: int, seq_lens: torch.Tensor,
+                              softmax_scale: float | None = None) -> torch.Tensor:
+    return K.paged_attention_quantized(query, k_cache, v_cache, k_scale, v_scale, block_tables,
+                                       block_size, seq_lens, softmax_scale=softmax_scale)
+
+
+@paged_attention_quantized.register_fake
+def _(query, k_cache, v_cache, k_scale, v_scale, block_tables, block_size, seq_lens,
+      softmax_scale=None):
+    return query.new_empty(query.shape)
+
+
+@torch.library.custom_op(f"{NS}::build_tree_mask", mutates_args=())
+def build_tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor,
+                    max_tree: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return K.build_tree_mask(parents, cu_seqlens, max_tree)
+
+
+@build_tree_mask.register_fake
+def _(parents, cu_seqlens, max_tree):
+    n = parents.numel()
+    return (parents.new_empty(n, (max_tree + 63) // 64, dtype=torch.int64),
+            parents.new_empty(n, dtype=torch.int32))
+
+
+@torch.library.custom_op(f"{NS}::paged_tree_attention", mutates_args=())
+def paged_tree_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         block_tables: torch.Tensor, block_size: int, context_lens: torch.Tensor,
+                         cu_seqlens: torch.Tensor, tree_mask: torch.Tensor, max_tree: int,
+                         k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                         softmax_scale: float | None = None) -> torch.Tensor:
+    return K.paged_tree_attention(query, k_cache, v_cache, block_tables, block_size, context_lens,
+                                  cu_seqlens, tree_mask, max_tree, k_scale=k_scale,
+                                  v_scale=v_scale, softmax_scale=softmax_scale)
+
+
+@paged_tree_attention.register_fake
+def _(query, k_cache, v_cache, block_tables, block_size, context_lens, cu_seqlens, tree_mask,
+      max_tree, k_scale=None, v_scale=None, softmax_scale=None):
+    return query.new_empty(query.shape)
+
+
+# ---------------------------------------------------------------------------
 @torch.library.custom_op(f"{NS}::sample_tokens", mutates_args=())
 def sample_tokens(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
                   top_p: torch.Tensor, uniforms: torch.Tensor) -> torch.Tensor:
@@ -224,4 +302,6 @@ def _(seeds, steps):
 OPS = ("embedding", "rms_norm", "fused_add_rms_norm", "silu_and_mul", "rope_cos_sin",
        "qk_norm_rope_store", "apply_rotary_pos_emb", "store_kv_cache_batched", "store_kv_cache",
        "build_slot_mapping", "paged_attention_forward", "flash_attn_varlen_func",
+       "store_kv_cache_quantized", "load_kv_cache_quantized", "paged_attention_quantized",
+       "build_tree_mask", "paged_tree_attention",
        "sample_tokens", "sample_tokens_seeded", "uniforms_from_seeds")
