@@ -329,7 +329,7 @@ int qf_kv_load_quantized(const void* k_cache, const int64_t k_cache_strides[4],
  * context_lens[s] keys (decode), num_tokens = num_seqs, no mask.
  * A key that a query does not see has no part in its row, whatever the key's
  * K and V hold (infinities and NaN too).
- * q, out: (T, Hq, D), token and head strides, head_dim contiguous, rows of q
+ * q, out: (T, Hq, D), token and head strides, head_dim contiguous, rows
  * 16-byte aligned; caches (N, Hkv, B, D) with equal strides, head_dim
  * contiguous, rows 16-byte aligned (`cache_format` says what they hold); scales
  * (N, Hkv, B), equal strides, for the quantised formats; block_tables int32

@@ -10,7 +10,9 @@
 //
 // Which kernel:
 //  * float32: the CUDA-core kernel here (any cache format);
-//  * 16-bit: paged_tree_mma.cu (mma.sync, operands straight from global memory).
+//  * 16-bit, up to kMmaRows rows, or head_dim 64 / 256: paged_tree_mma.cu
+//    (mma.sync, operands straight from global memory);
+//  * 16-bit, head_dim 128, more rows: paged_tree_tc.cu (tcgen05).
 #include <math.h>
 
 #include "qf_mma.cuh"
@@ -239,9 +241,8 @@ template <int FMT, int D, int WR>
 int launch_f32(const TreeDev& a, cudaStream_t stream) {
     constexpr auto kernel = tree_f32_kernel<FMT, D, WR>;
     constexpr int smem = F32Tile<FMT, D, WR>::FLOATS * 4;
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return launch_failed(e);
+    const int rc = allow_smem<kernel>(smem);
+    if (rc) return rc;
     const int64_t groups = ceil_div((int64_t)a.max_tree * a.G, 4 * WR);
     if (groups * a.Hkv > 65535) return QF_ERR_UNSUPPORTED;
     kernel<<<dim3((unsigned)a.P, (unsigned)(groups * a.Hkv), (unsigned)a.S), 128, smem, stream>>>(a);
@@ -360,6 +361,7 @@ __global__ void __launch_bounds__(128)
 
 // ---------------------------------------------------------------------------
 struct TreePlan {
+    int tiles;  // row tiles per CTA of the tcgen05 kernel; 0: another kernel
     int part, P;
     int64_t rows;  // rows of one kv head in the longest tree
 };
@@ -371,10 +373,13 @@ TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     TreePlan p{};
     const int64_t G = g.num_q_heads / g.num_kv_heads, nq = g.cu_seqlens_q ? g.max_tree : 1;
     p.rows = nq * G;
-    int64_t per_cta = kMmaRows;
-    const int64_t slots = (int64_t)sm_count() * 3;
+    int64_t per_cta = kMmaRows, slots = (int64_t)sm_count() * 3;
     if (g.dtype == QF_F32) {
         per_cta = p.rows <= 4 ? 4 : 16;
+    } else if (g.head_dim == 128 && p.rows > kMmaRows) {
+        p.tiles = p.rows > 128 ? 2 : 1;
+        per_cta = 128 * p.tiles;
+        slots = (int64_t)sm_count() * (p.tiles == 1 ? 2 : 1);
     } else if (g.head_dim == 256 || p.rows <= 8) {
         per_cta = 8;
     }
@@ -421,11 +426,12 @@ int check_tree_args(const qf_paged_tree_attention_args& g) {
         g.mask_words > INT32_MAX || g.num_tokens > INT32_MAX || g.num_q_heads > (1 << 20))
         return QF_ERR_UNSUPPORTED;
     const int64_t es = g.dtype == QF_F32 ? 4 : 2, cs = g.cache_format == QF_CACHE_PLAIN ? es : 1;
-    // q rows and cache rows are read in 16-byte chunks
+    // rows of q, of out and of the caches are read and written in 16-byte chunks
     if ((g.q_stride_token * es) % 16 || (g.q_stride_head * es) % 16 || !aligned16(g.q) ||
         (g.cache_strides[0] * cs) % 16 || (g.cache_strides[1] * cs) % 16 ||
         (g.cache_strides[2] * cs) % 16 || g.cache_strides[3] != 1 || !aligned16(g.k_cache) ||
-        !aligned16(g.v_cache) || !aligned16(g.workspace))
+        !aligned16(g.v_cache) || !aligned16(g.workspace) || (g.out_stride_token * es) % 16 ||
+        (g.out_stride_head * es) % 16 || !aligned16(g.out))
         return QF_ERR_UNSUPPORTED;
     return QF_OK;
 }
@@ -513,6 +519,8 @@ extern "C" int qf_paged_tree_attention(const qf_paged_tree_attention_args* p, cu
     const int D = (int)g.head_dim;
     if (g.dtype == QF_F32)
         rc = qf::launch_tree_f32(a, g.cache_format, D, stream);
+    else if (plan.tiles)
+        rc = qf::launch_tree_tc(a, g.dtype, g.cache_format, plan.tiles, stream);
     else
         rc = qf::launch_tree_mma(a, g.dtype, g.cache_format, D, (int)plan.rows, stream);
     if (rc || a.P == 1) return rc;

@@ -143,7 +143,23 @@ __device__ __forceinline__ void zero_unowned_rows(const TreeDev& a, int s, int g
     if (s == a.S - 1) zero(e, a.T);
 }
 
-// The 16-bit kernel (paged_tree_mma.cu), `rows` rows per kv head in the longest tree.
+// Let a kernel take `bytes` of dynamic shared memory, once per device.
+template <auto Kernel>
+int allow_smem(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return launch_failed(e);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) >> dev) & 1) return QF_OK;
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return launch_failed(e);
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return QF_OK;
+}
+
+// The 16-bit kernels: paged_tree_mma.cu for few rows per kv head (`rows` in the
+// longest tree), paged_tree_tc.cu for many at head_dim 128 (`tiles` of 128 per CTA).
 int launch_tree_mma(const TreeDev& a, int dtype, int format, int D, int rows, cudaStream_t stream);
+int launch_tree_tc(const TreeDev& a, int dtype, int format, int tiles, cudaStream_t stream);
 
 }  // namespace qf
