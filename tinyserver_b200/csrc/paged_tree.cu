@@ -264,14 +264,15 @@ int launch_f32(const TreeDev& a, int D, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------------------
-// Join the partitions of sequences longer than one: a warp per (token, head)
-// row, partials in the workspace as (acc[D], max in log2 units, sum).
+// Join the partitions of sequences longer than one: a CTA of four warps per
+// (token, head) row, each warp a quarter of the partials (acc[D], reference in
+// log2 units, sum), eight of them in flight.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeDev a) {
     pdl_wait();
-    const int h = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const TreeSeq w = tree_seq(a, blockIdx.z);
-    if (h >= a.Hq || (int)blockIdx.y >= w.n || w.nparts == 1) return;
+    if ((int)blockIdx.y >= w.n || w.nparts == 1) return;
     const int64_t t = w.q0 + blockIdx.y;
     const float* ws = a.ws + (t * a.Hq + h) * a.P * (D + 2);
     float M = -INFINITY;
@@ -281,11 +282,12 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeDev a) {
     float Ls = 0.f, acc[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-#pragma unroll 2
-    for (int p = 0; p < w.nparts; ++p) {
+#pragma unroll 8
+    for (int p = warp; p < w.nparts; p += 4) {
         const float* wp = ws + (int64_t)p * (D + 2);
-        const float f = M == -INFINITY ? 0.f : exp2f(wp[D] - M);
-        Ls += wp[D + 1] * f;
+        const float2 ml = *reinterpret_cast<const float2*>(wp + D);
+        const float f = M == -INFINITY ? 0.f : exp2f(ml.x - M);
+        Ls += ml.y * f;
 #pragma unroll
         for (int e = 0; e < PER; e += 2) {
             const float2 v = *reinterpret_cast<const float2*>(wp + e * 32 + lane * 2);
@@ -293,16 +295,24 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeDev a) {
             acc[e + 1] += v.y * f;
         }
     }
-    T* o = reinterpret_cast<T*>(a.out) + t * a.ot + (int64_t)h * a.oh;
-    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+    __shared__ __align__(8) float part[4][D];
+    __shared__ float sums[4];
 #pragma unroll
-    for (int e = 0; e < PER; ++e)
-        o[(e & ~1) * 32 + lane * 2 + (e & 1)] = Dt<T>::from_f(Ls == 0.f ? 0.f : acc[e] * inv);
+    for (int e = 0; e < PER; e += 2)
+        *reinterpret_cast<float2*>(&part[warp][e * 32 + lane * 2]) = make_float2(acc[e], acc[e + 1]);
+    if (lane == 0) sums[warp] = Ls;
+    __syncthreads();
+    const float total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    T* o = reinterpret_cast<T*>(a.out) + t * a.ot + (int64_t)h * a.oh;
+    for (int d = threadIdx.x; d < D; d += 128) {
+        const float A = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
+        o[d] = Dt<T>::from_f(total == 0.f ? 0.f : A / total);
+    }
 }
 
 template <typename T>
 int launch_merge(const TreeDev& a, int D, cudaStream_t stream) {
-    const dim3 grid((unsigned)ceil_div(a.Hq, 4), (unsigned)a.max_tree, (unsigned)a.S);
+    const dim3 grid((unsigned)a.Hq, (unsigned)a.max_tree, (unsigned)a.S);
     switch (D) {
     case 64: return launch_pdl(tree_merge_kernel<T, 64>, grid, 128, 0, stream, a);
     case 128: return launch_pdl(tree_merge_kernel<T, 128>, grid, 128, 0, stream, a);

@@ -54,8 +54,8 @@ template <int NT>
 struct TreeTc {
     static constexpr int ST = NT;                   // K and V stages
     static constexpr int SOFT = 128 * NT;           // softmax threads
-    static constexpr int MMA_WARP = 4 * NT, LOAD_WARP = MMA_WARP + 1;
-    static constexpr int THREADS = SOFT + 32 + 128;
+    static constexpr int MMA_WARP = 4 * NT, LOAD_WARP = MMA_WARP + 1;  // K, then V
+    static constexpr int THREADS = SOFT + 32 + 64;
     static constexpr int SLOTS = 2 * ST;            // blocks whose scales and valid bits are kept
     static constexpr int SMEM = (NT + 2 * ST) * kTile + 1024;
     static constexpr uint32_t COLS = 256 * NT;      // tensor memory: S_t at 128 t, O_t behind them
@@ -71,6 +71,11 @@ struct TreeBars {
 
 __device__ __forceinline__ void proxy_fence() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+__device__ __forceinline__ void cp_async16_at(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
 }
 
 // Byte offset of 16-byte chunk c (0..15) of row r in a tile.
@@ -134,6 +139,16 @@ __device__ __noinline__ void add_not_finite(const TreeDev& a, const int32_t* bt,
     }
 }
 
+// TMA: box {64 dims, `box` slots, 1 head, 1 block} at (x, slot, head, block) into `dst`.
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int x, int slot, int head,
+                                         int block, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(block), "r"(smem_u32(bar))
+        : "memory");
+}
+
 // S_t = Q_t K^T: head_dim in steps of 16.
 __device__ __forceinline__ void issue_scores(uint32_t d, uint32_t q, uint32_t k, uint32_t id) {
 #pragma unroll
@@ -145,7 +160,8 @@ __device__ __forceinline__ void issue_scores(uint32_t d, uint32_t q, uint32_t k,
 
 template <typename T, int FMT, int NT>
 __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
-    tree_tc_kernel(const TreeDev a) {
+    tree_tc_kernel(const TreeDev a, const __grid_constant__ CUtensorMap tk,
+                   const __grid_constant__ CUtensorMap tv, int box) {
     using C = TreeTc<NT>;
     constexpr bool Q8 = FMT != QF_CACHE_PLAIN;
     using MT = typename std::conditional<Q8, __half, T>::type;
@@ -181,10 +197,10 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, odd_v;
     __shared__ uint32_t valid[C::SLOTS][4];
-    // k-scale, log2 v-scale, 1 / v-scale of a block's keys; [.][2]: its least and largest log2 v-scale per warp
+    // k-scale, log2 v-scale, 1 / v-scale of a block's keys; least and largest log2 v-scale
     __shared__ __align__(16) float sk[Q8 ? C::SLOTS : 1][Q8 ? kRows : 1], sl[Q8 ? C::SLOTS : 1][Q8 ? kRows : 1],
         sr_[Q8 ? C::SLOTS : 1][Q8 ? kRows : 1];
-    __shared__ float srange[Q8 ? C::SLOTS : 1][2][2];
+    __shared__ float srange[Q8 ? C::SLOTS : 1][2];
     volatile int* abort = &abort_flag;
 
     const uint32_t raw = smem_u32(dsm);
@@ -194,12 +210,12 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     if (tid == 0) {
         mbar_init(&bars.q_full, (uint32_t)(ntile * kRows));
         for (int i = 0; i < ST; ++i) {
-            mbar_init(&bars.k_full[i], 64);
-            mbar_init(&bars.v_full[i], 64);
+            mbar_init(&bars.k_full[i], 32);
+            mbar_init(&bars.v_full[i], 32);
             mbar_init(&bars.k_empty[i], 1);
             mbar_init(&bars.v_empty[i], 1);
         }
-        for (int i = 0; i < C::SLOTS; ++i) mbar_init(&bars.info_full[i], 64);
+        for (int i = 0; i < C::SLOTS; ++i) mbar_init(&bars.info_full[i], 32);
         for (int t = 0; t < NT; ++t) {
             mbar_init(&bars.s_full[t], 1);
             mbar_init(&bars.p_full[t], kRows);
@@ -228,26 +244,27 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     const int first_draft = tree ? max(0, (w.ctx - k_begin) / kRows) : nblk;
 
     if (warp >= C::LOAD_WARP) {
-        // ---- loaders: two warps K, two warps V; a warp brings 64 of a block's 128 rows
-        const int side = (warp - C::LOAD_WARP) >> 1, lw = (warp - C::LOAD_WARP) & 1;
+        // ---- loaders: one warp K, one warp V
+        const int side = warp - C::LOAD_WARP;
         const char* src = side ? a.vc : a.kc;
         char* const tiles = side ? vbase : kbase;
         uint64_t* full = side ? bars.v_full : bars.k_full;
         uint64_t* empty = side ? bars.v_empty : bars.k_empty;
-        int j = 0;
-        for (; j < nblk; ++j) {
-            const int st = j % ST, slot = j % C::SLOTS, kb = k_begin + j * kRows;
-            char* tile = tiles + st * kTile;
-            int64_t off[2];
-            unsigned ok[2];
-            float ks[2] = {0.f, 0.f}, vs[2] = {1.f, 1.f};
+        // lane l: keys l, l + 32, l + 64, l + 96 of a block
+        int64_t off[4];
+        unsigned ok[4];
+        float ks[4], vs[4];
+        auto locate = [&](int j) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int key = kb + lw * 64 + x * 32 + lane;
+            for (int x = 0; x < 4; ++x) {
+                const int key = k_begin + j * kRows + x * 32 + lane;
                 int64_t srow = 0;
                 off[x] = 0;
+                ks[x] = 0.f;
+                vs[x] = 1.f;
                 const bool in = key < k_end && key_place(a, bt, g, key, off[x], srow);
                 ok[x] = __ballot_sync(kFull, in);
+                if (!Q8) off[x] *= 2;  // bytes
                 if (Q8 && side == 0 && in) {
                     ks[x] = __ldg(a.ks + srow);
                     vs[x] = __ldg(a.vs + srow);
@@ -255,78 +272,138 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                     if (vs[x] < kLeastScale) vs[x] = kLeastScale;
                 }
             }
-            if constexpr (!Q8) {
-                if (j >= ST && !mbar_wait(&empty[st], ((j / ST) - 1) & 1, abort)) break;
+        };
+        // What the softmax needs to know of block j's keys.  The slot's last reader, the
+        // softmax of block j - SLOTS, is done: S of block j - ST (whose K was in this
+        // stage) came after it.
+        auto inform = [&](int slot) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-#pragma unroll 8
+            for (int x = 0; x < 4; ++x) {
+                if (lane == 0) valid[slot][x] = ok[x];
+                if constexpr (Q8) {
+                    sk[slot][x * 32 + lane] = ks[x];
+                    sl[slot][x * 32 + lane] = log2f(vs[x]);
+                    sr_[slot][x * 32 + lane] = 1.f / vs[x];
+                }
+            }
+            if constexpr (Q8) {
+                float hi = -INFINITY, lo = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if ((ok[x] >> lane) & 1) {
+                        hi = fmaxf(hi, log2f(vs[x]));
+                        lo = fmaxf(lo, -log2f(vs[x]));
+                    }
+                hi = warp_max(hi);
+                lo = -warp_max(lo);
+                if (lane == 0) srange[slot][0] = lo, srange[slot][1] = hi;
+            }
+            __syncwarp();
+            mbar_arrive(&bars.info_full[slot]);
+        };
+        // block j's stage may be refilled (the whole warp learns the same)
+        auto vacant = [&](int j) -> bool {
+            return __all_sync(kFull, j < ST || mbar_wait(&empty[j % ST], ((j / ST) - 1) & 1, abort));
+        };
+        if constexpr (Q8) {
+            // codes into registers, 16 rows' worth a lane group in flight all the time: half a
+            // block is converted and stored while the other half, then the next block's, comes
+            uint4 raws[16];
+            const int c = lane & 7;
+            auto fetch = [&](int i, int half) {
+                const int r = (4 * i + (lane >> 3)) & 31, x = 2 * half + (i >> 3);
+                const int64_t o = __shfl_sync(kFull, x == 0 ? off[0] : x == 1 ? off[1] : x == 2 ? off[2] : off[3], r);
+                const unsigned m = x == 0 ? ok[0] : x == 1 ? ok[1] : x == 2 ? ok[2] : ok[3];
+                raws[i] = (m >> r) & 1 ? ld_stream16(src + o + c * 16) : make_uint4(0, 0, 0, 0);
+            };
+            locate(0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) fetch(i, 0);
+            for (int j = 0; j < nblk; ++j) {
+                const int st = j % ST;
+                char* tile = tiles + st * kTile;
+                if (!vacant(j)) break;
+                if (side == 0) inform(j % C::SLOTS);
+                bool odd = false;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (half == 1 && j + 1 < nblk) locate(j + 1);
+#pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int r = 2 * i + (lane >> 4), c = lane & 15;
-                        const int64_t o = __shfl_sync(kFull, off[x], r);
-                        cp_async16(tile + tile_off(lw * 64 + x * 32 + r, c), src + o * 2 + c * 16,
-                                   (ok[x] >> r) & 1 ? 16 : 0);
+                        const int r = half * 64 + 4 * i + (lane >> 3);
+                        uint4 lo, hi;
+                        codes_to_f16<FMT>(raws[i].x, lo.x, lo.y);
+                        codes_to_f16<FMT>(raws[i].y, lo.z, lo.w);
+                        codes_to_f16<FMT>(raws[i].z, hi.x, hi.y);
+                        codes_to_f16<FMT>(raws[i].w, hi.z, hi.w);
+                        if (half == 0) fetch(i, 1);
+                        else if (j + 1 < nblk) fetch(i, 0);
+                        if (FMT == QF_CACHE_E4M3 && side == 1 && j >= first_draft) {
+                            odd |= zero_not_finite<__half>(lo);
+                            odd |= zero_not_finite<__half>(hi);
+                        }
+                        *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c)) = lo;
+                        *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + 1)) = hi;
+                    }
+                }
+                if (odd) odd_v = 1;
+                proxy_fence();
+                mbar_arrive(&full[st]);
+            }
+        } else {
+            const CUtensorMap* map = side ? &tv : &tk;
+            const int hi = lane >> 4, c = lane & 15;
+            int j = 0;
+            for (; j < nblk; ++j) {
+                const int st = j % ST, kb = k_begin + j * kRows;
+                char* tile = tiles + st * kTile;
+                // A block whose keys are all context and all there comes by TMA, a box of
+                // `box` slots x 64 dims per lane (K and V alike, 128-byte swizzle)
+                bool bulk = box > 0 && j < first_draft && kb + kRows <= k_end;
+                int blk = 0, slot0 = 0;
+                const int pc = lane >> 1;  // this lane's piece of the block
+                if (bulk) {
+                    const int key = kb + min(pc * box, kRows - 1);
+                    const int lb = a.B.div(key);
+                    blk = __ldg(bt + lb);
+                    slot0 = key - lb * a.B.d;
+                    bulk = __all_sync(kFull, blk >= 0 && blk < a.N);
+                }
+                if (!bulk) locate(j);
+                if (!vacant(j)) break;
+                if (bulk) {
+                    if (side == 0) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) ok[x] = kFull;
+                        inform(j % C::SLOTS);
+                    }
+                    if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)kTile);
+                    else mbar_arrive(&full[st]);
+                    __syncwarp();
+                    if (pc * box < kRows)
+                        tma_page(tile + (lane & 1) * kSlab + pc * box * 128, map, (lane & 1) * 64, slot0, g, blk,
+                                 &full[st]);
+                    continue;
+                }
+                if (side == 0) inform(j % C::SLOTS);
+                // row by row: chunk c of rows 2 i + hi; the swizzle repeats every four i
+                const uint32_t dst = smem_u32(tile) + (uint32_t)((c >> 3) * kSlab + hi * 128);
+                const char* from = src + c * 16;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int64_t o = __shfl_sync(kFull, off[x], 2 * i + hi);
+                        cp_async16_at(dst + (uint32_t)((x * 32 + 2 * i) * 128 + (((c & 7) ^ ((2 * i & 7) + hi)) << 4)),
+                                      from + o, (ok[x] >> (2 * i + hi)) & 1 ? 16 : 0);
                     }
                 }
                 cp_async_commit();
-            } else {
-                uint4 raws[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int r = (4 * i + (lane >> 3)) & 31, c = lane & 7;
-                    const int64_t o = __shfl_sync(kFull, off[i >> 3], r);
-                    raws[i] = (ok[i >> 3] >> r) & 1 ? ld_stream16(src + o + c * 16) : make_uint4(0, 0, 0, 0);
-                }
-                if (j >= ST && !mbar_wait(&empty[st], ((j / ST) - 1) & 1, abort)) break;
-                bool odd = false;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int r = lw * 64 + 4 * i + (lane >> 3), c = lane & 7;
-                    uint4 lo, hi;
-                    codes_to_f16<FMT>(raws[i].x, lo.x, lo.y);
-                    codes_to_f16<FMT>(raws[i].y, lo.z, lo.w);
-                    codes_to_f16<FMT>(raws[i].z, hi.x, hi.y);
-                    codes_to_f16<FMT>(raws[i].w, hi.z, hi.w);
-                    if (FMT == QF_CACHE_E4M3 && side == 1 && j >= first_draft) {
-                        odd |= zero_not_finite<__half>(lo);
-                        odd |= zero_not_finite<__half>(hi);
-                    }
-                    *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c)) = lo;
-                    *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + 1)) = hi;
-                }
-                if (odd) odd_v = 1;
-            }
-            if (side == 0) {
-                // the slot's last reader, the softmax of block j - SLOTS, is done: S of
-                // block j - ST (whose K was in this stage) came after it
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    if (lane == 0) valid[slot][lw * 2 + x] = ok[x];
-                    if constexpr (Q8) {
-                        const int r = lw * 64 + x * 32 + lane;
-                        sk[slot][r] = ks[x];
-                        sl[slot][r] = log2f(vs[x]);
-                        sr_[slot][r] = 1.f / vs[x];
-                    }
-                }
-                if constexpr (Q8) {
-                    const float l0 = log2f(vs[0]), l1 = log2f(vs[1]);
-                    const bool in0 = (ok[0] >> lane) & 1, in1 = (ok[1] >> lane) & 1;
-                    const float hi = warp_max(fmaxf(in0 ? l0 : -INFINITY, in1 ? l1 : -INFINITY));
-                    const float lo = -warp_max(fmaxf(in0 ? -l0 : -INFINITY, in1 ? -l1 : -INFINITY));
-                    if (lane == 0) srange[slot][lw][0] = lo, srange[slot][lw][1] = hi;
-                }
-                __syncwarp();
-                mbar_arrive(&bars.info_full[slot]);
-            }
-            // signal the block whose copies have landed: this one, or with two
-            // stages of cp.async the one before it
-            auto landed = [&](int jj) {
-                if (!Q8 && side == 1 && jj >= first_draft) {  // this lane's own chunks
-                    char* t = tiles + (jj % ST) * kTile;
+                cp_async_wait<0>();
+                if (side == 1 && j >= first_draft) {  // this lane's own chunks
                     bool odd = false;
-                    for (int i = 0; i < 32; ++i) {
-                        uint4* at = reinterpret_cast<uint4*>(
-                            t + tile_off(lw * 64 + 2 * i + (lane >> 4), lane & 15));
+                    for (int i = 0; i < 64; ++i) {
+                        uint4* at = reinterpret_cast<uint4*>(tile + tile_off(2 * i + hi, c));
                         uint4 v = *at;
                         if (zero_not_finite<MT>(v)) {
                             *at = v;
@@ -336,25 +413,11 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                     if (odd) odd_v = 1;
                 }
                 proxy_fence();
-                mbar_arrive(&full[jj % ST]);
-            };
-            if constexpr (Q8) {
-                landed(j);
-            } else if constexpr (ST == 1) {
-                cp_async_wait<0>();
-                landed(j);
-            } else {
-                if (j > 0) {
-                    cp_async_wait<1>();
-                    landed(j - 1);
-                }
-                if (j == nblk - 1) {
-                    cp_async_wait<0>();
-                    landed(j);
-                }
+                mbar_arrive(&full[st]);
             }
+            // every copy issued has landed before the CTA can leave
+            for (int d = max(0, j - ST); d < j; ++d) mbar_wait(&full[d % ST], (d / ST) & 1, nullptr);
         }
-        cp_async_wait<0>();
     } else if (warp == C::MMA_WARP) {
         // ---- MMA issue: S_t,0 | PV_t,j S_t,j+1 | ...
         if (lane == 0) {
@@ -412,6 +475,11 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         {
             using P = Packed<T>;
             float f = 1.f;
+            uint32_t flip = 0;
+            if (!Q8) {  // rs > 0: a negative scale's sign goes to Q, and 0 becomes as good as 0
+                flip = sl2 < 0.f ? 0x80008000u : 0u;
+                rs = fabsf(sl2) < 1e-30f ? 1e-30f : fabsf(sl2);
+            }
             if constexpr (Q8) {  // a power-of-two factor brings the largest element to [2^14, 2^15)
                 uint32_t mx = 0;
                 if (live)
@@ -433,6 +501,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                     for (int i = 0; i < 4; ++i)
                         set_word(v, i, MP::pack(P::lo(word(v, i)) * f, P::hi(word(v, i)) * f));
                 }
+                if (!Q8) v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
                 *reinterpret_cast<uint4*>(base + t * kTile + tile_off(r, c)) = v;
             }
             proxy_fence();
@@ -457,35 +526,83 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 if (j >= first_draft && live) see[q] &= tree_bits32(mrow, a.words, kb + 32 * q - w.ctx);
             }
             const bool masked = __any_sync(kFull, (see[0] & see[1] & see[2] & see[3]) != kFull);
-            // a column's score in log2 units, with V's scale where there is one
+            // Scores in log2 units, with V's scale where there is one: 16-bit rows x * rs,
+            // rs > 0 (a negative scale is in Q), so the maximum is that of x.
             auto score = [&](float x, int c) -> float {
                 if constexpr (Q8) return fmaf(x * rs, sk[slot][c], sl[slot][c]);
-                else return x * rs;
+                else return x;
             };
-            // the row's maximum over the block
-            float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint32_t x[32];
-                tmem_ld32(sS + 32 * q, x);
-                tmem_wait_ld();
-                if (masked) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if ((see[q] >> e) & 1) mx0 = fmaxf(mx0, score(__uint_as_float(x[e]), 32 * q + e));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        mx0 = max3(mx0, score(__uint_as_float(x[e]), 32 * q + e),
-                                   score(__uint_as_float(x[e + 1]), 32 * q + e + 1));
-                        mx1 = max3(mx1, score(__uint_as_float(x[e + 2]), 32 * q + e + 2),
-                                   score(__uint_as_float(x[e + 3]), 32 * q + e + 3));
-                    }
-                }
+            bool wide = false;
+            if constexpr (Q8) {
+                lvtop = fmaxf(lvtop, srange[slot][1]);
+                wide = lvtop - srange[slot][0] > kScaleRange;
             }
-            const float mx = fmaxf(mx0, mx1);
-            const bool move = mx > m + kKeepLog2 || (m == -INFINITY && mx > -INFINITY);
-            if (__any_sync(kFull, move)) {
+            // One pass over S against the reference m, P in registers, the block's maximum on
+            // the side.  While no row's maximum has grown past 2^8 (but for the first blocks,
+            // nearly always) P stands; else the reference moves, O and l with it, and
+            // the pass is made again over S, which P has not touched yet.
+            uint32_t pk[64];
+            float sum;
+            for (int turn = 0;; ++turn) {
+                const float mref = m == -INFINITY ? 0.f : m;
+                float mx0 = -INFINITY, mx1 = -INFINITY;
+                float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+                constexpr int NX = NT == 2 ? 2 : 1;  // registers allow: the next quarter's load in flight
+                uint32_t x[NX][32];
+                tmem_ld32(sS, x[0]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if (NX == 2 && q < 3) tmem_ld32(sS + 32 * (q + 1), x[(q + 1) % NX]);
+                    uint32_t* xs = x[q % NX];
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!((see[q] >> e) & 1)) xs[e] = __float_as_uint(-INFINITY);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const int c = 32 * q + e;
+                        const float x0 = __uint_as_float(xs[e]), x1 = __uint_as_float(xs[e + 1]);
+                        float t0, t1;
+                        if constexpr (Q8) {
+                            t0 = score(x0, c);
+                            t1 = score(x1, c + 1);
+                            if (masked) {  // an unseen key's scales may be anything
+                                if (x0 == -INFINITY) t0 = -INFINITY;
+                                if (x1 == -INFINITY) t1 = -INFINITY;
+                            }
+                            mx0 = max3(mx0, t0, t1);
+                            t0 -= mref;
+                            t1 -= mref;
+                        } else {
+                            if (e & 2) mx1 = max3(mx1, x0, x1);
+                            else mx0 = max3(mx0, x0, x1);
+                            fma2(t0, t1, x0, x1, rs, -mref);
+                        }
+                        const float p0 = ex2(t0), p1 = ex2(t1);
+                        if constexpr (Q8) {
+                            if (!wide) {
+                                s0 = fmaf(p0, !masked || t0 != -INFINITY ? sr_[slot][c] : 0.f, s0);
+                                s1 = fmaf(p1, !masked || t1 != -INFINITY ? sr_[slot][c + 1] : 0.f, s1);
+                            } else {
+                                s0 += t0 == -INFINITY ? 0.f : ex2(t0 - sl[slot][c]);
+                                s1 += t1 == -INFINITY ? 0.f : ex2(t1 - sl[slot][c + 1]);
+                            }
+                        } else if (e & 2) {
+                            add2(s2, s3, p0, p1);
+                        } else {
+                            add2(s0, s1, p0, p1);
+                        }
+                        pk[16 * q + (e >> 1)] = MP::pack(p0, p1);
+                    }
+                    if (NX == 1 && q < 3) tmem_ld32(sS + 32 * (q + 1), x[0]);
+                    if (q < 3) tmem_wait_ld();
+                }
+                sum = (s0 + s1) + (s2 + s3);
+                const float mx = fmaxf(mx0, mx1) * (Q8 ? 1.f : rs);
+                const bool move = turn == 0 && (mx > m + kKeepLog2 || (m == -INFINITY && mx > -INFINITY));
+                if (!__any_sync(kFull, move)) break;
                 // the block before's P V is done: S of this block was issued after it
                 const float corr = move ? ex2(m - mx) : 1.f;
                 if (j > 0) {
@@ -502,46 +619,9 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 l *= corr;
                 if (move) m = mx;
             }
-            const float mref = m == -INFINITY ? 0.f : m;
-            bool wide = false;
-            if constexpr (Q8) {
-                lvtop = fmaxf(lvtop, fmaxf(srange[slot][0][1], srange[slot][1][1]));
-                wide = lvtop - fminf(srange[slot][0][0], srange[slot][1][0]) > kScaleRange;
-            }
-            float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint32_t x[32], pk[16];
-                tmem_ld32(sS + 32 * q, x);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const int c = 32 * q + e;
-                    float t0 = score(__uint_as_float(x[e]), c) - mref;
-                    float t1 = score(__uint_as_float(x[e + 1]), c + 1) - mref;
-                    if (masked) {
-                        if (!((see[q] >> e) & 1)) t0 = -INFINITY;
-                        if (!((see[q] >> (e + 1)) & 1)) t1 = -INFINITY;
-                    }
-                    const float p0 = ex2(t0), p1 = ex2(t1);
-                    if constexpr (Q8) {
-                        if (!wide) {
-                            // an unseen key's factor may be anything: only a seen one counts
-                            s0 = fmaf(p0, !masked || ((see[q] >> e) & 1) ? sr_[slot][c] : 0.f, s0);
-                            s1 = fmaf(p1, !masked || ((see[q] >> (e + 1)) & 1) ? sr_[slot][c + 1] : 0.f, s1);
-                        } else {
-                            s0 += t0 == -INFINITY ? 0.f : ex2(t0 - sl[slot][c]);
-                            s1 += t1 == -INFINITY ? 0.f : ex2(t1 - sl[slot][c + 1]);
-                        }
-                    } else {
-                        s0 += p0;
-                        s1 += p1;
-                    }
-                    pk[e >> 1] = MP::pack(p0, p1);
-                }
-                tmem_st16(sS + 16 * q, pk);
-            }
-            l += s0 + s1;
+            for (int q = 0; q < 4; ++q) tmem_st16(sS + 16 * q, pk + 16 * q);
+            l += sum;
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&bars.p_full[t]);
@@ -595,6 +675,20 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     }
 }
 
+// A map over a 16-bit cache (128 dims, B slots, Hkv heads, N blocks), boxes of 64 dims x `box` slots.
+bool page_map(CUtensorMap* map, const char* ptr, const TreeDev& a, int bf16, int box) {
+    PFN_cuTensorMapEncodeTiled fn = tensor_map_encode();
+    if (!fn || a.N <= 0) return false;
+    const cuuint64_t dims[4] = {kD, (cuuint64_t)a.B.d, (cuuint64_t)a.Hkv, (cuuint64_t)a.N};
+    const cuuint64_t strides[3] = {(cuuint64_t)a.c2 * 2, (cuuint64_t)a.c1 * 2, (cuuint64_t)a.c0 * 2};
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
+    const cuuint32_t step[4] = {1, 1, 1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+              const_cast<char*>(ptr), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int FMT, int NT>
 int launch_nt(const TreeDev& a, cudaStream_t stream) {
     constexpr auto kernel = tree_tc_kernel<T, FMT, NT>;
@@ -602,8 +696,17 @@ int launch_nt(const TreeDev& a, cudaStream_t stream) {
     if (rc) return rc;
     const int64_t groups = ceil_div((int64_t)a.max_tree * a.G, NT * kRows);
     if (groups * a.Hkv > 65535) return QF_ERR_UNSUPPORTED;
+    // The largest power of two that divides a page and a block: a piece never crosses a
+    // page.  Below 8 (or where the cache's shape has no map) rows come one by one.
+    CUtensorMap tk{}, tv{};
+    int box = 0;
+    if (FMT == QF_CACHE_PLAIN) {
+        const int bf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+        box = std::min(a.B.d & -a.B.d, kRows);
+        if (box < 8 || !page_map(&tk, a.kc, a, bf16, box) || !page_map(&tv, a.vc, a, bf16, box)) box = 0;
+    }
     kernel<<<dim3((unsigned)a.P, (unsigned)(groups * a.Hkv), (unsigned)a.S), TreeTc<NT>::THREADS,
-             TreeTc<NT>::SMEM, stream>>>(a);
+             TreeTc<NT>::SMEM, stream>>>(a, tk, tv, box);
     return check_launch();
 }
 

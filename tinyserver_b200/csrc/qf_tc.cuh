@@ -7,6 +7,9 @@
 // swizzle (row r at r * 128, 16-byte chunk c at (c ^ r % 8) * 16).
 #pragma once
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "qf_common.cuh"
 
 namespace qf {
@@ -193,6 +196,21 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
           "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
+}
+
+// cuTensorMapEncodeTiled, looked up once through the runtime.
+inline PFN_cuTensorMapEncodeTiled tensor_map_encode() {
+    static std::once_flag once;
+    static PFN_cuTensorMapEncodeTiled fn = nullptr;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+                cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(p);
+    });
+    return fn;
 }
 
 }  // namespace qf

@@ -37,10 +37,6 @@
 // 128-byte swizzle (row r at r * 128, 16-byte chunk c at (c ^ r % 8) * 16),
 // which is what a TMA box of 64 x 1 x 128 with SWIZZLE_128B writes.  Q and K
 // are read K-major, V MN-major (rows = keys, the reduction dimension).
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include <mutex>
 #include <type_traits>
 
 #include "qf_tc.cuh"
@@ -678,25 +674,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// cuTensorMapEncodeTiled, looked up once through the runtime.
-PFN_cuTensorMapEncodeTiled encode_fn() {
-    static std::once_flag once;
-    static PFN_cuTensorMapEncodeTiled fn = nullptr;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-                cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled>(p);
-    });
-    return fn;
-}
-
 // A 3-D map over (head_dim = 128, heads, tokens) with 64 x 1 x 128 boxes.
 bool make_map(CUtensorMap* map, const char* ptr, int bf16, int64_t heads, int64_t tokens,
               int64_t head_stride, int64_t token_stride, int rows = kRows) {
-    PFN_cuTensorMapEncodeTiled fn = encode_fn();
+    PFN_cuTensorMapEncodeTiled fn = tensor_map_encode();
     if (!fn) return false;
     const cuuint64_t dims[3] = {128, (cuuint64_t)heads, (cuuint64_t)tokens};
     const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)token_stride * 2};
