@@ -24,7 +24,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMmaRows = 16;
-constexpr int kMinPart = 256, kMaxPart = 1 << 30;  // keys of a partition
+constexpr int kF32Keys = 64;  // keys of a work unit of the fp32 kernel
 
 // ---------------------------------------------------------------------------
 // fp32.  A CTA of 4 warps takes NR = 4 WR rows and steps through tiles of 32
@@ -61,14 +61,6 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const TreeDev a) {
     using FT = F32Tile<FMT, D, WR>;
     constexpr int WK = FT::WK, NR = FT::NR, KW = FT::KW, KROW = FT::KROW, PER = D / 32;
     constexpr int EB = FMT == QF_CACHE_PLAIN ? 4 : 1, EPC = 16 / EB;
-    const int p = blockIdx.x, s = blockIdx.z;
-    const int g = blockIdx.y % a.Hkv, rg = blockIdx.y / a.Hkv;
-    const TreeSeq w = tree_seq(a, s);
-    if (p == 0 && rg == 0) zero_unowned_rows<float, D>(a, s, g, w);
-    const int rows = w.n * a.G, r0 = rg * NR;
-    if (p >= w.nparts || r0 >= rows) return;
-    const int k_begin = p * a.part, k_end = k_begin + min(w.L - k_begin, a.part);
-
     extern __shared__ __align__(16) float fsm[];
     float* qs = fsm;
     float* kt = qs + FT::Q;
@@ -77,15 +69,24 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const TreeDev a) {
     float* corr = ps + FT::PS;  // [4 warps][4 rows]
     int* kval = reinterpret_cast<int*>(corr + 16);
 
+    __shared__ int64_t scratch[34];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wr = warp % WR, wk = warp / WR;
+    TreeWalk<kF32Keys, NR> walk;
+    walk.begin(a, scratch);
+    zero_unowned_rows<float, D>(a);
+    if (tid == 0) walk.record(a);
+    TreeSeg sg;
+    while (walk.next(a, sg)) {
+    const TreeSeq& w = sg.w;
+    const int rows = w.n * a.G, r0 = sg.rg * NR, g = sg.g, k_begin = sg.k_begin, k_end = sg.k_end;
     for (int i = tid; i < NR * D; i += 128) {
         const int r = r0 + i / D, d = i % D;
         qs[i] = r < rows ? reinterpret_cast<const float*>(a.q)[(int64_t)(w.q0 + r / a.G) * a.qt +
                                                                (int64_t)(g * a.G + r % a.G) * a.qh + d]
                          : 0.f;
     }
-    const int32_t* bt = a.bt + (int64_t)s * a.bts;
+    const int32_t* bt = a.bt + (int64_t)sg.s * a.bts;
     const float sl2 = a.scale * kLog2e;
     constexpr int NS = 4 * KW / 32;  // scores per lane
     float m[NS], l[NS], acc[4][PER];
@@ -224,10 +225,10 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const TreeDev a) {
             A += wacc[(k * NR + ri) * D + d] * f;
         }
         const int64_t t = w.q0 + r / a.G, h = g * a.G + r % a.G;
-        if (w.nparts == 1) {
+        if (sg.slot < 0) {
             reinterpret_cast<float*>(a.out)[t * a.ot + h * a.oh + d] = Ls == 0.f ? 0.f : A / Ls;
         } else {
-            float* o = a.ws + ((t * a.Hq + h) * a.P + p) * (D + 2);
+            float* o = tree_partial(a, gridDim.x, blockIdx.x, sg.slot, NR, ri, D);
             o[d] = A;
             if (d == 0) {
                 o[D] = M;
@@ -235,88 +236,115 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const TreeDev a) {
             }
         }
     }
+    __syncthreads();  // the merge area becomes the tiles again
+    }
 }
 
 template <int FMT, int D, int WR>
-int launch_f32(const TreeDev& a, cudaStream_t stream) {
+int launch_f32(const TreeDev& a, int ctas, cudaStream_t stream) {
     constexpr auto kernel = tree_f32_kernel<FMT, D, WR>;
     constexpr int smem = F32Tile<FMT, D, WR>::FLOATS * 4;
     const int rc = allow_smem<kernel>(smem);
     if (rc) return rc;
-    const int64_t groups = ceil_div((int64_t)a.max_tree * a.G, 4 * WR);
-    if (groups * a.Hkv > 65535) return QF_ERR_UNSUPPORTED;
-    kernel<<<dim3((unsigned)a.P, (unsigned)(groups * a.Hkv), (unsigned)a.S), 128, smem, stream>>>(a);
+    kernel<<<(unsigned)ctas, 128, smem, stream>>>(a);
     return check_launch();
 }
 
 template <int FMT, int D>
-int launch_f32(const TreeDev& a, cudaStream_t stream) {
-    return a.max_tree * a.G <= 4 ? launch_f32<FMT, D, 1>(a, stream) : launch_f32<FMT, D, 4>(a, stream);
+int launch_f32(const TreeDev& a, int rows, int ctas, cudaStream_t stream) {
+    return rows == 4 ? launch_f32<FMT, D, 1>(a, ctas, stream) : launch_f32<FMT, D, 4>(a, ctas, stream);
 }
 
 template <int FMT>
-int launch_f32(const TreeDev& a, int D, cudaStream_t stream) {
+int launch_f32(const TreeDev& a, int D, int rows, int ctas, cudaStream_t stream) {
     switch (D) {
-    case 64: return launch_f32<FMT, 64>(a, stream);
-    case 128: return launch_f32<FMT, 128>(a, stream);
-    default: return launch_f32<FMT, 256>(a, stream);
+    case 64: return launch_f32<FMT, 64>(a, rows, ctas, stream);
+    case 128: return launch_f32<FMT, 128>(a, rows, ctas, stream);
+    default: return launch_f32<FMT, 256>(a, rows, ctas, stream);
     }
 }
 
 // ---------------------------------------------------------------------------
-// Join the partitions of sequences longer than one: a CTA of four warps per
-// (token, head) row, each warp a quarter of the partials (acc[D], reference in
-// log2 units, sum), eight of them in flight.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeDev a) {
+// Join the partials of the items that a CTA began and later ones went on with:
+// blockIdx.x + 1 is the item's second CTA, whose record has it.  WPR warps per row
+// share its partials (acc[D], reference in log2 units, sum), eight each in flight.
+template <typename T, int D, int WPR>
+__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeDev a, int rows_per_item) {
     pdl_wait();
-    const int h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const TreeSeq w = tree_seq(a, blockIdx.z);
-    if ((int)blockIdx.y >= w.n || w.nparts == 1) return;
-    const int64_t t = w.q0 + blockIdx.y;
-    const float* ws = a.ws + (t * a.Hq + h) * a.P * (D + 2);
-    float M = -INFINITY;
-    for (int p = lane; p < w.nparts; p += 32) M = fmaxf(M, ws[(int64_t)p * (D + 2) + D]);
-    M = warp_max(M);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t ctas = gridDim.x + 1, cta = blockIdx.x + 1;
+    const TreeRec rec = reinterpret_cast<const TreeRec*>(a.ws)[cta];
+    if (rec.last == 0) return;
+    const TreeSeq w = tree_seq(a, rec.s, false);
+    const int ri = blockIdx.y * (4 / WPR) + warp / WPR, sub = warp % WPR;
+    const int r = rec.rg * rows_per_item + ri;
+    const bool live = r < w.n * a.G;
+    if (WPR == 4 && !live) return;  // (the whole CTA)
     constexpr int PER = D / 32;
     float Ls = 0.f, acc[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    if (live) {
+        const int n = rec.last - (int)cta + 2;
+        auto partial = [&](int p) -> const float* {
+            return tree_partial(a, ctas, cta - 1 + p, p == 0 ? 1 : 0, rows_per_item, ri, D);
+        };
+        float M = -INFINITY;
+        for (int p = lane; p < n; p += 32) M = fmaxf(M, partial(p)[D]);
+        M = warp_max(M);
 #pragma unroll 8
-    for (int p = warp; p < w.nparts; p += 4) {
-        const float* wp = ws + (int64_t)p * (D + 2);
-        const float2 ml = *reinterpret_cast<const float2*>(wp + D);
-        const float f = M == -INFINITY ? 0.f : exp2f(ml.x - M);
-        Ls += ml.y * f;
+        for (int p = sub; p < n; p += WPR) {
+            const float* wp = partial(p);
+            const float2 ml = *reinterpret_cast<const float2*>(wp + D);
+            const float f = M == -INFINITY ? 0.f : exp2f(ml.x - M);
+            Ls += ml.y * f;
 #pragma unroll
-        for (int e = 0; e < PER; e += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(wp + e * 32 + lane * 2);
-            acc[e] += v.x * f;
-            acc[e + 1] += v.y * f;
+            for (int e = 0; e < PER; e += 2) {
+                const float2 v = *reinterpret_cast<const float2*>(wp + e * 32 + lane * 2);
+                acc[e] += v.x * f;
+                acc[e + 1] += v.y * f;
+            }
         }
     }
-    __shared__ __align__(8) float part[4][D];
-    __shared__ float sums[4];
+    const int tok = r / a.G;
+    T* o = reinterpret_cast<T*>(a.out) + (int64_t)(w.q0 + tok) * a.ot +
+           (int64_t)(rec.g * a.G + r - tok * a.G) * a.oh;
+    if constexpr (WPR == 1) {
+        if (!live) return;
 #pragma unroll
-    for (int e = 0; e < PER; e += 2)
-        *reinterpret_cast<float2*>(&part[warp][e * 32 + lane * 2]) = make_float2(acc[e], acc[e + 1]);
-    if (lane == 0) sums[warp] = Ls;
-    __syncthreads();
-    const float total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-    T* o = reinterpret_cast<T*>(a.out) + t * a.ot + (int64_t)h * a.oh;
-    for (int d = threadIdx.x; d < D; d += 128) {
-        const float A = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
-        o[d] = Dt<T>::from_f(total == 0.f ? 0.f : A / total);
+        for (int e = 0; e < PER; ++e)
+            o[(e & ~1) * 32 + lane * 2 + (e & 1)] = Dt<T>::from_f(Ls == 0.f ? 0.f : acc[e] / Ls);
+    } else {
+        __shared__ __align__(8) float part[4][D];
+        __shared__ float sums[4];
+#pragma unroll
+        for (int e = 0; e < PER; e += 2)
+            *reinterpret_cast<float2*>(&part[warp][e * 32 + lane * 2]) = make_float2(acc[e], acc[e + 1]);
+        if (lane == 0) sums[warp] = Ls;
+        __syncthreads();
+        const float total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        for (int d = threadIdx.x; d < D; d += 128) {
+            const float A = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
+            o[d] = Dt<T>::from_f(total == 0.f ? 0.f : A / total);
+        }
     }
 }
 
+template <typename T, int D>
+int launch_merge(const TreeDev& a, int rows, int ctas, cudaStream_t stream) {
+    if (rows <= 16)
+        return launch_pdl(tree_merge_kernel<T, D, 4>, dim3((unsigned)ctas - 1, (unsigned)rows), 128, 0, stream, a,
+                          rows);
+    return launch_pdl(tree_merge_kernel<T, D, 1>, dim3((unsigned)ctas - 1, (unsigned)rows / 4), 128, 0, stream, a,
+                      rows);
+}
+
 template <typename T>
-int launch_merge(const TreeDev& a, int D, cudaStream_t stream) {
-    const dim3 grid((unsigned)a.Hq, (unsigned)a.max_tree, (unsigned)a.S);
+int launch_merge(const TreeDev& a, int D, int rows, int ctas, cudaStream_t stream) {
     switch (D) {
-    case 64: return launch_pdl(tree_merge_kernel<T, 64>, grid, 128, 0, stream, a);
-    case 128: return launch_pdl(tree_merge_kernel<T, 128>, grid, 128, 0, stream, a);
-    default: return launch_pdl(tree_merge_kernel<T, 256>, grid, 128, 0, stream, a);
+    case 64: return launch_merge<T, 64>(a, rows, ctas, stream);
+    case 128: return launch_merge<T, 128>(a, rows, ctas, stream);
+    default: return launch_merge<T, 256>(a, rows, ctas, stream);
     }
 }
 
@@ -371,34 +399,41 @@ __global__ void __launch_bounds__(128)
 
 // ---------------------------------------------------------------------------
 struct TreePlan {
-    int tiles;  // row tiles per CTA of the tcgen05 kernel; 0: another kernel
-    int part, P;
-    int64_t rows;  // rows of one kv head in the longest tree
+    int tiles;      // row tiles per CTA of the tcgen05 kernel; 0: another kernel
+    int rows;       // rows per work item
+    int ctas;       // persistent CTAs: as many as fit, or one per unit of work if that is fewer
+    int min_units;  // least stretch of a CTA
+    bool split;     // whether sequences may be cut
 };
 
-// Keys per partition.  Splitting costs a partial of (D + 2) floats a row,
-// written and read back, so the sequences are split only until the grid has
-// some `kWaves` times as many CTAs as fit on the GPU, and never below kMinPart keys.
+// The kernel and its grid, by sizes alone (lengths are on the device; the block
+// tables bound them).  A cut costs a partial of (D + 2) floats a row, written and
+// read back, so a CTA's stretch is at least two blocks of 128 keys, or four of 64.
 TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     TreePlan p{};
-    const int64_t G = g.num_q_heads / g.num_kv_heads, nq = g.cu_seqlens_q ? g.max_tree : 1;
-    p.rows = nq * G;
-    int64_t per_cta = kMmaRows, slots = (int64_t)sm_count() * 3;
+    const int64_t G = g.num_q_heads / g.num_kv_heads, rows = (g.cu_seqlens_q ? g.max_tree : 1) * G;
+    int64_t per_sm, keys = 64;
+    const bool plain = g.cache_format == QF_CACHE_PLAIN;
+    p.min_units = 4;
     if (g.dtype == QF_F32) {
-        per_cta = p.rows <= 4 ? 4 : 16;
-    } else if (g.head_dim == 128 && p.rows > kMmaRows) {
-        p.tiles = p.rows > 128 ? 2 : 1;
-        per_cta = 128 * p.tiles;
-        slots = (int64_t)sm_count() * (p.tiles == 1 ? 2 : 1);
-    } else if (g.head_dim == 256 || p.rows <= 8) {
-        per_cta = 8;
+        p.rows = rows <= 4 ? 4 : 16;
+        per_sm = g.head_dim == 256 ? 2 : 4;
+    } else if (g.head_dim == 128 && rows > kMmaRows) {
+        p.tiles = rows > 128 ? 2 : 1;
+        p.rows = 128 * p.tiles;
+        per_sm = p.tiles == 1 ? 2 : 1;
+        keys = 128;
+        p.min_units = 2;
+    } else {
+        p.rows = g.head_dim == 256 || rows <= 8 ? 8 : 16;
+        per_sm = tree_mma_ctas_per_sm(plain, (int)g.head_dim, p.rows);
     }
-    const int64_t ctas = std::max<int64_t>(1, g.num_seqs * g.num_kv_heads * ceil_div(p.rows, per_cta));
     const int64_t cap = std::max<int64_t>(1, g.max_blocks_per_seq * g.block_size);
-    const int64_t want = std::max<int64_t>(1, 4 * slots / ctas);  // partitions
-    int64_t part = std::max<int64_t>(kMinPart, ceil_div(ceil_div(cap, want), 128) * 128);
-    p.part = (int)std::min<int64_t>(part, kMaxPart);
-    p.P = (int)ceil_div(cap, p.part);
+    const int64_t blocks = ceil_div(cap, keys);  // of the longest sequence
+    const int64_t items = g.num_seqs * g.num_kv_heads * ceil_div(rows, p.rows);
+    const int64_t slots = (int64_t)sm_count() * per_sm;
+    p.split = blocks > p.min_units;
+    p.ctas = (int)(items >= slots ? slots : std::min(slots, items * blocks));
     return p;
 }
 
@@ -447,20 +482,15 @@ int check_tree_args(const qf_paged_tree_attention_args& g) {
 }
 
 size_t plan_bytes(const qf_paged_tree_attention_args& g, const TreePlan& p) {
-    if (p.P <= 1) return 0;
-    int64_t n = 0;
-    if (__builtin_mul_overflow(g.num_tokens, g.num_q_heads, &n) ||
-        __builtin_mul_overflow(n, (int64_t)p.P, &n) ||
-        __builtin_mul_overflow(n, (g.head_dim + 2) * (int64_t)sizeof(float), &n))
-        return SIZE_MAX;
-    return (size_t)n;
+    if (!p.split || p.ctas < 2) return 0;
+    return (size_t)TreeWs::floats(p.ctas, p.rows, g.head_dim) * sizeof(float);
 }
 
-int launch_tree_f32(const TreeDev& a, int format, int D, cudaStream_t stream) {
+int launch_tree_f32(const TreeDev& a, int format, int D, int rows, int ctas, cudaStream_t stream) {
     switch (format) {
-    case QF_CACHE_PLAIN: return launch_f32<QF_CACHE_PLAIN>(a, D, stream);
-    case QF_CACHE_E4M3: return launch_f32<QF_CACHE_E4M3>(a, D, stream);
-    default: return launch_f32<QF_CACHE_INT8>(a, D, stream);
+    case QF_CACHE_PLAIN: return launch_f32<QF_CACHE_PLAIN>(a, D, rows, ctas, stream);
+    case QF_CACHE_E4M3: return launch_f32<QF_CACHE_E4M3>(a, D, rows, ctas, stream);
+    default: return launch_f32<QF_CACHE_INT8>(a, D, rows, ctas, stream);
     }
 }
 
@@ -481,13 +511,10 @@ extern "C" int qf_paged_tree_attention(const qf_paged_tree_attention_args* p, cu
     const qf_paged_tree_attention_args& g = *p;
     int rc = qf::check_tree_args(g);
     if (rc || g.num_tokens == 0) return rc;
-    qf::TreePlan plan = qf::make_plan(g);
+    const qf::TreePlan plan = qf::make_plan(g);
     const size_t need = qf::plan_bytes(g, plan);
     if (need > 0 && g.workspace) {
         if (g.workspace_bytes < 0 || (size_t)g.workspace_bytes < need) return QF_ERR_INVALID;
-    } else {
-        plan.P = 1;
-        plan.part = qf::kMaxPart;
     }
     qf::TreeDev a{};
     a.q = static_cast<const char*>(g.q);
@@ -522,22 +549,21 @@ extern "C" int qf_paged_tree_attention(const qf_paged_tree_attention_args* p, cu
     a.out = static_cast<char*>(g.out);
     a.ot = g.out_stride_token;
     a.oh = g.out_stride_head;
-    a.ws = static_cast<float*>(g.workspace);
-    a.P = plan.P;
-    a.part = plan.part;
+    a.ws = need > 0 ? static_cast<float*>(g.workspace) : nullptr;
+    a.min_units = plan.min_units;
     a.status = g.status;
     const int D = (int)g.head_dim;
     if (g.dtype == QF_F32)
-        rc = qf::launch_tree_f32(a, g.cache_format, D, stream);
+        rc = qf::launch_tree_f32(a, g.cache_format, D, plan.rows, plan.ctas, stream);
     else if (plan.tiles)
-        rc = qf::launch_tree_tc(a, g.dtype, g.cache_format, plan.tiles, stream);
+        rc = qf::launch_tree_tc(a, g.dtype, g.cache_format, plan.tiles, plan.ctas, stream);
     else
-        rc = qf::launch_tree_mma(a, g.dtype, g.cache_format, D, (int)plan.rows, stream);
-    if (rc || a.P == 1) return rc;
+        rc = qf::launch_tree_mma(a, g.dtype, g.cache_format, D, plan.rows, plan.ctas, stream);
+    if (rc || !a.ws) return rc;
     switch (g.dtype) {
-    case QF_F32: return qf::launch_merge<float>(a, D, stream);
-    case QF_F16: return qf::launch_merge<__half>(a, D, stream);
-    default: return qf::launch_merge<__nv_bfloat16>(a, D, stream);
+    case QF_F32: return qf::launch_merge<float>(a, D, plan.rows, plan.ctas, stream);
+    case QF_F16: return qf::launch_merge<__half>(a, D, plan.rows, plan.ctas, stream);
+    default: return qf::launch_merge<__nv_bfloat16>(a, D, plan.rows, plan.ctas, stream);
     }
 }
 

@@ -3,11 +3,12 @@
 // cache.  Bound by HBM: every K and V row is read once and meets at most 16
 // rows.
 //
-// Warps take tiles of 16 keys in turn; nothing of K or V passes through shared
-// memory.  The reduction index of a matrix product may be permuted as long as
-// both operands agree, and so may the index of its output columns, so each
-// lane loads whole 16-byte pieces of rows and calls them the fragment
-// elements that mma.sync m16n8k16 wants of it:
+// Warps take tiles of 16 keys in turn, each through a ring of its own in shared
+// memory that cp.async fills three or four tiles deep: 40 KB and more per SM in
+// flight whatever the registers hold.  The reduction index of a matrix product may
+// be permuted as long as both operands agree, and so may the index of its output
+// columns, so each lane reads whole 16-byte pieces of rows and calls them the
+// fragment elements that mma.sync m16n8k16 wants of it; no transposing loads:
 //  * S = Q K^T (rows x keys): B = K^T.  Lane (gid, tig) = (lane / 4, lane % 4)
 //    owns keys gid and gid + 8 and, of their rows, 16-byte chunks tig + 4 i; four
 //    consecutive elements are its four of one k-step, and Q's fragments are
@@ -18,16 +19,13 @@
 //    rows; a byte permute pairs two keys' elements of one dim.  With the rows
 //    as the 8-wide index, 8 rows cost half of what they would as the 16-wide.
 // Codes become fp16 in registers (both formats are exact there).  Their row
-// scales never touch the codes: K's multiplies the score, V's enters the
-// exponent, p' = 2^(t + log2 scale - m'), with a running maximum m' of its own,
-// so that p' is in [0, 1] however the scales vary.  Queries become fp16 after a
-// power-of-two row factor that puts their largest element in [2^14, 2^15): exact
-// for every element within 2^-28 of it.
+// scales never touch the codes: K's multiplies the score t, V's enters the
+// exponent, p' = 2^(t + log2 vs - m) with m the maximum of that sum, so that p' is
+// in [0, 1] however the scales vary; the row's sum takes 2^(t - m), and O / l is the
+// definition.  Queries become fp16 after a power-of-two row factor that puts
+// their largest element in [2^14, 2^15): exact for every element within 2^-28 of it.
 // P goes in as a 16-bit high part and the rounded remainder, so the product
 // keeps 16 significant bits or more of p; sums and maxima are fp32.
-//
-// Per warp one K tile is in flight while the one before is multiplied, and V is
-// issued before QK: 8 to 12 resident warps keep 40 KB or more per SM in flight.
 #include <math.h>
 
 #include "qf_mma.cuh"
@@ -57,12 +55,34 @@ __device__ __forceinline__ bool word_not_finite(uint32_t w) {
     }
 }
 
+template <int FMT, int D>
+struct MmaRing {
+    static constexpr int EB = FMT == QF_CACHE_PLAIN ? 2 : 1;
+    static constexpr int ROW = D * EB;                // bytes per cache row
+    static constexpr int NCH = ROW / 16;              // 16-byte chunks per row
+    static constexpr int MAT = 16 * ROW;              // one tile of K or V
+    static constexpr int STAGE = 2 * MAT + 128 + 16;  // K, V, 16 + 16 scales, valid bits
+    static constexpr int STAGES = MAT <= 2048 ? 4 : 3;
+    static constexpr int WARP = STAGE * STAGES;
+    static constexpr int SMEM = kWarps * WARP;
+    // Byte offset of 16-byte chunk c of row r: the rows that a quarter of a warp
+    // reads together (r and r + 1 of K, every other one of V) hold one chunk index in
+    // different banks.
+    __device__ __forceinline__ static int off(int r, int c) {
+        const int f = NCH >= 8 ? (r & 6) ^ ((r & 1) << 2) : (r >> 1) & 3;
+        return r * ROW + ((c ^ f) << 4);
+    }
+};
+
+constexpr int kMmaKeys = 16 * kWarps;  // keys of a work unit
+
 template <typename T, int FMT, int D, int NR>
 __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) {
     constexpr bool Q8 = FMT != QF_CACHE_PLAIN;
     using MT = typename std::conditional<Q8, __half, T>::type;  // the products' operand type
     using MP = Packed<MT>;
-    constexpr int EB = Q8 ? 1 : 2;                // bytes per cache element
+    using R = MmaRing<FMT, D>;
+    constexpr int EB = R::EB, ST = R::STAGES;
     constexpr int KS = D / 16;                    // k-steps of Q K^T
     constexpr int NRT = NR / 8;                   // 8-row tiles
     constexpr int KCH = D * EB / 64;              // 16-byte chunks of a K row per lane
@@ -71,403 +91,431 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
     constexpr int VW = VB / 4;                    // words per V chunk
     constexpr int EPC = VB / EB;                  // dims per V chunk
     constexpr int MTN = D / 16;                   // 16-dim tiles of O^T
+    static_assert(kWarps * NR * (D + 2) * 4 <= R::SMEM, "merge area");
 
-    const int p = blockIdx.x, s = blockIdx.z;
-    const int g = blockIdx.y % a.Hkv, rg = blockIdx.y / a.Hkv;
-    const TreeSeq w = tree_seq(a, s);
-    if (p == 0 && rg == 0) zero_unowned_rows<T, D>(a, s, g, w);
-    const int rows = w.n * a.G, r0 = rg * NR;
-    if (p >= w.nparts || r0 >= rows) return;
-    const int k_begin = p * a.part, k_end = k_begin + min(w.L - k_begin, a.part);
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int64_t scratch[34];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
-    const int32_t* bt = a.bt + (int64_t)s * a.bts;
     const float sl2 = a.scale * 1.4426950408889634f;
+    unsigned char* ring = smem + warp * R::WARP;
 
-    // Q fragments, rows gid and gid + 8 of the tile, four consecutive dims per k-step
-    uint32_t qa[KS][2 * NRT];
-    float rs[NRT];  // what a row's products are multiplied by
-    const int64_t* mrow[NRT];
-#pragma unroll
-    for (int nt = 0; nt < NRT; ++nt) {
-        const int r = r0 + nt * 8 + gid, tok = r / a.G;
-        const bool live = r < rows;
-        const char* qp = a.q + ((int64_t)(w.q0 + (live ? tok : 0)) * a.qt +
-                                (int64_t)(g * a.G + (live ? r - tok * a.G : 0)) * a.qh) * 2;
-        mrow[nt] = a.mask + (int64_t)(w.q0 + (live ? tok : 0)) * a.words;
-        uint2 raw[KS];
-        uint32_t mx = 0;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int d = Q8 ? (ks >> 2) * 64 + tig * 16 + (ks & 3) * 4
-                             : (ks >> 1) * 32 + tig * 8 + (ks & 1) * 4;
-            raw[ks] = live ? __ldg(reinterpret_cast<const uint2*>(qp + d * 2)) : make_uint2(0, 0);
-            if constexpr (Q8) {
-                using P = Packed<T>;
-                mx = max(max(mx, __float_as_uint(P::lo(raw[ks].x)) & 0x7fffffffu),
-                         __float_as_uint(P::hi(raw[ks].x)) & 0x7fffffffu);
-                mx = max(max(mx, __float_as_uint(P::lo(raw[ks].y)) & 0x7fffffffu),
-                         __float_as_uint(P::hi(raw[ks].y)) & 0x7fffffffu);
+    TreeWalk<kMmaKeys, NR> walk;
+    walk.begin(a, scratch);
+    zero_unowned_rows<T, D>(a);
+    if (tid == 0) walk.record(a);
+
+    TreeSeg sg;
+    while (walk.next(a, sg)) {
+        const TreeSeq& w = sg.w;
+        const int rows = w.n * a.G, r0 = sg.rg * NR, g = sg.g;
+        const int32_t* bt = a.bt + (int64_t)sg.s * a.bts;
+        const int ntiles = (sg.k_end - sg.k_begin + 15) / 16;  // (0: no key at all)
+
+        // copies of tile i (of this warp: 4 i + warp) into its stage; one group each
+        int ahead_blk = 0;  // the block of this lane's key of the tile issued next
+        auto look = [&](int i) {
+            const int j = sg.k_begin + (i * kWarps + warp) * 16 + (lane & 15);
+            if (j < sg.k_end) ahead_blk = __ldg(bt + a.B.div(j));
+        };
+        auto issue = [&](int i) {
+            const int j = sg.k_begin + (i * kWarps + warp) * 16 + (lane & 15);
+            bool ok = j < sg.k_end;
+            const int64_t blk = ahead_blk;
+            if (ok && (blk < 0 || blk >= a.N)) {
+                flag(a.status, QF_FLAG_BAD_BLOCK);
+                ok = false;
             }
-        }
-        rs[nt] = sl2;
-        float f = 1.f;
-        if constexpr (Q8) {
-            mx = max(mx, __shfl_xor_sync(kAll, mx, 1));
-            mx = max(mx, __shfl_xor_sync(kAll, mx, 2));
-            // largest element's exponent e: factor 2^(14 - e), its inverse with the scores
-            const int e = min(max((int)(mx >> 23) - 127, -100), 127);
-            f = __int_as_float((127 + 14 - e) << 23);
-            rs[nt] = sl2 * __int_as_float((127 - 14 + e) << 23);
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (Q8) {
-                using P = Packed<T>;
-                qa[ks][nt] = MP::pack(P::lo(raw[ks].x) * f, P::hi(raw[ks].x) * f);
-                qa[ks][NRT + nt] = MP::pack(P::lo(raw[ks].y) * f, P::hi(raw[ks].y) * f);
-            } else {
-                qa[ks][nt] = raw[ks].x;
-                qa[ks][NRT + nt] = raw[ks].y;
+            const int slot = j - a.B.div(j) * a.B.d;
+            int64_t row = 0, srow = 0;
+            if (ok) {
+                row = (blk * a.c0 + (int64_t)g * a.c1 + (int64_t)slot * a.c2) * EB;
+                srow = blk * a.s0 + (int64_t)g * a.s1 + (int64_t)slot * a.s2;
             }
-        }
-    }
-
-    float acc[NRT][MTN][4];
-    float m[NRT], mo[NRT], l[NRT];  // max of t, max of t + log2 v-scale, this lane's sum
+            look(i + 1);
+            const unsigned valid = __ballot_sync(kAll, ok) & 0xffffu;
+            unsigned char* kt = ring + (i % ST) * R::STAGE;
+            unsigned char* vt = kt + R::MAT;
+            if (valid) {
 #pragma unroll
-    for (int nt = 0; nt < NRT; ++nt) {
-        m[nt] = mo[nt] = -INFINITY;
-        l[nt] = 0.f;
-#pragma unroll
-        for (int i = 0; i < MTN; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
-    }
-
-    // lane k < 16: where key j0 + k is, and its scales; the tile's valid keys as a mask
-    struct Tile {
-        int64_t row;
-        float ks, lv;
-        unsigned valid;
-    };
-    auto locate = [&](int j0) {
-        Tile t{0, 0.f, 0.f, 0u};
-        bool ok = false;
-        int64_t srow = 0;
-        if (lane < 16 && j0 + lane < k_end) ok = key_place(a, bt, g, j0 + lane, t.row, srow);
-        if (Q8 && ok) {
-            t.ks = __ldg(a.ks + srow);
-            t.lv = __log2f(__ldg(a.vs + srow));
-        }
-        t.valid = __ballot_sync(kAll, ok);
-        return t;
-    };
-    uint4 kf[2][KCH];
-    auto load_k = [&](const Tile& t) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int64_t row = __shfl_sync(kAll, t.row, n * 8 + gid);
-            const bool ok = (t.valid >> (n * 8 + gid)) & 1;
-#pragma unroll
-            for (int i = 0; i < KCH; ++i)
-                kf[n][i] = ok ? ld_stream16(a.kc + row * EB + i * 64 + tig * 16) : make_uint4(0, 0, 0, 0);
-        }
-    };
-
-    int j0 = k_begin + warp * 16;
-    Tile cur = locate(j0);  // (no key at all: an empty mask, no loads)
-    load_k(cur);
-    for (; j0 < k_end; j0 += kWarps * 16) {
-        // V rows of keys 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9
-        uint32_t vf[4][VCH][VW];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = 2 * tig + (i & 1) + (i >> 1) * 8;
-            const int64_t row = __shfl_sync(kAll, cur.row, k);
-            const bool ok = (cur.valid >> k) & 1;
-#pragma unroll
-            for (int c = 0; c < VCH; ++c) {
-                const char* vp = a.vc + row * EB + c * 128 + gid * VB;
-                if constexpr (VB == 16) {
-                    const uint4 v = ok ? ld_stream16(vp) : make_uint4(0, 0, 0, 0);
-                    vf[i][c][0] = v.x, vf[i][c][1] = v.y, vf[i][c][2] = v.z, vf[i][c][3] = v.w;
-                } else {
-                    const uint2 v = ok ? ld_stream8(vp) : make_uint2(0, 0);
-                    vf[i][c][0] = v.x, vf[i][c][1] = v.y;
+                for (int x = 0; x < R::NCH / 2; ++x) {
+                    const int idx = x * 32 + lane, r = idx / R::NCH, c = idx % R::NCH;
+                    const int64_t o = __shfl_sync(kAll, row, r);
+                    const int bytes = (valid >> r) & 1 ? 16 : 0;
+                    cp_async16(kt + R::off(r, c), a.kc + o + c * 16, bytes);
+                    cp_async16(vt + R::off(r, c), a.vc + o + c * 16, bytes);
                 }
+                if (Q8 && ok)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(
+                                     __cvta_generic_to_shared(kt + 2 * R::MAT + lane * 4))),
+                                 "l"((lane < 16 ? a.ks : a.vs) + srow)
+                                 : "memory");
+                if (lane == 0) *reinterpret_cast<unsigned*>(kt + 2 * R::MAT + 128) = valid;
+            } else if (lane == 0) {
+                *reinterpret_cast<unsigned*>(kt + 2 * R::MAT + 128) = 0u;
             }
-        }
-        Tile next = locate(j0 + kWarps * 16);
+            cp_async_commit();
+        };
+        look(0);
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) issue(i);
 
-        // S = Q K^T
-        float sc[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-        for (int i = 0; i < KCH; ++i) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-#pragma unroll
-                for (int x = 0; x < (Q8 ? 4 : 2); ++x) {
-                    const int ks = i * (Q8 ? 4 : 2) + x;
-                    uint32_t b0, b1;
-                    if constexpr (Q8) codes_to_f16<FMT>(word(kf[n][i], x), b0, b1);
-                    else b0 = word(kf[n][i], 2 * x), b1 = word(kf[n][i], 2 * x + 1);
-                    const uint32_t fr[4] = {qa[ks][0], NRT == 2 ? qa[ks][1] : 0u, qa[ks][NRT],
-                                            NRT == 2 ? qa[ks][2 * NRT - 1] : 0u};
-                    Mma<MT>::run(sc[n], fr, b0, b1);
-                }
-            }
-        }
-        load_k(next);
-
-        // online softmax; this lane: rows gid (+ 8), keys 8 n + 2 tig + e
-        const bool draft = a.cu && j0 + 16 > w.ctx;
-        float ksv[2][2], lvv[2][2];
-        if constexpr (Q8) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    ksv[n][e] = __shfl_sync(kAll, cur.ks, 8 * n + 2 * tig + e);
-                    lvv[n][e] = __shfl_sync(kAll, cur.lv, 8 * n + 2 * tig + e);
-                }
-        }
-        float pw[NRT][2][2];
-        unsigned seen[NRT];
-        uint32_t ph[NRT][2], pl[NRT][2];
-        float corr[NRT];
-        bool moved = false;
+        // Q fragments, rows gid and gid + 8 of the tile, four consecutive dims per k-step
+        uint32_t qa[KS][2 * NRT];
+        float rs[NRT];  // what a row's products are multiplied by
+        const int64_t* mrow[NRT];
 #pragma unroll
         for (int nt = 0; nt < NRT; ++nt) {
-            seen[nt] = cur.valid;
-            if (draft) seen[nt] &= tree_bits32(mrow[nt], a.words, j0 - w.ctx);
-            float t[2][2], u[2][2], mx = -INFINITY, mu = -INFINITY;
+            const int r = r0 + nt * 8 + gid, tok = r / a.G;
+            const bool live = r < rows;
+            const char* qp = a.q + ((int64_t)(w.q0 + (live ? tok : 0)) * a.qt +
+                                    (int64_t)(g * a.G + (live ? r - tok * a.G : 0)) * a.qh) * 2;
+            mrow[nt] = a.mask + (int64_t)(w.q0 + (live ? tok : 0)) * a.words;
+            uint2 raw[KS];
+            uint32_t mx = 0;
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const bool ok = (seen[nt] >> (8 * n + 2 * tig + e)) & 1;
-                    float x = sc[n][2 * nt + e] * rs[nt];
-                    if constexpr (Q8) x *= ksv[n][e];
-                    t[n][e] = ok ? x : -INFINITY;
-                    mx = fmaxf(mx, t[n][e]);
-                    if constexpr (Q8) {
-                        u[n][e] = ok ? x + lvv[n][e] : -INFINITY;
-                        mu = fmaxf(mu, u[n][e]);
-                    }
+            for (int ks = 0; ks < KS; ++ks) {
+                const int d = Q8 ? (ks >> 2) * 64 + tig * 16 + (ks & 3) * 4
+                                 : (ks >> 1) * 32 + tig * 8 + (ks & 1) * 4;
+                raw[ks] = live ? __ldg(reinterpret_cast<const uint2*>(qp + d * 2)) : make_uint2(0, 0);
+                if constexpr (Q8) {
+                    using P = Packed<T>;
+                    mx = max(max(mx, __float_as_uint(P::lo(raw[ks].x)) & 0x7fffffffu),
+                             __float_as_uint(P::hi(raw[ks].x)) & 0x7fffffffu);
+                    mx = max(max(mx, __float_as_uint(P::lo(raw[ks].y)) & 0x7fffffffu),
+                             __float_as_uint(P::hi(raw[ks].y)) & 0x7fffffffu);
                 }
-            mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 2));
-            const float mn = fmaxf(m[nt], mx), base = mn == -INFINITY ? 0.f : mn;
-            const float cl = pow2(m[nt] - base);
-            m[nt] = mn;
-            corr[nt] = cl;
-            float sum = 0.f, obase = base;
+            }
+            rs[nt] = sl2;
+            float f = 1.f;
             if constexpr (Q8) {
-                mu = fmaxf(mu, __shfl_xor_sync(kAll, mu, 1));
-                mu = fmaxf(mu, __shfl_xor_sync(kAll, mu, 2));
-                const float un = fmaxf(mo[nt], mu);
-                obase = un == -INFINITY ? 0.f : un;
-                corr[nt] = pow2(mo[nt] - obase);
-                mo[nt] = un;
+                mx = max(mx, __shfl_xor_sync(kAll, mx, 1));
+                mx = max(mx, __shfl_xor_sync(kAll, mx, 2));
+                // largest element's exponent e: factor 2^(14 - e), its inverse with the scores
+                const int e = min(max((int)(mx >> 23) - 127, -100), 127);
+                f = __int_as_float((127 + 14 - e) << 23);
+                rs[nt] = sl2 * __int_as_float((127 - 14 + e) << 23);
             }
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float pr = pow2(t[n][e] - base);
-                    sum += pr;
-                    pw[nt][n][e] = Q8 ? pow2(u[n][e] - obase) : pr;
-                }
-            l[nt] = l[nt] * cl + sum;
-            moved |= corr[nt] != 1.f;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                ph[nt][n] = MP::pack(pw[nt][n][0], pw[nt][n][1]);
-                pl[nt][n] = MP::pack(pw[nt][n][0] - MP::lo(ph[nt][n]), pw[nt][n][1] - MP::hi(ph[nt][n]));
-            }
-        }
-        if (__any_sync(kAll, moved)) {
-#pragma unroll
-            for (int nt = 0; nt < NRT; ++nt) {
-                const float c0 = __shfl_sync(kAll, corr[nt], 8 * tig);
-                const float c1 = __shfl_sync(kAll, corr[nt], 8 * tig + 4);
-#pragma unroll
-                for (int i = 0; i < MTN; ++i) {
-                    acc[nt][i][0] *= c0;
-                    acc[nt][i][1] *= c1;
-                    acc[nt][i][2] *= c0;
-                    acc[nt][i][3] *= c1;
+            for (int ks = 0; ks < KS; ++ks) {
+                if constexpr (Q8) {
+                    using P = Packed<T>;
+                    qa[ks][nt] = MP::pack(P::lo(raw[ks].x) * f, P::hi(raw[ks].x) * f);
+                    qa[ks][NRT + nt] = MP::pack(P::lo(raw[ks].y) * f, P::hi(raw[ks].y) * f);
+                } else {
+                    qa[ks][nt] = raw[ks].x;
+                    qa[ks][NRT + nt] = raw[ks].y;
                 }
             }
         }
 
-        // An infinity or a NaN in the V of a drafted key that some row does not
-        // see: 0 times it is not 0, so such a (rare) tile is added up key by key,
-        // a row's unseen keys left out.
-        bool odd = false;
-        if (draft) {
+        float acc[NRT][MTN][4];
+        float m[NRT], l[NRT];  // reference: max of t (+ log2 v-scale); this lane's sum against it
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int nt = 0; nt < NRT; ++nt) {
+            m[nt] = -INFINITY;
+            l[nt] = 0.f;
 #pragma unroll
-                for (int c = 0; c < VCH; ++c)
-#pragma unroll
-                    for (int x = 0; x < VW; ++x) odd |= word_not_finite<T, FMT>(vf[i][c][x]);
-            odd = __any_sync(kAll, odd);
+            for (int i = 0; i < MTN; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
         }
-        if (odd) {
-            for (int k = 0; k < 16; ++k) {
-                const int64_t row = __shfl_sync(kAll, cur.row, k);
-                float pr[NRT][2];
-                bool in[NRT][2];
+
+        for (int i = 0; i * kWarps + warp < ntiles; ++i) {
+            issue(i + ST - 1);
+            cp_async_wait<ST - 1>();
+            __syncwarp();
+            const int j0 = sg.k_begin + (i * kWarps + warp) * 16;
+            const unsigned char* kt = ring + (i % ST) * R::STAGE;
+            const unsigned char* vt = kt + R::MAT;
+            const unsigned valid = *reinterpret_cast<const unsigned*>(kt + 2 * R::MAT + 128);
+            if (valid) {
+                // S = Q K^T
+                float sc[2][4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+                for (int c = 0; c < KCH; ++c) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const uint4 kf = *reinterpret_cast<const uint4*>(kt + R::off(n * 8 + gid, tig + 4 * c));
+#pragma unroll
+                        for (int x = 0; x < (Q8 ? 4 : 2); ++x) {
+                            const int ks = c * (Q8 ? 4 : 2) + x;
+                            uint32_t b0, b1;
+                            if constexpr (Q8) codes_to_f16<FMT>(word(kf, x), b0, b1);
+                            else b0 = word(kf, 2 * x), b1 = word(kf, 2 * x + 1);
+                            const uint32_t fr[4] = {qa[ks][0], NRT == 2 ? qa[ks][1] : 0u, qa[ks][NRT],
+                                                    NRT == 2 ? qa[ks][2 * NRT - 1] : 0u};
+                            Mma<MT>::run(sc[n], fr, b0, b1);
+                        }
+                    }
+                }
+
+                // online softmax; this lane: rows gid (+ 8), keys 8 n + 2 tig + e
+                const bool draft = a.cu && j0 + 16 > w.ctx;
+                float ksv[2][2], lvv[2][2];
+                if constexpr (Q8) {
+                    const float* sp = reinterpret_cast<const float*>(kt + 2 * R::MAT);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const float2 k2 = *reinterpret_cast<const float2*>(sp + 8 * n + 2 * tig);
+                        const float2 v2 = *reinterpret_cast<const float2*>(sp + 16 + 8 * n + 2 * tig);
+                        ksv[n][0] = k2.x, ksv[n][1] = k2.y;
+                        // a scale of 0 (a row never written) stands for zeros, as good as at 2^-120
+                        lvv[n][0] = __log2f(v2.x < kLeastScale ? kLeastScale : v2.x);
+                        lvv[n][1] = __log2f(v2.y < kLeastScale ? kLeastScale : v2.y);
+                    }
+                }
+                float pw[NRT][2][2];
+                unsigned seen[NRT];
+                uint32_t ph[NRT][2], pl[NRT][2];
+                float corr[NRT];
+                bool moved = false;
 #pragma unroll
                 for (int nt = 0; nt < NRT; ++nt) {
+                    seen[nt] = valid;
+                    if (draft) seen[nt] &= tree_bits32(mrow[nt], a.words, j0 - w.ctx);
+                    float t[2][2], u[2][2], mx = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {  // rows 2 tig + e: lanes 4 (2 tig + e) + key pair
-                        const int from = 4 * (2 * tig + e) + ((k & 7) >> 1);
-                        const float x0 = __shfl_sync(kAll, pw[nt][0][0], from);
-                        const float x1 = __shfl_sync(kAll, pw[nt][0][1], from);
-                        const float x2 = __shfl_sync(kAll, pw[nt][1][0], from);
-                        const float x3 = __shfl_sync(kAll, pw[nt][1][1], from);
-                        pr[nt][e] = k < 8 ? (k & 1 ? x1 : x0) : (k & 1 ? x3 : x2);
-                        in[nt][e] = (__shfl_sync(kAll, seen[nt], from) >> k) & 1;
-                    }
-                }
-                if (!((cur.valid >> k) & 1)) continue;
+                    for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int i = 0; i < MTN; ++i) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int d = (i / (EPC / 2)) * (EPC * 8) + gid * EPC + 2 * (i % (EPC / 2)) + half;
-                        float v;
-                        if constexpr (Q8) v = code_to_float<FMT>(reinterpret_cast<const uint8_t*>(a.vc)[row + d]);
-                        else v = Dt<T>::to_f(reinterpret_cast<const T*>(a.vc)[row + d]);
-#pragma unroll
-                        for (int nt = 0; nt < NRT; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                if (in[nt][e]) acc[nt][i][2 * half + e] = fmaf(pr[nt][e], v, acc[nt][i][2 * half + e]);
-                    }
-                }
-            }
-        } else {
-            // O^T += V^T P^T
-#pragma unroll
-            for (int c = 0; c < VCH; ++c) {
-#pragma unroll
-                for (int x = 0; x < VW; ++x) {
-#pragma unroll
-                    for (int half = 0; half < (Q8 ? 2 : 1); ++half) {
-                        uint32_t va[4];
-                        if constexpr (Q8) {
-                            const uint32_t sel = half ? 0x7362u : 0x5140u;
-                            codes_to_f16<FMT>(__byte_perm(vf[0][c][x], vf[1][c][x], sel), va[0], va[1]);
-                            codes_to_f16<FMT>(__byte_perm(vf[2][c][x], vf[3][c][x], sel), va[2], va[3]);
-                        } else {
-                            va[0] = __byte_perm(vf[0][c][x], vf[1][c][x], 0x5410);
-                            va[1] = __byte_perm(vf[0][c][x], vf[1][c][x], 0x7632);
-                            va[2] = __byte_perm(vf[2][c][x], vf[3][c][x], 0x5410);
-                            va[3] = __byte_perm(vf[2][c][x], vf[3][c][x], 0x7632);
+                        for (int e = 0; e < 2; ++e) {
+                            const bool ok = (seen[nt] >> (8 * n + 2 * tig + e)) & 1;
+                            float x = sc[n][2 * nt + e] * rs[nt];
+                            if constexpr (Q8) x *= ksv[n][e];
+                            t[n][e] = ok ? x : -INFINITY;
+                            u[n][e] = Q8 ? (ok ? x + lvv[n][e] : -INFINITY) : t[n][e];
+                            mx = fmaxf(mx, u[n][e]);
                         }
-                        const int i = c * (EPC / 2) + (Q8 ? 2 * x + half : x);
+                    mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 2));
+                    const float mn = fmaxf(m[nt], mx), base = mn == -INFINITY ? 0.f : mn;
+                    corr[nt] = pow2(m[nt] - base);
+                    m[nt] = mn;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            pw[nt][n][e] = pow2(u[n][e] - base);
+                            sum += Q8 ? pow2(t[n][e] - base) : pw[nt][n][e];
+                        }
+                    l[nt] = l[nt] * corr[nt] + sum;
+                    moved |= corr[nt] != 1.f;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        ph[nt][n] = MP::pack(pw[nt][n][0], pw[nt][n][1]);
+                        pl[nt][n] = MP::pack(pw[nt][n][0] - MP::lo(ph[nt][n]), pw[nt][n][1] - MP::hi(ph[nt][n]));
+                    }
+                }
+                if (__any_sync(kAll, moved)) {
+#pragma unroll
+                    for (int nt = 0; nt < NRT; ++nt) {
+                        const float c0 = __shfl_sync(kAll, corr[nt], 8 * tig);
+                        const float c1 = __shfl_sync(kAll, corr[nt], 8 * tig + 4);
+#pragma unroll
+                        for (int x = 0; x < MTN; ++x) {
+                            acc[nt][x][0] *= c0;
+                            acc[nt][x][1] *= c1;
+                            acc[nt][x][2] *= c0;
+                            acc[nt][x][3] *= c1;
+                        }
+                    }
+                }
+
+                // V rows of keys 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9
+                uint32_t vf[4][VCH][VW];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int k = 2 * tig + (x & 1) + (x >> 1) * 8;
+#pragma unroll
+                    for (int c = 0; c < VCH; ++c) {
+                        if constexpr (VB == 16) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(vt + R::off(k, gid + 8 * c));
+                            vf[x][c][0] = v.x, vf[x][c][1] = v.y, vf[x][c][2] = v.z, vf[x][c][3] = v.w;
+                        } else {
+                            const uint2 v = *reinterpret_cast<const uint2*>(vt + R::off(k, gid >> 1) + (gid & 1) * 8);
+                            vf[x][c][0] = v.x, vf[x][c][1] = v.y;
+                        }
+                    }
+                }
+                // An infinity or a NaN in the V of a drafted key that some row does not
+                // see: 0 times it is not 0, so such a (rare) tile is added up key by key,
+                // a row's unseen keys left out.
+                bool odd = false;
+                if (draft) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int c = 0; c < VCH; ++c)
+#pragma unroll
+                            for (int y = 0; y < VW; ++y) odd |= word_not_finite<T, FMT>(vf[x][c][y]);
+                    odd = __any_sync(kAll, odd);
+                }
+                if (odd) {
+                    for (int k = 0; k < 16; ++k) {
+                        float pr[NRT][2];
+                        bool in[NRT][2];
 #pragma unroll
                         for (int nt = 0; nt < NRT; ++nt) {
-                            Mma<MT>::run(acc[nt][i], va, ph[nt][0], ph[nt][1]);
-                            Mma<MT>::run(acc[nt][i], va, pl[nt][0], pl[nt][1]);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {  // rows 2 tig + e: lanes 4 (2 tig + e) + key pair
+                                const int from = 4 * (2 * tig + e) + ((k & 7) >> 1);
+                                const float x0 = __shfl_sync(kAll, pw[nt][0][0], from);
+                                const float x1 = __shfl_sync(kAll, pw[nt][0][1], from);
+                                const float x2 = __shfl_sync(kAll, pw[nt][1][0], from);
+                                const float x3 = __shfl_sync(kAll, pw[nt][1][1], from);
+                                pr[nt][e] = k < 8 ? (k & 1 ? x1 : x0) : (k & 1 ? x3 : x2);
+                                in[nt][e] = (__shfl_sync(kAll, seen[nt], from) >> k) & 1;
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < MTN; ++x) {
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const int d = (x / (EPC / 2)) * (EPC * 8) + gid * EPC + 2 * (x % (EPC / 2)) + half;
+                                const unsigned char* at = vt + R::off(k, d * EB / 16) + (d * EB & 15);
+                                float v;
+                                if constexpr (Q8) v = code_to_float<FMT>(*at);
+                                else v = Dt<T>::to_f(*reinterpret_cast<const T*>(at));
+#pragma unroll
+                                for (int nt = 0; nt < NRT; ++nt)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e)
+                                        if (in[nt][e])
+                                            acc[nt][x][2 * half + e] = fmaf(pr[nt][e], v, acc[nt][x][2 * half + e]);
+                            }
+                        }
+                    }
+                } else {
+                    // O^T += V^T P^T
+#pragma unroll
+                    for (int c = 0; c < VCH; ++c) {
+#pragma unroll
+                        for (int x = 0; x < VW; ++x) {
+#pragma unroll
+                            for (int half = 0; half < (Q8 ? 2 : 1); ++half) {
+                                uint32_t va[4];
+                                if constexpr (Q8) {
+                                    const uint32_t sel = half ? 0x7362u : 0x5140u;
+                                    codes_to_f16<FMT>(__byte_perm(vf[0][c][x], vf[1][c][x], sel), va[0], va[1]);
+                                    codes_to_f16<FMT>(__byte_perm(vf[2][c][x], vf[3][c][x], sel), va[2], va[3]);
+                                } else {
+                                    va[0] = __byte_perm(vf[0][c][x], vf[1][c][x], 0x5410);
+                                    va[1] = __byte_perm(vf[0][c][x], vf[1][c][x], 0x7632);
+                                    va[2] = __byte_perm(vf[2][c][x], vf[3][c][x], 0x5410);
+                                    va[3] = __byte_perm(vf[2][c][x], vf[3][c][x], 0x7632);
+                                }
+                                const int y = c * (EPC / 2) + (Q8 ? 2 * x + half : x);
+#pragma unroll
+                                for (int nt = 0; nt < NRT; ++nt) {
+                                    Mma<MT>::run(acc[nt][y], va, ph[nt][0], ph[nt][1]);
+                                    Mma<MT>::run(acc[nt][y], va, pl[nt][0], pl[nt][1]);
+                                }
+                            }
                         }
                     }
                 }
             }
+            __syncwarp();  // every lane is done with this stage before it is refilled
         }
-        cur = next;
-    }
+        cp_async_wait<0>();
+        __syncthreads();  // the rings become the merge area
 
-    // merge the warps through shared memory
-    __shared__ float wm[kWarps][NR], wl[kWarps][NR];
-    __shared__ __align__(16) float wacc[kWarps][NR][D];
+        float* wm = reinterpret_cast<float*>(smem);  // [warps][NR] maxima, sums, then [warps][NR][D]
+        float* wl = wm + kWarps * NR;
+        float* wacc = wl + kWarps * NR;
 #pragma unroll
-    for (int nt = 0; nt < NRT; ++nt) {
-        l[nt] += __shfl_xor_sync(kAll, l[nt], 1);
-        l[nt] += __shfl_xor_sync(kAll, l[nt], 2);
-        if (tig == 0) {
-            wm[warp][nt * 8 + gid] = m[nt];
-            wl[warp][nt * 8 + gid] = l[nt];
-        }
-        // accumulators against m' (scales in) brought back against m
-        const float f = Q8 ? (m[nt] == -INFINITY ? 0.f : exp2f(mo[nt] - m[nt])) : 1.f;
-        const float f0 = __shfl_sync(kAll, f, 8 * tig), f1 = __shfl_sync(kAll, f, 8 * tig + 4);
+        for (int nt = 0; nt < NRT; ++nt) {
+            l[nt] += __shfl_xor_sync(kAll, l[nt], 1);
+            l[nt] += __shfl_xor_sync(kAll, l[nt], 2);
+            if (tig == 0) {
+                wm[warp * NR + nt * 8 + gid] = m[nt];
+                wl[warp * NR + nt * 8 + gid] = l[nt];
+            }
 #pragma unroll
-        for (int i = 0; i < MTN; ++i) {
-            const int d = (i / (EPC / 2)) * (EPC * 8) + gid * EPC + 2 * (i % (EPC / 2));
-            *reinterpret_cast<float2*>(&wacc[warp][nt * 8 + 2 * tig][d]) =
-                make_float2(acc[nt][i][0] * f0, acc[nt][i][2] * f0);
-            *reinterpret_cast<float2*>(&wacc[warp][nt * 8 + 2 * tig + 1][d]) =
-                make_float2(acc[nt][i][1] * f1, acc[nt][i][3] * f1);
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < NR * D; i += 32 * kWarps) {
-        const int ri = i / D, d = i % D, r = r0 + ri;
-        if (r >= rows) break;
-        float M = -INFINITY, Ls = 0.f, A = 0.f;
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) M = fmaxf(M, wm[k][ri]);
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-            const float f = M == -INFINITY ? 0.f : exp2f(wm[k][ri] - M);
-            Ls += wl[k][ri] * f;
-            A += wacc[k][ri][d] * f;
-        }
-        const int tok = r / a.G;
-        const int64_t t = w.q0 + tok, h = g * a.G + (r - tok * a.G);
-        if (w.nparts == 1) {
-            reinterpret_cast<T*>(a.out)[t * a.ot + h * a.oh + d] =
-                Dt<T>::from_f(Ls == 0.f ? 0.f : A / Ls);
-        } else {
-            float* o = a.ws + ((t * a.Hq + h) * a.P + p) * (D + 2);
-            o[d] = A;
-            if (d == 0) {
-                o[D] = M;
-                o[D + 1] = Ls;
+            for (int x = 0; x < MTN; ++x) {
+                const int d = (x / (EPC / 2)) * (EPC * 8) + gid * EPC + 2 * (x % (EPC / 2));
+                float* at = wacc + (warp * NR + nt * 8 + 2 * tig) * D + d;
+                *reinterpret_cast<float2*>(at) = make_float2(acc[nt][x][0], acc[nt][x][2]);
+                *reinterpret_cast<float2*>(at + D) = make_float2(acc[nt][x][1], acc[nt][x][3]);
             }
         }
+        __syncthreads();
+        for (int i = tid; i < NR * D; i += 32 * kWarps) {
+            const int ri = i / D, d = i % D, r = r0 + ri;
+            if (r >= rows) break;
+            float M = -INFINITY, Ls = 0.f, A = 0.f;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) M = fmaxf(M, wm[k * NR + ri]);
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                const float f = M == -INFINITY ? 0.f : exp2f(wm[k * NR + ri] - M);
+                Ls += wl[k * NR + ri] * f;
+                A += wacc[(k * NR + ri) * D + d] * f;
+            }
+            if (sg.slot < 0) {
+                const int tok = r / a.G;
+                reinterpret_cast<T*>(a.out)[(int64_t)(w.q0 + tok) * a.ot + (int64_t)(g * a.G + r - tok * a.G) * a.oh + d] =
+                    Dt<T>::from_f(Ls == 0.f ? 0.f : A / Ls);
+            } else {
+                float* o = tree_partial(a, gridDim.x, blockIdx.x, sg.slot, NR, ri, D);
+                o[d] = A;
+                if (d == 0) {
+                    o[D] = M;
+                    o[D + 1] = Ls;
+                }
+            }
+        }
+        __syncthreads();  // the merge area becomes the rings again
     }
 }
 
 template <typename T, int FMT, int D, int NR>
-int launch_nr(const TreeDev& a, int rows, cudaStream_t stream) {
-    const int64_t groups = ceil_div(rows, NR);
-    if (groups * a.Hkv > 65535) return QF_ERR_UNSUPPORTED;
-    tree_mma_kernel<T, FMT, D, NR><<<dim3((unsigned)a.P, (unsigned)(groups * a.Hkv), (unsigned)a.S),
-                                     32 * kWarps, 0, stream>>>(a);
+int launch_nr(const TreeDev& a, int ctas, cudaStream_t stream) {
+    constexpr auto kernel = tree_mma_kernel<T, FMT, D, NR>;
+    const int rc = allow_smem<kernel>(MmaRing<FMT, D>::SMEM);
+    if (rc) return rc;
+    kernel<<<(unsigned)ctas, 32 * kWarps, MmaRing<FMT, D>::SMEM, stream>>>(a);
     return check_launch();
 }
 
 template <typename T, int FMT>
-int launch_d(const TreeDev& a, int D, int rows, cudaStream_t stream) {
+int launch_d(const TreeDev& a, int D, int rows, int ctas, cudaStream_t stream) {
     switch (D) {
     case 64:
-        return rows <= 8 ? launch_nr<T, FMT, 64, 8>(a, rows, stream) : launch_nr<T, FMT, 64, 16>(a, rows, stream);
+        return rows == 8 ? launch_nr<T, FMT, 64, 8>(a, ctas, stream) : launch_nr<T, FMT, 64, 16>(a, ctas, stream);
     case 128:
-        return rows <= 8 ? launch_nr<T, FMT, 128, 8>(a, rows, stream) : launch_nr<T, FMT, 128, 16>(a, rows, stream);
+        return rows == 8 ? launch_nr<T, FMT, 128, 8>(a, ctas, stream) : launch_nr<T, FMT, 128, 16>(a, ctas, stream);
     default:  // 16 rows of 256 would not fit the registers
-        return launch_nr<T, FMT, 256, 8>(a, rows, stream);
+        return launch_nr<T, FMT, 256, 8>(a, ctas, stream);
     }
 }
 
 template <typename T>
-int launch_fmt(const TreeDev& a, int format, int D, int rows, cudaStream_t stream) {
+int launch_fmt(const TreeDev& a, int format, int D, int rows, int ctas, cudaStream_t stream) {
     switch (format) {
-    case QF_CACHE_PLAIN: return launch_d<T, QF_CACHE_PLAIN>(a, D, rows, stream);
-    case QF_CACHE_E4M3: return launch_d<T, QF_CACHE_E4M3>(a, D, rows, stream);
-    default: return launch_d<T, QF_CACHE_INT8>(a, D, rows, stream);
+    case QF_CACHE_PLAIN: return launch_d<T, QF_CACHE_PLAIN>(a, D, rows, ctas, stream);
+    case QF_CACHE_E4M3: return launch_d<T, QF_CACHE_E4M3>(a, D, rows, ctas, stream);
+    default: return launch_d<T, QF_CACHE_INT8>(a, D, rows, ctas, stream);
     }
 }
 
 }  // namespace
 
-int launch_tree_mma(const TreeDev& a, int dtype, int format, int D, int rows, cudaStream_t stream) {
-    return dtype == QF_F16 ? launch_fmt<__half>(a, format, D, rows, stream)
-                           : launch_fmt<__nv_bfloat16>(a, format, D, rows, stream);
+// CTAs that fit on an SM: by the rings' shared memory, and by the registers,
+// which 16 rows' accumulators take more of.
+int tree_mma_ctas_per_sm(bool plain, int D, int rows) {
+    const int smem = plain ? (D == 64 ? MmaRing<QF_CACHE_PLAIN, 64>::SMEM
+                                      : D == 128 ? MmaRing<QF_CACHE_PLAIN, 128>::SMEM : MmaRing<QF_CACHE_PLAIN, 256>::SMEM)
+                           : (D == 64 ? MmaRing<QF_CACHE_E4M3, 64>::SMEM
+                                      : D == 128 ? MmaRing<QF_CACHE_E4M3, 128>::SMEM : MmaRing<QF_CACHE_E4M3, 256>::SMEM);
+    const int by_regs = D == 256 ? 2 : (D == 64 ? 4 : 3) - (rows == 16);
+    return std::max(1, std::min(by_regs, 232448 / (smem + 2048)));
+}
+
+int launch_tree_mma(const TreeDev& a, int dtype, int format, int D, int rows, int ctas,
+                    cudaStream_t stream) {
+    return dtype == QF_F16 ? launch_fmt<__half>(a, format, D, rows, ctas, stream)
+                           : launch_fmt<__nv_bfloat16>(a, format, D, rows, ctas, stream);
 }
 
 }  // namespace qf

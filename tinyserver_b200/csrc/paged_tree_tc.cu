@@ -8,11 +8,16 @@
 //   softmax of row r by thread r of the tile's warpgroup, whose tensor-memory
 //   lane the row is; P_t back over the first half of S_t
 //   O_t += P_t V_j      A = P_t from tensor memory, V in shared memory
-// Roles: 4 NT softmax warps, one MMA thread, two warps that bring K and two that
-// bring V.  Pages may have any size and the rows any place, so rows are fetched
-// one by one: 16-bit rows with cp.async, straight into the swizzled tile; 8-bit
-// rows into registers and, converted to fp16 (exact), into the tile, so the next
-// block's codes are in flight while this block's tile is in use.
+// P goes back by halves of a block: the first half's products run during the
+// second's softmax.  (Scores by halves too, taking turns in S_t, overlap better on
+// paper, but 64 columns cost the tensor core as much as 128: 511 cycles for a tile's
+// eight steps against 515.)
+// Roles: 4 NT softmax warps, one MMA thread, a warp that brings K and one that
+// brings V.  16-bit pages come by TMA, one box per lane, where a block's keys are
+// all context; else (the drafted keys, the tail, pages whose size is no multiple of
+// 8) row by row with cp.async.  8-bit rows come into registers and, converted to
+// fp16 (exact), into the tile, the next block's codes in flight while this block's
+// tile is in use.
 //
 // What bounds it: a block is 64 KB of 16-bit K and V, ~2900 cycles of an SM's
 // share of HBM; a tile's softmax is 16384 exponentials, 1024 cycles of the MUFU,
@@ -48,7 +53,6 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr float kKeepLog2 = 8.f;    // the reference maximum moves when the row's has grown by 2^8
 constexpr float kScaleRange = 90.f;  // log2 of the v-scales' ratio up to which one exponential will do
 
-constexpr float kLeastScale = 7.52316384526264e-37f;  // 2^-120
 
 template <int NT>
 struct TreeTc {
@@ -66,7 +70,9 @@ struct TreeBars {
     uint64_t q_full;
     uint64_t k_full[NT], v_full[NT], k_empty[NT], v_empty[NT];
     uint64_t info_full[2 * NT];  // a block's valid bits and scales
-    uint64_t s_full[NT], p_full[NT], o_full, drain;
+    uint64_t s_full[NT], p_full[NT][2];  // P by halves of a block
+    uint64_t pv_done[NT], o_full, drain;
+    uint64_t v_raw;  // a V tile that the loader still looks through has landed
 };
 
 __device__ __forceinline__ void proxy_fence() {
@@ -83,19 +89,49 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c) {
     return (uint32_t)((c >> 3) * kSlab + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// Infinities and NaN of 8 16-bit values set to zero; whether there were any.
+// Whether two 16-bit values hold an infinity or a NaN: an exponent of all ones
+// carries into the sign's place when one is added to it.
 template <typename T>
-__device__ __forceinline__ bool zero_not_finite(uint4& v) {
-    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    bool any = false;
+__device__ __forceinline__ uint32_t odd_pair(uint32_t w) {
+    constexpr bool H = std::is_same<T, __half>::value;
+    return ((w & (H ? 0x7c007c00u : 0x7f807f80u)) + (H ? 0x04000400u : 0x00800080u)) & 0x80008000u;
+}
+
+// Infinities and NaN of 8 16-bit values set to zero.
+template <typename T>
+__device__ __forceinline__ void zero_not_finite(uint4& v) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint32_t w = word(v, i);
-        if ((w & E) == E) w &= 0xffff0000u, any = true;
-        if ((w & (E << 16)) == (E << 16)) w &= 0xffffu, any = true;
+        const uint32_t o = odd_pair<T>(w);
+        if (o & 0x8000u) w &= 0xffff0000u;
+        if (o & 0x80000000u) w &= 0xffffu;
         set_word(v, i, w);
     }
-    return any;
+}
+
+// By one warp: rows [r0, r1) of a V tile looked through, and infinities and NaN in
+// them set to zero; whether there were any.
+template <typename T>
+__device__ __forceinline__ bool clean_rows(char* tile, int r0, int r1, int lane) {
+    const int c = lane & 15, hi = lane >> 4;
+    uint32_t odd = 0;
+    for (int r = r0; r < r1; r += 16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int rr = min(r + 2 * i + hi, r1 - 1);
+            const uint4 v = *reinterpret_cast<const uint4*>(tile + tile_off(rr, c));
+            odd |= odd_pair<T>(v.x) | odd_pair<T>(v.y) | odd_pair<T>(v.z) | odd_pair<T>(v.w);
+        }
+    }
+    if (!__any_sync(kFull, odd != 0)) return false;
+    for (int r = r0 + hi; r < r1; r += 2) {
+        uint4* at = reinterpret_cast<uint4*>(tile + tile_off(r, c));
+        uint4 v = *at;
+        zero_not_finite<T>(v);
+        *at = v;
+    }
+    return true;
 }
 
 // q . k over the 128 dims on the CUDA cores, k a cache row.
@@ -149,12 +185,33 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
         : "memory");
 }
 
-// S_t = Q_t K^T: head_dim in steps of 16.
+// One lane of a converged warp, known as such to the assembler: the products'
+// operands, alike in all lanes, then stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
+
+// Shared-memory descriptors as their two words: the low one is the address in 16
+// bytes and the leading offset, so stepping through a tile is one add, and the
+// issuing thread, which shares its scheduler with softmax warps, has few
+// instructions per product.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) {
+    return (uint32_t)sdesc(addr, lbo, 1024);
+}
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
+    constexpr uint64_t hi = (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;  // as sdesc(., ., 1024)
+    return hi | lo;
+}
+
+// S = Q K^T, from the descriptors of Q's and K's first step: head_dim in steps of 16,
+// 32 bytes on in a slab, then the second slab.
 __device__ __forceinline__ void issue_scores(uint32_t d, uint32_t q, uint32_t k, uint32_t id) {
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) {
-        const uint32_t off = (uint32_t)((kk >> 2) * kSlab + (kk & 3) * 32);
-        mma_ss(d, sdesc(q + off, 16, 1024), sdesc(k + off, 16, 1024), id, kk > 0 ? 1u : 0u);
+        const uint32_t off = (uint32_t)((kk >> 2) * (kSlab >> 4) + (kk & 3) * 2);
+        mma_ss(d, desc_of(q + off), desc_of(k + off), id, kk > 0 ? 1u : 0u);
     }
 }
 
@@ -168,35 +225,14 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     using MP = Packed<MT>;
     constexpr int ST = C::ST;
 
-    const int p = blockIdx.x, s = blockIdx.z;
-    const int g = blockIdx.y % a.Hkv, rg = blockIdx.y / a.Hkv;
-    const TreeSeq w = tree_seq(a, s);
-    if (p == 0 && rg == 0) zero_unowned_rows<T, kD>(a, s, g, w);
-    const int rows = w.n * a.G, r0 = rg * NT * kRows;
-    if (p >= w.nparts || r0 >= rows) return;
-    const int k_begin = p * a.part, k_end = k_begin + min(w.L - k_begin, a.part);
-    const int nblk = (k_end - k_begin + kRows - 1) / kRows;
-    const int ntile = min(NT, (rows - r0 + kRows - 1) / kRows);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-    // where this softmax thread's row goes
-    const int trow = r0 + (tid & (NT * kRows - 1));
-    const bool live = tid < C::SOFT && trow < rows;
-    const int tok = live ? trow / a.G : 0;
-    const int hq = g * a.G + (live ? trow - tok * a.G : 0);
-    const int64_t trow_q = w.q0 + tok;
-    T* const orow = reinterpret_cast<T*>(a.out) + trow_q * a.ot + (int64_t)hq * a.oh;
-    if (nblk == 0) {  // no key at all
-        if (live)
-            for (int c = 0; c < kD / 8; ++c) st16(orow + 8 * c, make_uint4(0, 0, 0, 0));
-        return;
-    }
 
     extern __shared__ __align__(1024) char dsm[];
     __shared__ TreeBars<NT> bars;
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag, odd_v;
-    __shared__ uint32_t valid[C::SLOTS][4];
+    __shared__ int abort_flag, odd_v;  // odd_v: the last segment whose drafted V was not finite, from 1
+    __shared__ int64_t scratch[34];
+    __shared__ __align__(16) uint32_t valid[C::SLOTS][4];
     // k-scale, log2 v-scale, 1 / v-scale of a block's keys; least and largest log2 v-scale
     __shared__ __align__(16) float sk[Q8 ? C::SLOTS : 1][Q8 ? kRows : 1], sl[Q8 ? C::SLOTS : 1][Q8 ? kRows : 1],
         sr_[Q8 ? C::SLOTS : 1][Q8 ? kRows : 1];
@@ -208,7 +244,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     char* const kbase = base + NT * kTile;
     char* const vbase = kbase + ST * kTile;
     if (tid == 0) {
-        mbar_init(&bars.q_full, (uint32_t)(ntile * kRows));
+        mbar_init(&bars.q_full, kRows * NT);
         for (int i = 0; i < ST; ++i) {
             mbar_init(&bars.k_full[i], 32);
             mbar_init(&bars.v_full[i], 32);
@@ -218,10 +254,12 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         for (int i = 0; i < C::SLOTS; ++i) mbar_init(&bars.info_full[i], 32);
         for (int t = 0; t < NT; ++t) {
             mbar_init(&bars.s_full[t], 1);
-            mbar_init(&bars.p_full[t], kRows);
+            for (int h = 0; h < 2; ++h) mbar_init(&bars.p_full[t][h], kRows);
+            mbar_init(&bars.pv_done[t], 1);
         }
         mbar_init(&bars.o_full, 1);
         mbar_init(&bars.drain, 1);
+        mbar_init(&bars.v_raw, 1);
         abort_flag = 0;
         odd_v = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -237,11 +275,20 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const int32_t* bt = a.bt + (int64_t)s * a.bts;
     const float sl2 = a.scale * 1.4426950408889634f;
-    const bool tree = a.cu != nullptr;
+
+    // every role walks the same segments; barrier phases run on across them
+    TreeWalk<kRows, NT * kRows> walk;
+    walk.begin(a, scratch);
+    zero_unowned_rows<T, kD>(a);
+    if (tid == 0) walk.record(a);
+    TreeSeg sg{};
+    auto blocks_of = [&]() { return (sg.k_end - sg.k_begin + kRows - 1) / kRows; };
+    auto tiles_of = [&]() {
+        return min(NT, (sg.w.n * a.G - sg.rg * NT * kRows + kRows - 1) / kRows);
+    };
     // the first block that a row may not see whole
-    const int first_draft = tree ? max(0, (w.ctx - k_begin) / kRows) : nblk;
+    auto draft_of = [&](int nblk) { return a.cu ? max(0, (sg.w.ctx - sg.k_begin) / kRows) : nblk; };
 
     if (warp >= C::LOAD_WARP) {
         // ---- loaders: one warp K, one warp V
@@ -250,6 +297,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         char* const tiles = side ? vbase : kbase;
         uint64_t* full = side ? bars.v_full : bars.k_full;
         uint64_t* empty = side ? bars.v_empty : bars.k_empty;
+        const int32_t* bt = nullptr;
         // lane l: keys l, l + 32, l + 64, l + 96 of a block
         int64_t off[4];
         unsigned ok[4];
@@ -257,12 +305,12 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         auto locate = [&](int j) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const int key = k_begin + j * kRows + x * 32 + lane;
+                const int key = sg.k_begin + j * kRows + x * 32 + lane;
                 int64_t srow = 0;
                 off[x] = 0;
                 ks[x] = 0.f;
                 vs[x] = 1.f;
-                const bool in = key < k_end && key_place(a, bt, g, key, off[x], srow);
+                const bool in = key < sg.k_end && key_place(a, bt, sg.g, key, off[x], srow);
                 ok[x] = __ballot_sync(kFull, in);
                 if (!Q8) off[x] *= 2;  // bytes
                 if (Q8 && side == 0 && in) {
@@ -273,8 +321,8 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 }
             }
         };
-        // What the softmax needs to know of block j's keys.  The slot's last reader, the
-        // softmax of block j - SLOTS, is done: S of block j - ST (whose K was in this
+        // What the softmax needs to know of a block's keys.  The slot's last reader, the
+        // softmax SLOTS blocks ago, is done: S of ST blocks ago (whose K was in this
         // stage) came after it.
         auto inform = [&](int slot) {
 #pragma unroll
@@ -301,10 +349,12 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             __syncwarp();
             mbar_arrive(&bars.info_full[slot]);
         };
-        // block j's stage may be refilled (the whole warp learns the same)
-        auto vacant = [&](int j) -> bool {
-            return __all_sync(kFull, j < ST || mbar_wait(&empty[j % ST], ((j / ST) - 1) & 1, abort));
+        // the stage of block n (of all segments) may be refilled; the whole warp learns the same
+        auto vacant = [&](int n) -> bool {
+            return __all_sync(kFull, n < ST || mbar_wait(&empty[n % ST], ((n / ST) - 1) & 1, abort));
         };
+        bool go = true;
+        int seq_no = 0;  // segments begun
         if constexpr (Q8) {
             // codes into registers, 16 rows' worth a lane group in flight all the time: half a
             // block is converted and stored while the other half, then the next block's, comes
@@ -316,18 +366,47 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 const unsigned m = x == 0 ? ok[0] : x == 1 ? ok[1] : x == 2 ? ok[2] : ok[3];
                 raws[i] = (m >> r) & 1 ? ld_stream16(src + o + c * 16) : make_uint4(0, 0, 0, 0);
             };
-            locate(0);
+            bool more = walk.next(a, sg);
+            ++seq_no;
+            if (more) {
+                bt = a.bt + (int64_t)sg.s * a.bts;
+                locate(0);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) fetch(i, 0);
-            for (int j = 0; j < nblk; ++j) {
-                const int st = j % ST;
+                for (int i = 0; i < 16; ++i) fetch(i, 0);
+            }
+            int j = 0, n = 0;  // block of the segment, of all segments
+            while (more) {
+                const int nblk = blocks_of(), first_draft = draft_of(nblk);
+                if (nblk == 0) {  // (a sequence without keys: nothing was fetched but zeros)
+                    more = walk.next(a, sg);
+                    ++seq_no;
+                    if (more) {
+                        bt = a.bt + (int64_t)sg.s * a.bts;
+                        locate(0);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) fetch(i, 0);
+                    }
+                    continue;
+                }
+                const int st = n % ST;
                 char* tile = tiles + st * kTile;
-                if (!vacant(j)) break;
-                if (side == 0) inform(j % C::SLOTS);
+                if (!vacant(n)) break;
+                if (side == 0) inform(n % C::SLOTS);
+                const bool drafted = j >= first_draft;
+                const int own_no = seq_no;
+                ++n;
                 bool odd = false;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    if (half == 1 && j + 1 < nblk) locate(j + 1);
+                    if (half == 1) {  // the block after this one, of the next segment if need be
+                        if (++j == nblk) {
+                            j = 0;
+                            more = walk.next(a, sg);
+                            ++seq_no;
+                            if (more) bt = a.bt + (int64_t)sg.s * a.bts;
+                        }
+                        if (more) locate(j);
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int r = half * 64 + 4 * i + (lane >> 3);
@@ -337,195 +416,276 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                         codes_to_f16<FMT>(raws[i].z, hi.x, hi.y);
                         codes_to_f16<FMT>(raws[i].w, hi.z, hi.w);
                         if (half == 0) fetch(i, 1);
-                        else if (j + 1 < nblk) fetch(i, 0);
-                        if (FMT == QF_CACHE_E4M3 && side == 1 && j >= first_draft) {
-                            odd |= zero_not_finite<__half>(lo);
-                            odd |= zero_not_finite<__half>(hi);
+                        else if (more) fetch(i, 0);
+                        if (FMT == QF_CACHE_E4M3 && side == 1 && drafted) {
+                            odd |= (odd_pair<__half>(lo.x) | odd_pair<__half>(lo.y) | odd_pair<__half>(lo.z) |
+                                    odd_pair<__half>(lo.w) | odd_pair<__half>(hi.x) | odd_pair<__half>(hi.y) |
+                                    odd_pair<__half>(hi.z) | odd_pair<__half>(hi.w)) != 0;
+                            zero_not_finite<__half>(lo);
+                            zero_not_finite<__half>(hi);
                         }
                         *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c)) = lo;
                         *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + 1)) = hi;
                     }
                 }
-                if (odd) odd_v = 1;
+                if (odd) odd_v = own_no;
                 proxy_fence();
                 mbar_arrive(&full[st]);
             }
         } else {
             const CUtensorMap* map = side ? &tv : &tk;
             const int hi = lane >> 4, c = lane & 15;
-            int j = 0;
-            for (; j < nblk; ++j) {
-                const int st = j % ST, kb = k_begin + j * kRows;
-                char* tile = tiles + st * kTile;
-                // A block whose keys are all context and all there comes by TMA, a box of
-                // `box` slots x 64 dims per lane (K and V alike, 128-byte swizzle)
-                bool bulk = box > 0 && j < first_draft && kb + kRows <= k_end;
-                int blk = 0, slot0 = 0;
-                const int pc = lane >> 1;  // this lane's piece of the block
-                if (bulk) {
-                    const int key = kb + min(pc * box, kRows - 1);
-                    const int lb = a.B.div(key);
-                    blk = __ldg(bt + lb);
-                    slot0 = key - lb * a.B.d;
-                    bulk = __all_sync(kFull, blk >= 0 && blk < a.N);
-                }
-                if (!bulk) locate(j);
-                if (!vacant(j)) break;
-                if (bulk) {
-                    if (side == 0) {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) ok[x] = kFull;
-                        inform(j % C::SLOTS);
+            const int pc = lane >> 1;  // this lane's piece of a block: `box` slots of one page, 64 dims
+            int n = 0, raw = 0;        // blocks, looked-through V tiles of all segments
+            while (go && walk.next(a, sg)) {
+                ++seq_no;
+                bt = a.bt + (int64_t)sg.s * a.bts;
+                const int nblk = blocks_of(), k_end = sg.k_end;
+                for (int j = 0; j < nblk; ++j, ++n) {
+                    const int st = n % ST, kb = sg.k_begin + j * kRows, nk = min(kRows, k_end - kb);
+                    char* tile = tiles + st * kTile;
+                    // rows of V that some query row may not see
+                    const int d0 = a.cu ? max(0, sg.w.ctx - kb) : kRows;
+                    bool bulk = box > 0;
+                    int blk = 0, slot0 = 0;
+                    const bool mine = pc * box < nk;
+                    if (bulk) {
+                        const int key = kb + (mine ? pc * box : 0);
+                        const int lb = a.B.div(key);
+                        blk = __ldg(bt + lb);
+                        slot0 = key - lb * a.B.d;
+                        bulk = __all_sync(kFull, blk >= 0 && blk < a.N);
                     }
-                    if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)kTile);
-                    else mbar_arrive(&full[st]);
-                    __syncwarp();
-                    if (pc * box < kRows)
-                        tma_page(tile + (lane & 1) * kSlab + pc * box * 128, map, (lane & 1) * 64, slot0, g, blk,
-                                 &full[st]);
-                    continue;
-                }
-                if (side == 0) inform(j % C::SLOTS);
-                // row by row: chunk c of rows 2 i + hi; the swizzle repeats every four i
-                const uint32_t dst = smem_u32(tile) + (uint32_t)((c >> 3) * kSlab + hi * 128);
-                const char* from = src + c * 16;
+                    if (bulk) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int64_t o = __shfl_sync(kFull, off[x], 2 * i + hi);
-                        cp_async16_at(dst + (uint32_t)((x * 32 + 2 * i) * 128 + (((c & 7) ^ ((2 * i & 7) + hi)) << 4)),
-                                      from + o, (ok[x] >> (2 * i + hi)) & 1 ? 16 : 0);
+                        for (int x = 0; x < 4; ++x)
+                            ok[x] = nk >= 32 * (x + 1) ? kFull : nk > 32 * x ? (1u << (nk - 32 * x)) - 1u : 0u;
+                    } else {
+                        locate(j);
                     }
-                }
-                cp_async_commit();
-                cp_async_wait<0>();
-                if (side == 1 && j >= first_draft) {  // this lane's own chunks
-                    bool odd = false;
-                    for (int i = 0; i < 64; ++i) {
-                        uint4* at = reinterpret_cast<uint4*>(tile + tile_off(2 * i + hi, c));
-                        uint4 v = *at;
-                        if (zero_not_finite<MT>(v)) {
-                            *at = v;
-                            odd = true;
+                    if (!vacant(n)) {
+                        go = false;
+                        break;
+                    }
+                    if (side == 0) inform(n % C::SLOTS);
+                    const bool look = side == 1 && (nk < kRows || d0 < nk);
+                    if (bulk) {
+                        // K behind the last key may hold anything: those columns are masked
+                        uint64_t* bar = look ? &bars.v_raw : &full[st];
+                        const uint32_t bytes = (uint32_t)((nk + box - 1) / box * box) * 256u;
+                        if (lane == 0) mbar_expect_tx(bar, bytes);
+                        else if (!look) mbar_arrive(bar);
+                        __syncwarp();
+                        if (mine)
+                            tma_page(tile + (lane & 1) * kSlab + pc * box * 128, map, (lane & 1) * 64, slot0, sg.g,
+                                     blk, bar);
+                        if (!look) continue;
+                        if (!__all_sync(kFull, mbar_wait(&bars.v_raw, raw++ & 1, nullptr))) {
+                            go = false;
+                            break;
                         }
+                        for (int r = nk + hi; r < kRows; r += 2)
+                            *reinterpret_cast<uint4*>(tile + tile_off(r, c)) = make_uint4(0, 0, 0, 0);
+                    } else {
+                        // row by row: chunk c of rows 2 i + hi; the swizzle repeats every four i
+                        const uint32_t dst = smem_u32(tile) + (uint32_t)((c >> 3) * kSlab + hi * 128);
+                        const char* from = src + c * 16;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const int64_t o = __shfl_sync(kFull, off[x], 2 * i + hi);
+                                cp_async16_at(dst + (uint32_t)((x * 32 + 2 * i) * 128 + (((c & 7) ^ ((2 * i & 7) + hi)) << 4)),
+                                              from + o, (ok[x] >> (2 * i + hi)) & 1 ? 16 : 0);
+                            }
+                        }
+                        cp_async_commit();
+                        cp_async_wait<0>();
+                        __syncwarp();
                     }
-                    if (odd) odd_v = 1;
+                    if (look && d0 < nk && clean_rows<MT>(tile, d0, nk, lane)) odd_v = seq_no;
+                    proxy_fence();
+                    mbar_arrive(&full[st]);
                 }
-                proxy_fence();
-                mbar_arrive(&full[st]);
             }
             // every copy issued has landed before the CTA can leave
-            for (int d = max(0, j - ST); d < j; ++d) mbar_wait(&full[d % ST], (d / ST) & 1, nullptr);
+            for (int d = max(0, n - ST); d < n; ++d) mbar_wait(&full[d % ST], (d / ST) & 1, nullptr);
         }
     } else if (warp == C::MMA_WARP) {
-        // ---- MMA issue: S_t,0 | PV_t,j S_t,j+1 | ...
-        if (lane == 0) {
-            const uint32_t bf = std::is_same<MT, __nv_bfloat16>::value ? 1u : 0u;
-            const uint32_t id_qk = idesc(bf, 0u), id_pv = idesc(bf, 1u);
-            const uint32_t qa = smem_u32(base), ka = smem_u32(kbase), va = smem_u32(vbase);
-            bool go = mbar_wait(&bars.q_full, 0, abort) && mbar_wait(&bars.k_full[0], 0, abort);
-            if (go) {
-                tc_fence_after();
-                for (int t = 0; t < ntile; ++t) {
-                    issue_scores(tmem + t * kRows, qa + t * kTile, ka, id_qk);
+        // ---- MMA issue, the warp together and one lane for it: S_t,0 | PV_t,j by the two
+        // halves of P, S_t,j+1 | ...
+        const uint32_t bf = std::is_same<MT, __nv_bfloat16>::value ? 1u : 0u;
+        const uint32_t id_qk = idesc(bf, 0u), id_pv = idesc(bf, 1u);
+        const uint32_t qa = desc_lo(smem_u32(base), 16), ka = desc_lo(smem_u32(kbase), 16);
+        const uint32_t va = desc_lo(smem_u32(vbase), kSlab);
+        bool go = true;
+        auto wait = [&](uint64_t* bar, uint32_t phase) {
+            go = __all_sync(kFull, go && mbar_wait(bar, phase & 1, abort));
+            tc_fence_after();
+        };
+        uint32_t n = 0, seg = 0;  // blocks, segments with keys so far
+        uint32_t uses[NT] = {};   // blocks of each tile so far
+        while (go && walk.next(a, sg)) {
+            const int nblk = blocks_of(), ntile = tiles_of();
+            if (nblk == 0) continue;
+            wait(&bars.q_full, seg);
+            wait(&bars.k_full[n % ST], n / ST);
+            if (!go) break;
+            // scores of block bn; K's stage is free once the last tile's have been issued
+            auto scores = [&](uint32_t bn, int t) {
+                if (elect_one()) {
+                    issue_scores(tmem + (uint32_t)(t * kRows), qa + t * (kTile >> 4), ka + (bn % ST) * (kTile >> 4), id_qk);
                     mma_commit(&bars.s_full[t]);
+                    if (t == ntile - 1) mma_commit(&bars.k_empty[bn % ST]);
                 }
-                mma_commit(&bars.k_empty[0]);
-            }
-            for (int j = 0; go && j < nblk; ++j) {
-                const int st = j % ST, sn = (j + 1) % ST;
-                go = mbar_wait(&bars.v_full[st], (j / ST) & 1, abort);
-                for (int t = 0; go && t < ntile; ++t) {
-                    go = mbar_wait(&bars.p_full[t], j & 1, abort);
-                    if (!go) break;
-                    tc_fence_after();
-                    const uint32_t o = tmem + (uint32_t)((NT + t) * kRows), pt = tmem + (uint32_t)(t * kRows);
-                    const uint32_t v = va + (uint32_t)(st * kTile);
+                __syncwarp();
+            };
+            for (int t = 0; t < ntile; ++t) scores(n, t);
+            for (int j = 0; go && j < nblk; ++j, ++n) {
+                const uint32_t st = n % ST;
+                wait(&bars.v_full[st], n / ST);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k)  // keys in steps of 16
-                        mma_ts(o, pt + 8u * k, sdesc(v + k * 2048, kSlab, 1024), id_pv,
-                               (j > 0 || k > 0) ? 1u : 0u);
-                    if (j + 1 < nblk) {
-                        if (t == 0) {
-                            go = mbar_wait(&bars.k_full[sn], ((j + 1) / ST) & 1, abort);
-                            if (!go) break;
-                            tc_fence_after();
+                for (int t = 0; t < NT; ++t) {
+                    if (!go || t >= ntile) break;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        wait(&bars.p_full[t][h], uses[t] + (uint32_t)j);
+                        if (!go) break;
+                        if (elect_one()) {
+                            const uint32_t o = tmem + (uint32_t)((NT + t) * kRows);
+                            const uint32_t pt = tmem + (uint32_t)(t * kRows + h * 64);
+                            const uint32_t v = va + st * (kTile >> 4) + h * (8192 >> 4);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)  // keys in steps of 16
+                                mma_ts(o, pt + 8u * k, desc_of(v + k * (2048 >> 4)), id_pv,
+                                       (j > 0 || h > 0 || k > 0) ? 1u : 0u);
+                            if (h == 0) mma_commit(&bars.pv_done[t]);
+                            else if (t == ntile - 1) mma_commit(&bars.v_empty[st]);
                         }
-                        issue_scores(pt, qa + t * kTile, ka + sn * kTile, id_qk);
-                        mma_commit(&bars.s_full[t]);
+                        __syncwarp();
+                    }
+                    if (go && j + 1 < nblk) {
+                        if (t == 0) wait(&bars.k_full[(n + 1) % ST], (n + 1) / ST);
+                        if (!go) break;
+                        scores(n + 1, t);
                     }
                 }
-                mma_commit(&bars.v_empty[st]);
-                if (j + 1 < nblk) mma_commit(&bars.k_empty[sn]);
             }
-            mma_commit(&bars.o_full);
-            mma_commit(&bars.drain);  // every MMA issued has completed before the CTA can leave
-            mbar_wait(&bars.drain, 0, nullptr);
+            if (elect_one()) mma_commit(&bars.o_full);
+            __syncwarp();
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (t < ntile) uses[t] += (uint32_t)nblk;
+            ++seg;
         }
-    } else if (warp < 4 * ntile) {
+        if (elect_one()) mma_commit(&bars.drain);  // every MMA issued has completed before the CTA can leave
+        __syncwarp();
+        mbar_wait(&bars.drain, 0, nullptr);
+    } else {
         // ---- softmax of tile t, one row per thread
         const int t = warp >> 2, r = tid & (kRows - 1);
+        bool got = true;
+        uint32_t n0 = 0, seg = 0;                // blocks, segments with keys so far
+        uint32_t uses = 0;                       // this tile's blocks so far
+        int seq_no = 0;                    // segments
+        while (got && walk.next(a, sg)) {
+        ++seq_no;
+        const int nblk = blocks_of(), ntile = tiles_of(), first_draft = draft_of(nblk);
+        const TreeSeq& w = sg.w;
+        const int32_t* bt = a.bt + (int64_t)sg.s * a.bts;
+        const int rows = w.n * a.G, trow = sg.rg * NT * kRows + tid, k_begin = sg.k_begin, k_end = sg.k_end;
+        const bool live = trow < rows;
+        const int tok = live ? trow / a.G : 0;
+        const int hq = sg.g * a.G + (live ? trow - tok * a.G : 0);
+        const int64_t trow_q = w.q0 + tok;
+        T* const orow = reinterpret_cast<T*>(a.out) + trow_q * a.ot + (int64_t)hq * a.oh;
+        if (nblk == 0) {  // no key at all
+            if (live)
+                for (int c = 0; c < kD / 8; ++c) st16(orow + 8 * c, make_uint4(0, 0, 0, 0));
+            __syncwarp();
+            continue;
+        }
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t sS = tmem + lanes + (uint32_t)(t * kRows);
         const uint32_t sO = tmem + lanes + (uint32_t)((NT + t) * kRows);
         const T* qrow = reinterpret_cast<const T*>(a.q) + trow_q * a.qt + (int64_t)hq * a.qh;
         const int64_t* mrow = a.mask + trow_q * a.words;
         float rs = sl2;
+        char* const qtile = base + t * kTile;
         {
+            // The warp's 32 rows of Q, two at a time and whole (lane: chunk lane % 16 of row
+            // 2 i + lane / 16), into the tile.  (The segment before is done with Q: its O,
+            // which this thread has read, was final.)
             using P = Packed<T>;
-            float f = 1.f;
+            const int hi = lane >> 4, c = lane & 15;
+            const int64_t at = live ? trow_q * a.qt + (int64_t)hq * a.qh : -1;
             uint32_t flip = 0;
             if (!Q8) {  // rs > 0: a negative scale's sign goes to Q, and 0 becomes as good as 0
                 flip = sl2 < 0.f ? 0x80008000u : 0u;
                 rs = fabsf(sl2) < 1e-30f ? 1e-30f : fabsf(sl2);
             }
-            if constexpr (Q8) {  // a power-of-two factor brings the largest element to [2^14, 2^15)
-                uint32_t mx = 0;
-                if (live)
-                    for (int c = 0; c < 16; ++c) {
-                        const uint4 v = ld_shared_ro16(qrow + 8 * c);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            mx = max(mx, max(__float_as_uint(P::lo(word(v, i))) & 0x7fffffffu,
-                                             __float_as_uint(P::hi(word(v, i))) & 0x7fffffffu));
-                    }
-                const int e = min(max((int)(mx >> 23) - 127, -100), 127);
-                f = __int_as_float((127 + 14 - e) << 23);
-                rs = sl2 * __int_as_float((127 - 14 + e) << 23);
-            }
-            for (int c = 0; c < 16; ++c) {
-                uint4 v = live ? ld_shared_ro16(qrow + 8 * c) : make_uint4(0, 0, 0, 0);
-                if constexpr (Q8) {
+            for (int i0 = 0; i0 < 16; i0 += 8) {
+                uint4 v[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        set_word(v, i, MP::pack(P::lo(word(v, i)) * f, P::hi(word(v, i)) * f));
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t o = __shfl_sync(kFull, at, 2 * (i0 + i) + hi);
+                    v[i] = o >= 0 ? ld_shared_ro16(reinterpret_cast<const T*>(a.q) + o + 8 * c) : make_uint4(0, 0, 0, 0);
                 }
-                if (!Q8) v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                *reinterpret_cast<uint4*>(base + t * kTile + tile_off(r, c)) = v;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if constexpr (Q8) {  // a power-of-two factor brings the row's largest element to [2^14, 2^15)
+                        uint32_t mx = 0;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            mx = max(mx, max(__float_as_uint(P::lo(word(v[i], x))) & 0x7fffffffu,
+                                             __float_as_uint(P::hi(word(v[i], x))) & 0x7fffffffu));
+#pragma unroll
+                        for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
+                        const int e = min(max((int)(mx >> 23) - 127, -100), 127);
+                        const float f = __int_as_float((127 + 14 - e) << 23);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            set_word(v[i], x, MP::pack(P::lo(word(v[i], x)) * f, P::hi(word(v[i], x)) * f));
+                        const int er = __shfl_sync(kFull, e, (lane & 1) * 16);  // lane's own row's, if it is one of these
+                        if ((lane >> 1) == i0 + i) rs = sl2 * __int_as_float((127 - 14 + er) << 23);
+                    } else {
+                        v[i].x ^= flip, v[i].y ^= flip, v[i].z ^= flip, v[i].w ^= flip;
+                    }
+                    *reinterpret_cast<uint4*>(qtile + tile_off((warp & 3) * 32 + 2 * (i0 + i) + hi, c)) = v[i];
+                }
             }
             proxy_fence();
             mbar_arrive(&bars.q_full);
         }
         float m = -INFINITY, l = 0.f;  // reference maximum and the sum against it
         float lvtop = -INFINITY;       // largest log2 v-scale so far
-        bool got = true;
-        for (int j = 0; j < nblk; ++j) {
-            const int slot = j % C::SLOTS, kb = k_begin + j * kRows;
-            got = mbar_wait(&bars.info_full[slot], (j / C::SLOTS) & 1, abort) &&
-                  mbar_wait(&bars.s_full[t], j & 1, abort);
+        for (int j = 0; t < ntile && j < nblk; ++j) {
+            const uint32_t nb = n0 + (uint32_t)j;
+            const int slot = (int)(nb % C::SLOTS), kb = k_begin + j * kRows;
+            got = mbar_wait(&bars.info_full[slot], (nb / C::SLOTS) & 1, abort) &&
+                  mbar_wait(&bars.s_full[t], (uses + (uint32_t)j) & 1, abort);
             if (!__all_sync(kFull, got)) {
                 got = false;
                 break;
             }
             tc_fence_after();
             uint32_t see[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                see[q] = live ? valid[slot][q] : 0u;
-                if (j >= first_draft && live) see[q] &= tree_bits32(mrow, a.words, kb + 32 * q - w.ctx);
+            {
+                const uint4 v = *reinterpret_cast<const uint4*>(valid[slot]);
+                see[0] = v.x, see[1] = v.y, see[2] = v.z, see[3] = v.w;
             }
+            if (j >= first_draft || !live)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    see[q] = live ? see[q] & tree_bits32(mrow, a.words, kb + 32 * q - w.ctx) : 0u;
             const bool masked = __any_sync(kFull, (see[0] & see[1] & see[2] & see[3]) != kFull);
+            // the two halves of a block one after the other: the first's products run during
+            // the second's softmax
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+            const int c0 = 64 * h;
+            const uint32_t sh = sS + (uint32_t)c0;
             // Scores in log2 units, with V's scale where there is one: 16-bit rows x * rs,
             // rs > 0 (a negative scale is in Q), so the maximum is that of x.
             auto score = [&](float x, int c) -> float {
@@ -537,32 +697,31 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 lvtop = fmaxf(lvtop, srange[slot][1]);
                 wide = lvtop - srange[slot][0] > kScaleRange;
             }
-            // One pass over S against the reference m, P in registers, the block's maximum on
-            // the side.  While no row's maximum has grown past 2^8 (but for the first blocks,
+            // One pass over S against the reference m, P in registers, the half block's maximum
+            // on the side.  While no row's maximum has grown past 2^8 (but for the first blocks,
             // nearly always) P stands; else the reference moves, O and l with it, and
             // the pass is made again over S, which P has not touched yet.
-            uint32_t pk[64];
+            uint32_t pk[32];
             float sum;
             for (int turn = 0;; ++turn) {
                 const float mref = m == -INFINITY ? 0.f : m;
                 float mx0 = -INFINITY, mx1 = -INFINITY;
                 float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-                constexpr int NX = NT == 2 ? 2 : 1;  // registers allow: the next quarter's load in flight
-                uint32_t x[NX][32];
-                tmem_ld32(sS, x[0]);
+                uint32_t x[2][32];
+                tmem_ld32(sh, x[0]);
                 tmem_wait_ld();
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if (NX == 2 && q < 3) tmem_ld32(sS + 32 * (q + 1), x[(q + 1) % NX]);
-                    uint32_t* xs = x[q % NX];
+                for (int q = 0; q < 2; ++q) {
+                    if (q == 0) tmem_ld32(sh + 32, x[1]);  // in flight meanwhile
+                    uint32_t* xs = x[q];
                     if (masked) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (!((see[q] >> e) & 1)) xs[e] = __float_as_uint(-INFINITY);
+                            if (!((see[2 * h + q] >> e) & 1)) xs[e] = __float_as_uint(-INFINITY);
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const int c = 32 * q + e;
+                        const int c = c0 + 32 * q + e;
                         const float x0 = __uint_as_float(xs[e]), x1 = __uint_as_float(xs[e + 1]);
                         float t0, t1;
                         if constexpr (Q8) {
@@ -596,16 +755,21 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                         }
                         pk[16 * q + (e >> 1)] = MP::pack(p0, p1);
                     }
-                    if (NX == 1 && q < 3) tmem_ld32(sS + 32 * (q + 1), x[0]);
-                    if (q < 3) tmem_wait_ld();
+                    if (q == 0) tmem_wait_ld();
                 }
                 sum = (s0 + s1) + (s2 + s3);
                 const float mx = fmaxf(mx0, mx1) * (Q8 ? 1.f : rs);
                 const bool move = turn == 0 && (mx > m + kKeepLog2 || (m == -INFINITY && mx > -INFINITY));
                 if (!__any_sync(kFull, move)) break;
-                // the block before's P V is done: S of this block was issued after it
                 const float corr = move ? ex2(m - mx) : 1.f;
-                if (j > 0) {
+                if (j > 0 || h > 0) {
+                    // O is between two products: those of the block before were done before this
+                    // block's S, the first half's are waited for, this half's wait for P
+                    if (h == 1) {
+                        got = mbar_wait(&bars.pv_done[t], (uses + (uint32_t)j) & 1, abort);
+                        if (!__all_sync(kFull, got)) break;
+                        tc_fence_after();
+                    }
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         uint32_t o[32];
@@ -619,49 +783,87 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 l *= corr;
                 if (move) m = mx;
             }
+            got = __all_sync(kFull, got);
+            if (!got) break;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) tmem_st16(sS + 16 * q, pk + 16 * q);
+            for (int q = 0; q < 2; ++q) tmem_st16(sh + 16 * q, pk + 16 * q);
             l += sum;
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&bars.p_full[t]);
+            mbar_arrive(&bars.p_full[t][h]);
+            }
+            if (!got) break;
         }
-        got = got && mbar_wait(&bars.o_full, 0, abort);
-        if (__all_sync(kFull, got)) {
+        got = got && mbar_wait(&bars.o_full, seg & 1, abort);
+        got = __all_sync(kFull, got);
+        ++seg;
+        n0 += (uint32_t)nblk;
+        if (t < ntile) uses += (uint32_t)nblk;
+        if (got && t < ntile) {
             tc_fence_after();
-            const bool whole = w.nparts == 1;
+            const bool whole = sg.slot < 0;
             const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            float* part = a.ws + ((trow_q * a.Hq + hq) * a.P + p) * (kD + 2);
+            float* part = whole ? nullptr : tree_partial(a, gridDim.x, blockIdx.x, sg.slot, NT * kRows, tid, kD);
+            // O leaves through Q's tile, which nothing reads any more: each thread its row
+            // there, then the warp whole rows (partials: half rows of 64 floats) to memory
+            const int hi = lane >> 4, c = lane & 15, w0 = (warp & 3) * 32;
+            const int64_t to = !live ? -1 : whole ? trow_q * a.ot + (int64_t)hq * a.oh : 0;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                uint32_t o[32];
-                tmem_ld32(sO + 32 * q, o);
-                tmem_wait_ld();
-                if (live && whole) {
-                    using P = Packed<T>;
+            for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint4 v;
-                        v.x = P::pack(__uint_as_float(o[8 * c]) * inv, __uint_as_float(o[8 * c + 1]) * inv);
-                        v.y = P::pack(__uint_as_float(o[8 * c + 2]) * inv, __uint_as_float(o[8 * c + 3]) * inv);
-                        v.z = P::pack(__uint_as_float(o[8 * c + 4]) * inv, __uint_as_float(o[8 * c + 5]) * inv);
-                        v.w = P::pack(__uint_as_float(o[8 * c + 6]) * inv, __uint_as_float(o[8 * c + 7]) * inv);
-                        st16(orow + 32 * q + 8 * c, v);
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t o[32];
+                    tmem_ld32(sO + 64 * half + 32 * q, o);
+                    tmem_wait_ld();
+                    if (whole) {
+                        using P = Packed<T>;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            uint4 v;
+                            v.x = P::pack(__uint_as_float(o[8 * x]) * inv, __uint_as_float(o[8 * x + 1]) * inv);
+                            v.y = P::pack(__uint_as_float(o[8 * x + 2]) * inv, __uint_as_float(o[8 * x + 3]) * inv);
+                            v.z = P::pack(__uint_as_float(o[8 * x + 4]) * inv, __uint_as_float(o[8 * x + 5]) * inv);
+                            v.w = P::pack(__uint_as_float(o[8 * x + 6]) * inv, __uint_as_float(o[8 * x + 7]) * inv);
+                            *reinterpret_cast<uint4*>(qtile + tile_off(r, 8 * half + 4 * q + x)) = v;
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            *reinterpret_cast<uint4*>(qtile + tile_off(r, 8 * q + x)) =
+                                make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
                     }
-                } else if (live) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2)
-                        *reinterpret_cast<float2*>(part + 32 * q + e) =
-                            make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
                 }
-                __syncwarp();  // the next quarter's load is warp-wide
+                if (whole && half == 0) continue;
+                __syncwarp();
+#pragma unroll 4
+                for (int i = 0; i < 16; ++i) {
+                    const int rr = 2 * i + hi;
+                    const int64_t row = __shfl_sync(kFull, to, rr);
+                    const uint4 v = *reinterpret_cast<const uint4*>(qtile + tile_off(w0 + rr, c));
+                    if (row >= 0) {
+                        if (whole) {
+                            st16(reinterpret_cast<T*>(a.out) + row + 8 * c, v);
+                        } else {  // (rows of D + 2 floats: 8-byte aligned)
+                            float* dst = tree_partial(a, gridDim.x, blockIdx.x, sg.slot, NT * kRows,
+                                                      t * kRows + w0 + rr, kD) + 64 * half + 4 * c;
+                            *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
+                            *reinterpret_cast<uint2*>(dst + 2) = make_uint2(v.z, v.w);
+                        }
+                    }
+                }
+                __syncwarp();
             }
             if (live && !whole) *reinterpret_cast<float2*>(part + kD) = make_float2(m, l);
-            if (live && *static_cast<volatile int*>(&odd_v)) {  // (set before the last v_full, which o_full follows)
+            // (set before the last v_full, which o_full follows; the next segment's can only raise
+            // it, and makes this one look where nothing is to be found)
+            if (live && *static_cast<volatile int*>(&odd_v) >= seq_no) {
                 const int j0 = k_begin + min(first_draft, nblk) * kRows;
-                if (whole) add_not_finite<T, FMT, T>(a, bt, g, w.ctx, mrow, qrow, sl2, m, j0, k_end, orow);
-                else add_not_finite<T, FMT, float>(a, bt, g, w.ctx, mrow, qrow, sl2, m, j0, k_end, part);
+                if (whole) add_not_finite<T, FMT, T>(a, bt, sg.g, w.ctx, mrow, qrow, sl2, m, j0, k_end, orow);
+                else add_not_finite<T, FMT, float>(a, bt, sg.g, w.ctx, mrow, qrow, sl2, m, j0, k_end, part);
             }
+            __syncwarp();
+            tc_fence_before();  // O is read: the next segment's products follow q_full, or p_full
+        }
         }
     }
 
@@ -690,12 +892,10 @@ bool page_map(CUtensorMap* map, const char* ptr, const TreeDev& a, int bf16, int
 }
 
 template <typename T, int FMT, int NT>
-int launch_nt(const TreeDev& a, cudaStream_t stream) {
+int launch_nt(const TreeDev& a, int ctas, cudaStream_t stream) {
     constexpr auto kernel = tree_tc_kernel<T, FMT, NT>;
     const int rc = allow_smem<kernel>(TreeTc<NT>::SMEM);
     if (rc) return rc;
-    const int64_t groups = ceil_div((int64_t)a.max_tree * a.G, NT * kRows);
-    if (groups * a.Hkv > 65535) return QF_ERR_UNSUPPORTED;
     // The largest power of two that divides a page and a block: a piece never crosses a
     // page.  Below 8 (or where the cache's shape has no map) rows come one by one.
     CUtensorMap tk{}, tv{};
@@ -705,30 +905,29 @@ int launch_nt(const TreeDev& a, cudaStream_t stream) {
         box = std::min(a.B.d & -a.B.d, kRows);
         if (box < 8 || !page_map(&tk, a.kc, a, bf16, box) || !page_map(&tv, a.vc, a, bf16, box)) box = 0;
     }
-    kernel<<<dim3((unsigned)a.P, (unsigned)(groups * a.Hkv), (unsigned)a.S), TreeTc<NT>::THREADS,
-             TreeTc<NT>::SMEM, stream>>>(a, tk, tv, box);
+    kernel<<<(unsigned)ctas, TreeTc<NT>::THREADS, TreeTc<NT>::SMEM, stream>>>(a, tk, tv, box);
     return check_launch();
 }
 
 template <typename T, int FMT>
-int launch_fmt(const TreeDev& a, int tiles, cudaStream_t stream) {
-    return tiles == 1 ? launch_nt<T, FMT, 1>(a, stream) : launch_nt<T, FMT, 2>(a, stream);
+int launch_fmt(const TreeDev& a, int tiles, int ctas, cudaStream_t stream) {
+    return tiles == 1 ? launch_nt<T, FMT, 1>(a, ctas, stream) : launch_nt<T, FMT, 2>(a, ctas, stream);
 }
 
 template <typename T>
-int launch_t(const TreeDev& a, int format, int tiles, cudaStream_t stream) {
+int launch_t(const TreeDev& a, int format, int tiles, int ctas, cudaStream_t stream) {
     switch (format) {
-    case QF_CACHE_PLAIN: return launch_fmt<T, QF_CACHE_PLAIN>(a, tiles, stream);
-    case QF_CACHE_E4M3: return launch_fmt<T, QF_CACHE_E4M3>(a, tiles, stream);
-    default: return launch_fmt<T, QF_CACHE_INT8>(a, tiles, stream);
+    case QF_CACHE_PLAIN: return launch_fmt<T, QF_CACHE_PLAIN>(a, tiles, ctas, stream);
+    case QF_CACHE_E4M3: return launch_fmt<T, QF_CACHE_E4M3>(a, tiles, ctas, stream);
+    default: return launch_fmt<T, QF_CACHE_INT8>(a, tiles, ctas, stream);
     }
 }
 
 }  // namespace
 
-int launch_tree_tc(const TreeDev& a, int dtype, int format, int tiles, cudaStream_t stream) {
-    return dtype == QF_F16 ? launch_t<__half>(a, format, tiles, stream)
-                           : launch_t<__nv_bfloat16>(a, format, tiles, stream);
+int launch_tree_tc(const TreeDev& a, int dtype, int format, int tiles, int ctas, cudaStream_t stream) {
+    return dtype == QF_F16 ? launch_t<__half>(a, format, tiles, ctas, stream)
+                           : launch_t<__nv_bfloat16>(a, format, tiles, ctas, stream);
 }
 
 }  // namespace qf

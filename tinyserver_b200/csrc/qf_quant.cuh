@@ -18,6 +18,10 @@
 
 namespace qf {
 
+// The kernels that take log2 of a row's scale read a smaller one (0: a row never
+// written) as this.
+constexpr float kLeastScale = 7.52316384526264e-37f;  // 2^-120
+
 template <int FMT>
 __device__ __forceinline__ float code_top() {
     return FMT == QF_CACHE_E4M3 ? 448.f : 127.f;

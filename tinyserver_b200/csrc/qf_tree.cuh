@@ -45,49 +45,201 @@ struct TreeDev {
     float scale;
     char* out;
     int64_t ot, oh;
-    float* ws;  // [T][Hq][P][D + 2]: acc[0:D], max, sum
-    int P;      // partitions per sequence in the grid and the workspace
-    int part;   // keys per partition
+    float* ws;     // partials and records (TreeWs), or NULL: no sequence is split
+    int min_units;  // least work of a CTA, in key blocks
     int32_t* status;
 };
 
-// One sequence as every CTA of it sees it.
+// One sequence: its first query row, query tokens (at most max_tree), context
+// keys, and keys in all.  `report`: this thread flags what had to be cut.
 struct TreeSeq {
-    int q0, n;    // first query row, query tokens (at most max_tree)
-    int ctx, L;   // context keys, keys in all
-    int nparts;   // partitions with keys (at least 1)
+    int q0, n, ctx, L;
 };
 
-__device__ __forceinline__ TreeSeq tree_seq(const TreeDev& a, int s) {
+__device__ __forceinline__ TreeSeq tree_seq(const TreeDev& a, int s, bool report) {
     TreeSeq w;
     int ctx = __ldg(a.lens + s), bad = 0;
     if (ctx < 0) {
         ctx = 0;
         bad = QF_FLAG_BAD_TABLE;
     }
-    int keys_n = 0;  // drafted keys
+    int drafted = 0;
     if (a.cu) {
         const int b = __ldg(a.cu + s), e = __ldg(a.cu + s + 1);
         const int q0 = min(max(b, 0), a.T), q1 = min(max(e, q0), a.T);
         if (q0 != b || q1 != e) bad |= QF_FLAG_BAD_TABLE;
         w.q0 = q0;
-        keys_n = q1 - q0;
-        w.n = min(keys_n, a.max_tree);
-        if (w.n < keys_n) bad |= QF_FLAG_BAD_TREE;
-        keys_n = w.n;
+        w.n = min(q1 - q0, a.max_tree);
+        if (w.n < q1 - q0) bad |= QF_FLAG_BAD_TREE;
+        drafted = w.n;
     } else {
         w.q0 = s;
         w.n = 1;
     }
-    if (ctx > a.cap - keys_n) {  // (cap >= 0, keys_n >= 0: no overflow)
+    if (ctx > a.cap - drafted) {  // (cap, drafted >= 0: no overflow)
         bad |= QF_FLAG_BAD_TABLE;
         ctx = min(ctx, a.cap);
     }
     w.ctx = ctx;
-    w.L = min(ctx + keys_n, a.cap);
-    w.nparts = max(1, (w.L + a.part - 1) / a.part);
-    if (bad && threadIdx.x == 0) flag(a.status, bad);
+    w.L = min(ctx + drafted, a.cap);
+    if (bad && report) flag(a.status, bad);
     return w;
+}
+
+// ---------------------------------------------------------------------------
+// Who does what.  The work is a line of units, one unit a block of KB keys for
+// one tile group (ROWS rows) of one kv head of one sequence: sequence by
+// sequence, in it head by head and group by group, in that the keys in order.
+// gridDim.x CTAs, as many as fit on the GPU at once, take equal stretches of the
+// line, so lengths may be as ragged as they like.  A stretch cuts at most
+// two (sequence, head, group) items, its first and its last, so a CTA leaves at
+// most two partials, in its own slots of the workspace: slot 0 for an item that an
+// earlier CTA began, slot 1 for one that it begins and a later CTA goes on with.
+// Its record says what slot 0 belongs to, for the kernel that joins them.
+// Without a workspace a CTA does whole items: those that begin in its stretch.
+struct TreeRec {
+    int s, g, rg;
+    int last;  // the last CTA of slot 0's item; 0 unless the CTA before this one began it
+};
+
+struct TreeWs {  // workspace: records, then [CTA][2][ROWS][D + 2] floats: acc, reference, sum
+    __host__ __device__ static int64_t rec_floats(int64_t ctas) { return (ctas * 4 + 63) / 64 * 64; }
+    __host__ __device__ static int64_t floats(int64_t ctas, int64_t rows, int64_t d) {
+        return rec_floats(ctas) + ctas * 2 * rows * (d + 2);
+    }
+};
+
+struct TreeSeg {
+    TreeSeq w;
+    int s, g, rg;
+    int k_begin, k_end;
+    int slot;  // of the partial; -1: the item is whole
+};
+
+template <int KB, int ROWS>
+struct TreeWalk {
+    int64_t pos, end, base, us;  // this CTA's stretch; the current sequence's first unit and units
+    int64_t per;                 // units of a stretch
+    int s, nb, ng;               // the current sequence, its key blocks and groups per head
+    TreeSeq w;
+
+    __device__ __forceinline__ static int blocks(const TreeSeq& w) { return max(1, (w.L + KB - 1) / KB); }
+    __device__ __forceinline__ static int groups(const TreeDev& a, const TreeSeq& w) {
+        return (int)(((int64_t)w.n * a.G + ROWS - 1) / ROWS);
+    }
+    __device__ __forceinline__ static int64_t units(const TreeDev& a, const TreeSeq& w) {
+        return (int64_t)blocks(w) * groups(a, w) * a.Hkv;
+    }
+    __device__ __forceinline__ void enter(const TreeDev& a, int seq) {
+        s = seq;
+        w = tree_seq(a, s, false);
+        nb = blocks(w);
+        ng = groups(a, w);
+        us = units(a, w);
+    }
+
+    // By all threads of the CTA (`scratch`: 34 int64 of shared memory): the units
+    // of all sequences, this CTA's stretch, and the sequence it begins in.  CTA 0
+    // reports what had to be cut.
+    __device__ void begin(const TreeDev& a, int64_t* scratch) {
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
+        const int nt = nw * 32;
+        int64_t mine = 0;
+        for (int i = tid; i < a.S; i += nt) mine += units(a, tree_seq(a, i, blockIdx.x == 0));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+        if (lane == 0) scratch[warp] = mine;
+        __syncthreads();
+        int64_t total = 0;
+        for (int i = 0; i < nw; ++i) total += scratch[i];
+        per = max((int64_t)a.min_units, (total + gridDim.x - 1) / gridDim.x);
+        pos = min(total, per * blockIdx.x);
+        end = min(total, pos + per);
+        __syncthreads();
+        // the sequence with base <= pos < base + us, by scans of nt sequences
+        if (tid == 0) scratch[32] = -1;
+        int64_t before = 0;
+        for (int i0 = 0; i0 < a.S; i0 += nt) {
+            const int i = i0 + tid;
+            const int64_t u = i < a.S ? units(a, tree_seq(a, i, false)) : 0;
+            int64_t incl = u;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            if (lane == 31) scratch[warp] = incl;
+            __syncthreads();
+            int64_t warps = 0, all = 0;
+            for (int x = 0; x < nw; ++x) {
+                if (x < warp) warps += scratch[x];
+                all += scratch[x];
+            }
+            const int64_t first = before + warps + incl - u;
+            if (first <= pos && pos < first + u) {
+                scratch[32] = i;
+                scratch[33] = first;
+            }
+            before += all;
+            __syncthreads();
+            if (before > pos) break;
+        }
+        if (pos < end) {
+            base = scratch[33];
+            enter(a, (int)scratch[32]);
+        }
+        __syncthreads();
+    }
+
+    __device__ __forceinline__ bool next(const TreeDev& a, TreeSeg& t) {
+        while (pos < end) {
+            if (pos >= base + us) {
+                base += us;
+                enter(a, s + 1);
+                continue;
+            }
+            const int64_t rel = pos - base;
+            const int item = (int)(rel / nb), b0 = (int)(rel - (int64_t)item * nb);
+            if (!a.ws && b0 > 0) {  // an item of the CTA before
+                pos += nb - b0;
+                continue;
+            }
+            const int b1 = a.ws ? (int)min((int64_t)nb, b0 + (end - pos)) : nb;
+            t.w = w;
+            t.s = s;
+            t.g = item / ng;
+            t.rg = item - t.g * ng;
+            t.k_begin = b0 * KB;
+            t.k_end = min(w.L, b1 * KB);
+            t.slot = b0 > 0 ? 0 : b1 < nb ? 1 : -1;
+            pos += b1 - b0;
+            return true;
+        }
+        return false;
+    }
+
+    // By one thread, before the walk: the record of this CTA.
+    __device__ __forceinline__ void record(const TreeDev& a) const {
+        if (!a.ws) return;
+        TreeRec r{0, 0, 0, 0};
+        if (pos < end && pos > base) {
+            const int64_t rel = pos - base;
+            const int item = (int)(rel / nb), b0 = (int)(rel - (int64_t)item * nb);
+            const int64_t first = pos - b0;  // the item's first unit
+            if (b0 > 0 && first >= pos - per) {
+                r.s = s;
+                r.g = item / ng;
+                r.rg = item - r.g * ng;
+                r.last = (int)((first + nb - 1) / per);
+            }
+        }
+        reinterpret_cast<TreeRec*>(a.ws)[blockIdx.x] = r;
+    }
+};
+
+__device__ __forceinline__ float* tree_partial(const TreeDev& a, int64_t ctas, int64_t cta, int slot,
+                                               int rows, int row, int D) {
+    return a.ws + TreeWs::rec_floats(ctas) + ((cta * 2 + slot) * rows + row) * (D + 2);
 }
 
 // Element offset of key j's row of kv head g in the caches; and of its scale.
@@ -120,27 +272,27 @@ __device__ __forceinline__ uint32_t tree_bits32(const int64_t* row, int words, i
     return (uint32_t)v;
 }
 
-// Zero the rows of kv head g's query heads that no kernel computes: query
-// tokens of this sequence past max_tree, and, from the first and the last
-// sequence, the rows before and behind all sequences.
+// Zero the output rows that no item owns, all CTAs together: before the first
+// and behind the last sequence, and query tokens past max_tree.
 template <typename T, int D>
-__device__ __forceinline__ void zero_unowned_rows(const TreeDev& a, int s, int g, const TreeSeq& w) {
+__device__ __forceinline__ void zero_unowned_rows(const TreeDev& a) {
     if (!a.cu) return;
+    constexpr int CH = D * (int)sizeof(T) / 16;
     auto zero = [&](int t0, int t1) {
-        constexpr int CH = D * (int)sizeof(T) / 16;
-        const int64_t n = (int64_t)max(0, t1 - t0) * a.G * CH;
+        const int64_t n = (int64_t)max(0, t1 - t0) * a.Hq * CH;
         for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
             const int64_t r = i / CH;
-            const int c = (int)(i - r * CH), h = (int)(r % a.G);
-            T* o = reinterpret_cast<T*>(a.out) + (t0 + r / a.G) * a.ot + (int64_t)(g * a.G + h) * a.oh;
-            for (int e = 0; e < 16 / (int)sizeof(T); ++e)
-                o[c * (16 / (int)sizeof(T)) + e] = Dt<T>::from_f(0.f);
+            char* o = a.out + ((t0 + r / a.Hq) * a.ot + (r % a.Hq) * a.oh) * (int64_t)sizeof(T);
+            st16(o + (i - r * CH) * 16, make_uint4(0, 0, 0, 0));
         }
     };
-    const int b = min(max(__ldg(a.cu + s), 0), a.T), e = min(max(__ldg(a.cu + s + 1), b), a.T);
-    zero(b + w.n, e);
-    if (s == 0) zero(0, b);
-    if (s == a.S - 1) zero(e, a.T);
+    auto row = [&](int s) { return min(max(__ldg(a.cu + s), 0), a.T); };
+    if (blockIdx.x == 0) zero(0, row(0));
+    if (blockIdx.x == gridDim.x - 1) zero(max(row(a.S - 1), row(a.S)), a.T);
+    for (int s = blockIdx.x; s < a.S; s += gridDim.x) {
+        const int b = row(s), e = max(b, row(s + 1));
+        if (e - b > a.max_tree) zero(b + a.max_tree, e);
+    }
 }
 
 // Let a kernel take `bytes` of dynamic shared memory, once per device.
@@ -159,7 +311,9 @@ int allow_smem(int bytes) {
 
 // The 16-bit kernels: paged_tree_mma.cu for few rows per kv head (`rows` in the
 // longest tree), paged_tree_tc.cu for many at head_dim 128 (`tiles` of 128 per CTA).
-int launch_tree_mma(const TreeDev& a, int dtype, int format, int D, int rows, cudaStream_t stream);
-int launch_tree_tc(const TreeDev& a, int dtype, int format, int tiles, cudaStream_t stream);
+int tree_mma_ctas_per_sm(bool plain, int D, int rows);
+int launch_tree_mma(const TreeDev& a, int dtype, int format, int D, int rows, int ctas,
+                    cudaStream_t stream);
+int launch_tree_tc(const TreeDev& a, int dtype, int format, int tiles, int ctas, cudaStream_t stream);
 
 }  // namespace qf
