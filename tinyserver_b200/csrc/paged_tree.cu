@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const TreeDev a) {
     __shared__ int64_t scratch[34];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wr = warp % WR, wk = warp / WR;
-    TreeWalk<kF32Keys, NR> walk;
+    TreeWalk<kF32Keys, NR, 4> walk;
     walk.begin(a, scratch);
     zero_unowned_rows<float, D>(a);
     if (tid == 0) walk.record(a);

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
     const float sl2 = a.scale * 1.4426950408889634f;
     unsigned char* ring = smem + warp * R::WARP;
 
-    TreeWalk<kMmaKeys, NR> walk;
+    TreeWalk<kMmaKeys, NR, 4> walk;
     walk.begin(a, scratch);
     zero_unowned_rows<T, D>(a);
     if (tid == 0) walk.record(a);

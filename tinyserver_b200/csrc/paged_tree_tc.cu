@@ -15,9 +15,8 @@
 // Roles: 4 NT softmax warps, one MMA thread, a warp that brings K and one that
 // brings V.  16-bit pages come by TMA, one box per lane, where a block's keys are
 // all context; else (the drafted keys, the tail, pages whose size is no multiple of
-// 8) row by row with cp.async.  8-bit rows come into registers and, converted to
-// fp16 (exact), into the tile, the next block's codes in flight while this block's
-// tile is in use.
+// 8) row by row with cp.async.  8-bit rows land in half of their tile and are
+// converted to fp16 (exact) in place.
 //
 // What bounds it: a block is 64 KB of 16-bit K and V, ~2900 cycles of an SM's
 // share of HBM; a tile's softmax is 16384 exponentials, 1024 cycles of the MUFU,
@@ -27,10 +26,12 @@
 // Two tiles (more rows): one CTA per SM with two-deep rings; K and V meet 256 rows,
 // and tile 0's softmax overlaps tile 1's products.
 //
-// Quantised rows: K's scale multiplies the score; V's enters the exponent,
-// p' = 2^(t + log2 vs - m') in [0, 2^8], and the sum takes p' / vs, so that O / l is
-// the definition whatever the scales' range.  Where that range exceeds 2^90 the sum takes
-// its own exponential (p' may have underflowed where p has not).
+// Quantised rows: the codes go into the products as they are.  K's scale multiplies
+// the score, V's (times 2^x, x of the segment's first block) the probability before
+// its one rounding; the sum takes the probability alone.  A block with a scale
+// that 2^x does not bring into [2^-6, 2^6] has V's scale in the exponent instead,
+// p' = 2^(t + log2 vs + x - m), m being the maximum of that, so that p' fits fp16
+// whatever the scales' range.
 // P is rounded to the operand type (fp16 over quantised rows, else the query's):
 // half a step of the same size as the output's own.  Sums, maxima and O are fp32.
 //
@@ -50,8 +51,9 @@ namespace {
 
 constexpr int kD = 128;
 constexpr unsigned kFull = 0xffffffffu;
+constexpr int kItemBlocks = 4;      // what beginning and ending an item costs, in blocks
 constexpr float kKeepLog2 = 8.f;    // the reference maximum moves when the row's has grown by 2^8
-constexpr float kScaleRange = 90.f;  // log2 of the v-scales' ratio up to which one exponential will do
+constexpr float kScaleLog2 = 6.f;   // log2 of the v-scales (times 2^x) that a probability is multiplied by
 
 
 template <int NT>
@@ -72,7 +74,7 @@ struct TreeBars {
     uint64_t info_full[2 * NT];  // a block's valid bits and scales
     uint64_t s_full[NT], p_full[NT][2];  // P by halves of a block
     uint64_t pv_done[NT], o_full, drain;
-    uint64_t v_raw;  // a V tile that the loader still looks through has landed
+    uint64_t raw[2];  // a K, a V tile that its loader still works on has landed
 };
 
 __device__ __forceinline__ void proxy_fence() {
@@ -132,6 +134,46 @@ __device__ __forceinline__ bool clean_rows(char* tile, int r0, int r1, int lane)
         *at = v;
     }
     return true;
+}
+
+// By one warp: a tile's codes, which landed in its second slab (a row's 128 codes are
+// as long as half a row of fp16), into the fp16 tile, in place: a row is read by
+// eight lanes before any of them writes.  Rows from nk on are zero.  Infinities and NaN
+// in rows from d0 on are set to zero; whether there were any.
+template <int FMT>
+__device__ __forceinline__ bool expand(char* tile, int nk, int d0, int lane) {
+    const int c = lane & 7, r4 = lane >> 3;
+    uint32_t odd = 0;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 32; i0 += 8) {
+        uint4 raw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            raw[i] = *reinterpret_cast<const uint4*>(tile + kSlab + (4 * (i0 + i) + r4) * 128 + c * 16);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * (i0 + i) + r4;
+            uint4 lo, hi;
+            codes_to_f16<FMT>(raw[i].x, lo.x, lo.y);
+            codes_to_f16<FMT>(raw[i].y, lo.z, lo.w);
+            codes_to_f16<FMT>(raw[i].z, hi.x, hi.y);
+            codes_to_f16<FMT>(raw[i].w, hi.z, hi.w);
+            if (r >= nk) lo = hi = make_uint4(0, 0, 0, 0);
+            if (FMT == QF_CACHE_E4M3 && r >= d0) {
+                odd |= odd_pair<__half>(lo.x) | odd_pair<__half>(lo.y) | odd_pair<__half>(lo.z) |
+                       odd_pair<__half>(lo.w) | odd_pair<__half>(hi.x) | odd_pair<__half>(hi.y) |
+                       odd_pair<__half>(hi.z) | odd_pair<__half>(hi.w);
+                zero_not_finite<__half>(lo);
+                zero_not_finite<__half>(hi);
+            }
+            // (lanes of the second slab the odd chunk first: eight lanes, eight bank groups)
+            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + (c >> 2))) = c >> 2 ? hi : lo;
+            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + 1 - (c >> 2))) = c >> 2 ? lo : hi;
+        }
+        __syncwarp();
+    }
+    return __any_sync(kFull, odd != 0);
 }
 
 // q . k over the 128 dims on the CUDA cores, k a cache row.
@@ -233,10 +275,11 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     __shared__ int abort_flag, odd_v;  // odd_v: the last segment whose drafted V was not finite, from 1
     __shared__ int64_t scratch[34];
     __shared__ __align__(16) uint32_t valid[C::SLOTS][4];
-    // k-scale, log2 v-scale, 1 / v-scale of a block's keys; least and largest log2 v-scale
-    __shared__ __align__(16) float sk[Q8 ? C::SLOTS : 1][Q8 ? kRows : 1], sl[Q8 ? C::SLOTS : 1][Q8 ? kRows : 1],
-        sr_[Q8 ? C::SLOTS : 1][Q8 ? kRows : 1];
-    __shared__ float srange[Q8 ? C::SLOTS : 1][2];
+    // of a block's keys: k-scale, v-scale * 2^x, log2 of that; whether the block's all are
+    // near 1; x
+    __shared__ __align__(16) float sk[Q8 ? C::SLOTS : 1][Q8 ? kRows : 4], sv[Q8 ? C::SLOTS : 1][Q8 ? kRows : 4],
+        sl[Q8 ? C::SLOTS : 1][Q8 ? kRows : 4];
+    __shared__ int snear[C::SLOTS], sexp[C::SLOTS];
     volatile int* abort = &abort_flag;
 
     const uint32_t raw = smem_u32(dsm);
@@ -259,7 +302,8 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         }
         mbar_init(&bars.o_full, 1);
         mbar_init(&bars.drain, 1);
-        mbar_init(&bars.v_raw, 1);
+        mbar_init(&bars.raw[0], 1);
+        mbar_init(&bars.raw[1], 1);
         abort_flag = 0;
         odd_v = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -278,7 +322,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     const float sl2 = a.scale * 1.4426950408889634f;
 
     // every role walks the same segments; barrier phases run on across them
-    TreeWalk<kRows, NT * kRows> walk;
+    TreeWalk<kRows, NT * kRows, kItemBlocks> walk;
     walk.begin(a, scratch);
     zero_unowned_rows<T, kD>(a);
     if (tid == 0) walk.record(a);
@@ -324,27 +368,30 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         // What the softmax needs to know of a block's keys.  The slot's last reader, the
         // softmax SLOTS blocks ago, is done: S of ST blocks ago (whose K was in this
         // stage) came after it.
-        auto inform = [&](int slot) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                if (lane == 0) valid[slot][x] = ok[x];
-                if constexpr (Q8) {
-                    sk[slot][x * 32 + lane] = ks[x];
-                    sl[slot][x * 32 + lane] = log2f(vs[x]);
-                    sr_[slot][x * 32 + lane] = 1.f / vs[x];
-                }
-            }
+        int vexp = 0;  // x
+        auto inform = [&](int slot, bool first) {
+            if (lane == 0) *reinterpret_cast<uint4*>(valid[slot]) = make_uint4(ok[0], ok[1], ok[2], ok[3]);
             if constexpr (Q8) {
-                float hi = -INFINITY, lo = -INFINITY;
+                if (first) {
+                    float top = 0.f;
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    if ((ok[x] >> lane) & 1) {
-                        hi = fmaxf(hi, log2f(vs[x]));
-                        lo = fmaxf(lo, -log2f(vs[x]));
-                    }
-                hi = warp_max(hi);
-                lo = -warp_max(lo);
-                if (lane == 0) srange[slot][0] = lo, srange[slot][1] = hi;
+                    for (int x = 0; x < 4; ++x)
+                        if ((ok[x] >> lane) & 1) top = fmaxf(top, vs[x]);
+                    top = warp_max(top);
+                    vexp = 127 - min(max((int)(__float_as_uint(top) >> 23), 127 - 100), 127 + 100);
+                }
+                const float f = __int_as_float((127 + vexp) << 23);
+                bool near = true;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float v = vs[x] * f, lv = log2f(vs[x]) + (float)vexp;
+                    if ((ok[x] >> lane) & 1) near = near && fabsf(lv) <= kScaleLog2;  // (a NaN is not near)
+                    sk[slot][x * 32 + lane] = ks[x];
+                    sv[slot][x * 32 + lane] = v;
+                    sl[slot][x * 32 + lane] = lv;
+                }
+                near = __all_sync(kFull, near);
+                if (lane == 0) snear[slot] = near, sexp[slot] = vexp;
             }
             __syncwarp();
             mbar_arrive(&bars.info_full[slot]);
@@ -355,162 +402,114 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         };
         bool go = true;
         int seq_no = 0;  // segments begun
-        if constexpr (Q8) {
-            // codes into registers, 16 rows' worth a lane group in flight all the time: half a
-            // block is converted and stored while the other half, then the next block's, comes
-            uint4 raws[16];
-            const int c = lane & 7;
-            auto fetch = [&](int i, int half) {
-                const int r = (4 * i + (lane >> 3)) & 31, x = 2 * half + (i >> 3);
-                const int64_t o = __shfl_sync(kFull, x == 0 ? off[0] : x == 1 ? off[1] : x == 2 ? off[2] : off[3], r);
-                const unsigned m = x == 0 ? ok[0] : x == 1 ? ok[1] : x == 2 ? ok[2] : ok[3];
-                raws[i] = (m >> r) & 1 ? ld_stream16(src + o + c * 16) : make_uint4(0, 0, 0, 0);
-            };
-            bool more = walk.next(a, sg);
+        const CUtensorMap* map = side ? &tv : &tk;
+        const int hi = lane >> 4, c = lane & 15;
+        // this lane's piece of a block: `box` slots of one page, 64 dims of them or all codes
+        const int pc = Q8 ? lane : lane >> 1;
+        int n = 0, raw = 0;  // blocks, worked-on tiles of all segments
+        int blk = 0, slot0 = 0;
+        auto look = [&](int j) {  // the page and first slot of this lane's piece of block j
+            const int kb = sg.k_begin + j * kRows;
+            const int key = kb + (pc * box < min(kRows, sg.k_end - kb) ? pc * box : 0);
+            const int lb = a.B.div(key);
+            blk = __ldg(bt + lb);
+            slot0 = key - lb * a.B.d;
+        };
+        while (go && walk.next(a, sg)) {
             ++seq_no;
-            if (more) {
-                bt = a.bt + (int64_t)sg.s * a.bts;
-                locate(0);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) fetch(i, 0);
-            }
-            int j = 0, n = 0;  // block of the segment, of all segments
-            while (more) {
-                const int nblk = blocks_of(), first_draft = draft_of(nblk);
-                if (nblk == 0) {  // (a sequence without keys: nothing was fetched but zeros)
-                    more = walk.next(a, sg);
-                    ++seq_no;
-                    if (more) {
-                        bt = a.bt + (int64_t)sg.s * a.bts;
-                        locate(0);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) fetch(i, 0);
-                    }
-                    continue;
-                }
-                const int st = n % ST;
+            bt = a.bt + (int64_t)sg.s * a.bts;
+            const int nblk = blocks_of(), k_end = sg.k_end;
+            if (box > 0 && nblk > 0) look(0);
+            for (int j = 0; j < nblk; ++j, ++n) {
+                const int st = n % ST, kb = sg.k_begin + j * kRows, nk = min(kRows, k_end - kb);
                 char* tile = tiles + st * kTile;
-                if (!vacant(n)) break;
-                if (side == 0) inform(n % C::SLOTS);
-                const bool drafted = j >= first_draft;
-                const int own_no = seq_no;
-                ++n;
-                bool odd = false;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (half == 1) {  // the block after this one, of the next segment if need be
-                        if (++j == nblk) {
-                            j = 0;
-                            more = walk.next(a, sg);
-                            ++seq_no;
-                            if (more) bt = a.bt + (int64_t)sg.s * a.bts;
-                        }
-                        if (more) locate(j);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int r = half * 64 + 4 * i + (lane >> 3);
-                        uint4 lo, hi;
-                        codes_to_f16<FMT>(raws[i].x, lo.x, lo.y);
-                        codes_to_f16<FMT>(raws[i].y, lo.z, lo.w);
-                        codes_to_f16<FMT>(raws[i].z, hi.x, hi.y);
-                        codes_to_f16<FMT>(raws[i].w, hi.z, hi.w);
-                        if (half == 0) fetch(i, 1);
-                        else if (more) fetch(i, 0);
-                        if (FMT == QF_CACHE_E4M3 && side == 1 && drafted) {
-                            odd |= (odd_pair<__half>(lo.x) | odd_pair<__half>(lo.y) | odd_pair<__half>(lo.z) |
-                                    odd_pair<__half>(lo.w) | odd_pair<__half>(hi.x) | odd_pair<__half>(hi.y) |
-                                    odd_pair<__half>(hi.z) | odd_pair<__half>(hi.w)) != 0;
-                            zero_not_finite<__half>(lo);
-                            zero_not_finite<__half>(hi);
-                        }
-                        *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c)) = lo;
-                        *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + 1)) = hi;
-                    }
+                // rows of V that some query row may not see
+                const int d0 = a.cu ? max(0, sg.w.ctx - kb) : kRows;
+                bool bulk = box > 0;
+                const bool mine = pc * box < nk;
+                if (bulk) bulk = __all_sync(kFull, blk >= 0 && blk < a.N);
+                if (!bulk) locate(j);
+                if (!vacant(n)) {
+                    go = false;
+                    break;
                 }
-                if (odd) odd_v = own_no;
-                proxy_fence();
-                mbar_arrive(&full[st]);
-            }
-        } else {
-            const CUtensorMap* map = side ? &tv : &tk;
-            const int hi = lane >> 4, c = lane & 15;
-            const int pc = lane >> 1;  // this lane's piece of a block: `box` slots of one page, 64 dims
-            int n = 0, raw = 0;        // blocks, looked-through V tiles of all segments
-            while (go && walk.next(a, sg)) {
-                ++seq_no;
-                bt = a.bt + (int64_t)sg.s * a.bts;
-                const int nblk = blocks_of(), k_end = sg.k_end;
-                for (int j = 0; j < nblk; ++j, ++n) {
-                    const int st = n % ST, kb = sg.k_begin + j * kRows, nk = min(kRows, k_end - kb);
-                    char* tile = tiles + st * kTile;
-                    // rows of V that some query row may not see
-                    const int d0 = a.cu ? max(0, sg.w.ctx - kb) : kRows;
-                    bool bulk = box > 0;
-                    int blk = 0, slot0 = 0;
-                    const bool mine = pc * box < nk;
-                    if (bulk) {
-                        const int key = kb + (mine ? pc * box : 0);
-                        const int lb = a.B.div(key);
-                        blk = __ldg(bt + lb);
-                        slot0 = key - lb * a.B.d;
-                        bulk = __all_sync(kFull, blk >= 0 && blk < a.N);
+                // whether this warp works on the tile before the tensor core may have it
+                const bool work = Q8 || (side == 1 && (nk < kRows || d0 < nk));
+                if (bulk) {
+                    // (K behind the last key may hold anything: those columns are masked)
+                    uint64_t* bar = work ? &bars.raw[side] : &full[st];
+                    const uint32_t bytes = (uint32_t)((nk + box - 1) / box * box) * (Q8 ? 128u : 256u);
+                    if (lane == 0) mbar_expect_tx(bar, bytes);
+                    else if (!work) mbar_arrive(bar);
+                    __syncwarp();
+                    if (mine) {
+                        if constexpr (Q8)
+                            tma_page(tile + kSlab + pc * box * 128, map, 0, slot0, sg.g, blk, bar);
+                        else
+                            tma_page(tile + (lane & 1) * kSlab + pc * box * 128, map, (lane & 1) * 64, slot0, sg.g, blk,
+                                     bar);
                     }
-                    if (bulk) {
+                    if (j + 1 < nblk) look(j + 1);
+                    if (side == 0) {  // meanwhile, what the softmax needs to know
+                        if (Q8) locate(j);
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
                             ok[x] = nk >= 32 * (x + 1) ? kFull : nk > 32 * x ? (1u << (nk - 32 * x)) - 1u : 0u;
-                    } else {
-                        locate(j);
+                        inform(n % C::SLOTS, j == 0);
                     }
-                    if (!vacant(n)) {
+                    if (!work) continue;
+                    if (!__all_sync(kFull, mbar_wait(bar, raw++ & 1, nullptr))) {
                         go = false;
                         break;
                     }
-                    if (side == 0) inform(n % C::SLOTS);
-                    const bool look = side == 1 && (nk < kRows || d0 < nk);
-                    if (bulk) {
-                        // K behind the last key may hold anything: those columns are masked
-                        uint64_t* bar = look ? &bars.v_raw : &full[st];
-                        const uint32_t bytes = (uint32_t)((nk + box - 1) / box * box) * 256u;
-                        if (lane == 0) mbar_expect_tx(bar, bytes);
-                        else if (!look) mbar_arrive(bar);
-                        __syncwarp();
-                        if (mine)
-                            tma_page(tile + (lane & 1) * kSlab + pc * box * 128, map, (lane & 1) * 64, slot0, sg.g,
-                                     blk, bar);
-                        if (!look) continue;
-                        if (!__all_sync(kFull, mbar_wait(&bars.v_raw, raw++ & 1, nullptr))) {
-                            go = false;
-                            break;
-                        }
+                    if (!Q8)
                         for (int r = nk + hi; r < kRows; r += 2)
                             *reinterpret_cast<uint4*>(tile + tile_off(r, c)) = make_uint4(0, 0, 0, 0);
-                    } else {
-                        // row by row: chunk c of rows 2 i + hi; the swizzle repeats every four i
-                        const uint32_t dst = smem_u32(tile) + (uint32_t)((c >> 3) * kSlab + hi * 128);
-                        const char* from = src + c * 16;
+                } else if constexpr (Q8) {  // row by row, 16 codes a lane
+                    if (box > 0 && j + 1 < nblk) look(j + 1);
+                    const uint32_t dst = smem_u32(tile) + (uint32_t)(kSlab + (lane >> 3) * 128 + (lane & 7) * 16);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
+                    for (int x = 0; x < 4; ++x)
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const int64_t o = __shfl_sync(kFull, off[x], 2 * i + hi);
-                                cp_async16_at(dst + (uint32_t)((x * 32 + 2 * i) * 128 + (((c & 7) ^ ((2 * i & 7) + hi)) << 4)),
-                                              from + o, (ok[x] >> (2 * i + hi)) & 1 ? 16 : 0);
-                            }
+                        for (int i = 0; i < 8; ++i) {
+                            const int r = 4 * i + (lane >> 3);
+                            const int64_t o = __shfl_sync(kFull, off[x], r);
+                            cp_async16_at(dst + (uint32_t)((x * 32 + 4 * i) * 128), src + o + (lane & 7) * 16,
+                                          (ok[x] >> r) & 1 ? 16 : 0);
                         }
-                        cp_async_commit();
-                        cp_async_wait<0>();
-                        __syncwarp();
+                    cp_async_commit();
+                    if (side == 0) inform(n % C::SLOTS, j == 0);
+                    cp_async_wait<0>();
+                    __syncwarp();
+                } else {  // chunk c of rows 2 i + hi; the swizzle repeats every four i
+                    if (box > 0 && j + 1 < nblk) look(j + 1);
+                    const uint32_t dst = smem_u32(tile) + (uint32_t)((c >> 3) * kSlab + hi * 128);
+                    const char* from = src + c * 16;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int64_t o = __shfl_sync(kFull, off[x], 2 * i + hi);
+                            cp_async16_at(dst + (uint32_t)((x * 32 + 2 * i) * 128 + (((c & 7) ^ ((2 * i & 7) + hi)) << 4)),
+                                          from + o, (ok[x] >> (2 * i + hi)) & 1 ? 16 : 0);
+                        }
                     }
-                    if (look && d0 < nk && clean_rows<MT>(tile, d0, nk, lane)) odd_v = seq_no;
-                    proxy_fence();
-                    mbar_arrive(&full[st]);
+                    cp_async_commit();
+                    if (side == 0) inform(n % C::SLOTS, j == 0);
+                    cp_async_wait<0>();
+                    __syncwarp();
                 }
+                if constexpr (Q8) {
+                    if (expand<FMT>(tile, side == 1 ? nk : kRows, side == 1 ? d0 : kRows, lane)) odd_v = seq_no;
+                } else {
+                    if (work && d0 < nk && clean_rows<MT>(tile, d0, nk, lane)) odd_v = seq_no;
+                }
+                proxy_fence();
+                mbar_arrive(&full[st]);
             }
-            // every copy issued has landed before the CTA can leave
-            for (int d = max(0, n - ST); d < n; ++d) mbar_wait(&full[d % ST], (d / ST) & 1, nullptr);
         }
+        // every copy issued has landed before the CTA can leave
+        for (int d = max(0, n - ST); d < n; ++d) mbar_wait(&full[d % ST], (d / ST) & 1, nullptr);
     } else if (warp == C::MMA_WARP) {
         // ---- MMA issue, the warp together and one lane for it: S_t,0 | PV_t,j by the two
         // halves of P, S_t,j+1 | ...
@@ -619,47 +618,42 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             using P = Packed<T>;
             const int hi = lane >> 4, c = lane & 15;
             const int64_t at = live ? trow_q * a.qt + (int64_t)hq * a.qh : -1;
-            uint32_t flip = 0;
-            if (!Q8) {  // rs > 0: a negative scale's sign goes to Q, and 0 becomes as good as 0
-                flip = sl2 < 0.f ? 0x80008000u : 0u;
-                rs = fabsf(sl2) < 1e-30f ? 1e-30f : fabsf(sl2);
+            // rs > 0: a negative scale's sign goes to Q, and 0 becomes as good as 0
+            const uint32_t flip = sl2 < 0.f ? 0x80008000u : 0u;
+            const float sl_abs = fabsf(sl2) < 1e-30f ? 1e-30f : fabsf(sl2);
+            if (!Q8) rs = sl_abs;
+            uint4 v[16];  // all in flight
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int64_t o = __shfl_sync(kFull, at, 2 * i + hi);
+                v[i] = o >= 0 ? ld_stream16(reinterpret_cast<const T*>(a.q) + o + 8 * c) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (int i0 = 0; i0 < 16; i0 += 8) {
-                uint4 v[8];
+            for (int i = 0; i < 16; ++i) {
+                if constexpr (Q8) {  // a power-of-two factor brings the row's largest element to [2^14, 2^15)
+                    uint32_t mx = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int64_t o = __shfl_sync(kFull, at, 2 * (i0 + i) + hi);
-                    v[i] = o >= 0 ? ld_shared_ro16(reinterpret_cast<const T*>(a.q) + o + 8 * c) : make_uint4(0, 0, 0, 0);
+                    for (int x = 0; x < 4; ++x)
+                        mx = max(mx, max(__float_as_uint(P::lo(word(v[i], x))) & 0x7fffffffu,
+                                         __float_as_uint(P::hi(word(v[i], x))) & 0x7fffffffu));
+#pragma unroll
+                    for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
+                    const int e = min(max((int)(mx >> 23) - 127, -100), 127);
+                    const float f = __int_as_float((127 + 14 - e) << 23);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        set_word(v[i], x, MP::pack(P::lo(word(v[i], x)) * f, P::hi(word(v[i], x)) * f));
+                    const int er = __shfl_sync(kFull, e, (lane & 1) * 16);  // lane's own row's, if it is one of these
+                    if ((lane >> 1) == i) rs = fmaxf(sl_abs * __int_as_float((127 - 14 + er) << 23), 1.2e-38f);
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if constexpr (Q8) {  // a power-of-two factor brings the row's largest element to [2^14, 2^15)
-                        uint32_t mx = 0;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            mx = max(mx, max(__float_as_uint(P::lo(word(v[i], x))) & 0x7fffffffu,
-                                             __float_as_uint(P::hi(word(v[i], x))) & 0x7fffffffu));
-#pragma unroll
-                        for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
-                        const int e = min(max((int)(mx >> 23) - 127, -100), 127);
-                        const float f = __int_as_float((127 + 14 - e) << 23);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            set_word(v[i], x, MP::pack(P::lo(word(v[i], x)) * f, P::hi(word(v[i], x)) * f));
-                        const int er = __shfl_sync(kFull, e, (lane & 1) * 16);  // lane's own row's, if it is one of these
-                        if ((lane >> 1) == i0 + i) rs = sl2 * __int_as_float((127 - 14 + er) << 23);
-                    } else {
-                        v[i].x ^= flip, v[i].y ^= flip, v[i].z ^= flip, v[i].w ^= flip;
-                    }
-                    *reinterpret_cast<uint4*>(qtile + tile_off((warp & 3) * 32 + 2 * (i0 + i) + hi, c)) = v[i];
-                }
+                v[i].x ^= flip, v[i].y ^= flip, v[i].z ^= flip, v[i].w ^= flip;
+                *reinterpret_cast<uint4*>(qtile + tile_off((warp & 3) * 32 + 2 * i + hi, c)) = v[i];
             }
             proxy_fence();
             mbar_arrive(&bars.q_full);
         }
         float m = -INFINITY, l = 0.f;  // reference maximum and the sum against it
-        float lvtop = -INFINITY;       // largest log2 v-scale so far
+        float unscale = 1.f;           // 2^-x
         for (int j = 0; t < ntile && j < nblk; ++j) {
             const uint32_t nb = n0 + (uint32_t)j;
             const int slot = (int)(nb % C::SLOTS), kb = k_begin + j * kRows;
@@ -686,16 +680,10 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             for (int h = 0; h < 2; ++h) {
             const int c0 = 64 * h;
             const uint32_t sh = sS + (uint32_t)c0;
-            // Scores in log2 units, with V's scale where there is one: 16-bit rows x * rs,
-            // rs > 0 (a negative scale is in Q), so the maximum is that of x.
-            auto score = [&](float x, int c) -> float {
-                if constexpr (Q8) return fmaf(x * rs, sk[slot][c], sl[slot][c]);
-                else return x;
-            };
-            bool wide = false;
+            bool near = true;
             if constexpr (Q8) {
-                lvtop = fmaxf(lvtop, srange[slot][1]);
-                wide = lvtop - srange[slot][0] > kScaleRange;
+                near = snear[slot] != 0;
+                if (j == 0 && h == 0) unscale = __int_as_float((127 - sexp[slot]) << 23);
             }
             // One pass over S against the reference m, P in registers, the half block's maximum
             // on the side.  While no row's maximum has grown past 2^8 (but for the first blocks,
@@ -714,51 +702,59 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 for (int q = 0; q < 2; ++q) {
                     if (q == 0) tmem_ld32(sh + 32, x[1]);  // in flight meanwhile
                     uint32_t* xs = x[q];
-                    if (masked) {
+                    const int cq = c0 + 32 * q;
+                    if constexpr (Q8) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 k4 = *reinterpret_cast<const float4*>(&sk[slot][cq + e]);
+                            float* f = reinterpret_cast<float*>(xs + e);
+                            mul2(f[0], f[1], k4.x, k4.y);
+                            mul2(f[2], f[3], k4.z, k4.w);
+                        }
+                    }
+                    if (masked) {  // (an unseen key's score may be anything)
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (!((see[2 * h + q] >> e) & 1)) xs[e] = __float_as_uint(-INFINITY);
                     }
+                    if (!Q8 || near) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const int c = c0 + 32 * q + e;
-                        const float x0 = __uint_as_float(xs[e]), x1 = __uint_as_float(xs[e + 1]);
-                        float t0, t1;
-                        if constexpr (Q8) {
-                            t0 = score(x0, c);
-                            t1 = score(x1, c + 1);
-                            if (masked) {  // an unseen key's scales may be anything
-                                if (x0 == -INFINITY) t0 = -INFINITY;
-                                if (x1 == -INFINITY) t1 = -INFINITY;
+                        for (int e = 0; e < 32; e += 4) {
+                            float p[4];
+                            // raw maxima: rs > 0 (a negative scale's sign is in Q)
+                            mx0 = max3(mx0, __uint_as_float(xs[e]), __uint_as_float(xs[e + 1]));
+                            mx1 = max3(mx1, __uint_as_float(xs[e + 2]), __uint_as_float(xs[e + 3]));
+                            fma2(p[0], p[1], __uint_as_float(xs[e]), __uint_as_float(xs[e + 1]), rs, -mref);
+                            fma2(p[2], p[3], __uint_as_float(xs[e + 2]), __uint_as_float(xs[e + 3]), rs, -mref);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) p[x] = ex2(p[x]);
+                            add2(s0, s1, p[0], p[1]);
+                            add2(s2, s3, p[2], p[3]);
+                            if constexpr (Q8) {
+                                const float4 v4 = *reinterpret_cast<const float4*>(&sv[slot][cq + e]);
+                                mul2(p[0], p[1], v4.x, v4.y);
+                                mul2(p[2], p[3], v4.z, v4.w);
                             }
-                            mx0 = max3(mx0, t0, t1);
-                            t0 -= mref;
-                            t1 -= mref;
-                        } else {
-                            if (e & 2) mx1 = max3(mx1, x0, x1);
-                            else mx0 = max3(mx0, x0, x1);
-                            fma2(t0, t1, x0, x1, rs, -mref);
+                            pk[16 * q + (e >> 1)] = MP::pack(p[0], p[1]);
+                            pk[16 * q + (e >> 1) + 1] = MP::pack(p[2], p[3]);
                         }
-                        const float p0 = ex2(t0), p1 = ex2(t1);
-                        if constexpr (Q8) {
-                            if (!wide) {
-                                s0 = fmaf(p0, !masked || t0 != -INFINITY ? sr_[slot][c] : 0.f, s0);
-                                s1 = fmaf(p1, !masked || t1 != -INFINITY ? sr_[slot][c + 1] : 0.f, s1);
-                            } else {
-                                s0 += t0 == -INFINITY ? 0.f : ex2(t0 - sl[slot][c]);
-                                s1 += t1 == -INFINITY ? 0.f : ex2(t1 - sl[slot][c + 1]);
-                            }
-                        } else if (e & 2) {
-                            add2(s2, s3, p0, p1);
-                        } else {
-                            add2(s0, s1, p0, p1);
+                    } else {  // V's scales in the exponent
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const float x0 = __uint_as_float(xs[e]), x1 = __uint_as_float(xs[e + 1]);
+                            const float2 l2 = *reinterpret_cast<const float2*>(&sl[slot][cq + e]);
+                            const float t0 = x0 * rs, t1 = x1 * rs;
+                            const float u0 = x0 == -INFINITY ? x0 : t0 + l2.x, u1 = x1 == -INFINITY ? x1 : t1 + l2.y;
+                            mx0 = max3(mx0, u0, u1);
+                            s0 += ex2(t0 - mref);
+                            s1 += ex2(t1 - mref);
+                            pk[16 * q + (e >> 1)] = MP::pack(ex2(u0 - mref), ex2(u1 - mref));
                         }
-                        pk[16 * q + (e >> 1)] = MP::pack(p0, p1);
                     }
                     if (q == 0) tmem_wait_ld();
                 }
                 sum = (s0 + s1) + (s2 + s3);
-                const float mx = fmaxf(mx0, mx1) * (Q8 ? 1.f : rs);
+                const float mx = fmaxf(mx0, mx1) * (near ? rs : 1.f);
                 const bool move = turn == 0 && (mx > m + kKeepLog2 || (m == -INFINITY && mx > -INFINITY));
                 if (!__any_sync(kFull, move)) break;
                 const float corr = move ? ex2(m - mx) : 1.f;
@@ -802,7 +798,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         if (got && t < ntile) {
             tc_fence_after();
             const bool whole = sg.slot < 0;
-            const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            const float inv = unscale * (!whole ? 1.f : l == 0.f ? 0.f : 1.f / l);
             float* part = whole ? nullptr : tree_partial(a, gridDim.x, blockIdx.x, sg.slot, NT * kRows, tid, kD);
             // O leaves through Q's tile, which nothing reads any more: each thread its row
             // there, then the warp whole rows (partials: half rows of 64 floats) to memory
@@ -830,7 +826,10 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
 #pragma unroll
                         for (int x = 0; x < 8; ++x)
                             *reinterpret_cast<uint4*>(qtile + tile_off(r, 8 * q + x)) =
-                                make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                                make_uint4(__float_as_uint(__uint_as_float(o[4 * x]) * inv),
+                                           __float_as_uint(__uint_as_float(o[4 * x + 1]) * inv),
+                                           __float_as_uint(__uint_as_float(o[4 * x + 2]) * inv),
+                                           __float_as_uint(__uint_as_float(o[4 * x + 3]) * inv));
                     }
                 }
                 if (whole && half == 0) continue;
@@ -877,17 +876,19 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     }
 }
 
-// A map over a 16-bit cache (128 dims, B slots, Hkv heads, N blocks), boxes of 64 dims x `box` slots.
-bool page_map(CUtensorMap* map, const char* ptr, const TreeDev& a, int bf16, int box) {
+// A map over a cache (128 dims, B slots, Hkv heads, N blocks): boxes of `box` slots x 64
+// dims in the 128-byte swizzle, or x all 128 codes as they are.
+bool page_map(CUtensorMap* map, const char* ptr, const TreeDev& a, CUtensorMapDataType type, int box) {
     PFN_cuTensorMapEncodeTiled fn = tensor_map_encode();
     if (!fn || a.N <= 0) return false;
     const cuuint64_t dims[4] = {kD, (cuuint64_t)a.B.d, (cuuint64_t)a.Hkv, (cuuint64_t)a.N};
-    const cuuint64_t strides[3] = {(cuuint64_t)a.c2 * 2, (cuuint64_t)a.c1 * 2, (cuuint64_t)a.c0 * 2};
-    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
+    const bool codes = type == CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const cuuint64_t es = codes ? 1 : 2;
+    const cuuint64_t strides[3] = {(cuuint64_t)a.c2 * es, (cuuint64_t)a.c1 * es, (cuuint64_t)a.c0 * es};
+    const cuuint32_t boxes[4] = {codes ? 128u : 64u, (cuuint32_t)box, 1, 1};
     const cuuint32_t step[4] = {1, 1, 1, 1};
-    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-              const_cast<char*>(ptr), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    return fn(map, type, 4, const_cast<char*>(ptr), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              codes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -897,14 +898,15 @@ int launch_nt(const TreeDev& a, int ctas, cudaStream_t stream) {
     const int rc = allow_smem<kernel>(TreeTc<NT>::SMEM);
     if (rc) return rc;
     // The largest power of two that divides a page and a block: a piece never crosses a
-    // page.  Below 8 (or where the cache's shape has no map) rows come one by one.
+    // page.  Below 8 (the swizzle's rows; codes: 4, a lane per piece), or where the
+    // cache's strides make no map, rows come one by one.
+    constexpr bool Q8 = FMT != QF_CACHE_PLAIN;
+    const CUtensorMapDataType type = Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     CUtensorMap tk{}, tv{};
-    int box = 0;
-    if (FMT == QF_CACHE_PLAIN) {
-        const int bf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-        box = std::min(a.B.d & -a.B.d, kRows);
-        if (box < 8 || !page_map(&tk, a.kc, a, bf16, box) || !page_map(&tv, a.vc, a, bf16, box)) box = 0;
-    }
+    int box = std::min(a.B.d & -a.B.d, kRows);
+    if (box < (Q8 ? 4 : 8) || !page_map(&tk, a.kc, a, type, box) || !page_map(&tv, a.vc, a, type, box)) box = 0;
     kernel<<<(unsigned)ctas, TreeTc<NT>::THREADS, TreeTc<NT>::SMEM, stream>>>(a, tk, tv, box);
     return check_launch();
 }

@@ -171,6 +171,15 @@ __device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, f
         : "f"(a0), "f"(a1), "f"(b), "f"(c));
 }
 
+// (s0, s1) *= (a0, a1) as one packed fp32x2 multiply.
+__device__ __forceinline__ void mul2(float& s0, float& s1, float a0, float a1) {
+    asm("{\n\t.reg .b64 rs, ra;\n\t"
+        "mov.b64 rs, {%0, %1};\n\tmov.b64 ra, {%2, %3};\n\t"
+        "mul.rn.f32x2 rs, rs, ra;\n\tmov.b64 {%0, %1}, rs;\n\t}"
+        : "+f"(s0), "+f"(s1)
+        : "f"(a0), "f"(a1));
+}
+
 // (s0, s1) += (a0, a1) as one packed fp32x2 add.
 __device__ __forceinline__ void add2(float& s0, float& s1, float a0, float a1) {
     asm("{\n\t.reg .b64 rs, ra;\n\t"

@@ -96,6 +96,8 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeDev& a, int s, bool report
 // most two partials, in its own slots of the workspace: slot 0 for an item that an
 // earlier CTA began, slot 1 for one that it begins and a later CTA goes on with.
 // Its record says what slot 0 belongs to, for the kernel that joins them.
+// An item begins with EXTRA units without keys, what Q and O cost in units, so that
+// a stretch of many short items is no longer than one of few long ones.
 // Without a workspace a CTA does whole items: those that begin in its stretch.
 struct TreeRec {
     int s, g, rg;
@@ -116,11 +118,12 @@ struct TreeSeg {
     int slot;  // of the partial; -1: the item is whole
 };
 
-template <int KB, int ROWS>
+template <int KB, int ROWS, int EXTRA>
 struct TreeWalk {
     int64_t pos, end, base, us;  // this CTA's stretch; the current sequence's first unit and units
     int64_t per;                 // units of a stretch
     int s, nb, ng;               // the current sequence, its key blocks and groups per head
+                                 // (an item: EXTRA + nb units)
     TreeSeq w;
 
     __device__ __forceinline__ static int blocks(const TreeSeq& w) { return max(1, (w.L + KB - 1) / KB); }
@@ -128,7 +131,7 @@ struct TreeWalk {
         return (int)(((int64_t)w.n * a.G + ROWS - 1) / ROWS);
     }
     __device__ __forceinline__ static int64_t units(const TreeDev& a, const TreeSeq& w) {
-        return (int64_t)blocks(w) * groups(a, w) * a.Hkv;
+        return (int64_t)(EXTRA + blocks(w)) * groups(a, w) * a.Hkv;
     }
     __device__ __forceinline__ void enter(const TreeDev& a, int seq) {
         s = seq;
@@ -199,12 +202,15 @@ struct TreeWalk {
                 continue;
             }
             const int64_t rel = pos - base;
-            const int item = (int)(rel / nb), b0 = (int)(rel - (int64_t)item * nb);
-            if (!a.ws && b0 > 0) {  // an item of the CTA before
-                pos += nb - b0;
+            const int item = (int)(rel / (EXTRA + nb)), u0 = (int)(rel - (int64_t)item * (EXTRA + nb));
+            const int u1 = (int)min((int64_t)(EXTRA + nb), u0 + (end - pos));
+            if (!a.ws && u0 > 0) {  // an item of the CTA before
+                pos += EXTRA + nb - u0;
                 continue;
             }
-            const int b1 = a.ws ? (int)min((int64_t)nb, b0 + (end - pos)) : nb;
+            const int b0 = max(0, u0 - EXTRA), b1 = a.ws ? max(0, u1 - EXTRA) : nb;
+            pos += a.ws ? u1 - u0 : EXTRA + nb;
+            if (b1 == 0) continue;  // the item's keys are the next CTA's
             t.w = w;
             t.s = s;
             t.g = item / ng;
@@ -212,7 +218,6 @@ struct TreeWalk {
             t.k_begin = b0 * KB;
             t.k_end = min(w.L, b1 * KB);
             t.slot = b0 > 0 ? 0 : b1 < nb ? 1 : -1;
-            pos += b1 - b0;
             return true;
         }
         return false;
@@ -224,8 +229,8 @@ struct TreeWalk {
         TreeRec r{0, 0, 0, 0};
         if (pos < end && pos > base) {
             const int64_t rel = pos - base;
-            const int item = (int)(rel / nb), b0 = (int)(rel - (int64_t)item * nb);
-            const int64_t first = pos - b0;  // the item's first unit
+            const int item = (int)(rel / (EXTRA + nb)), b0 = (int)(rel - (int64_t)item * (EXTRA + nb)) - EXTRA;
+            const int64_t first = pos - b0;  // the unit of the item's first block
             if (b0 > 0 && first >= pos - per) {
                 r.s = s;
                 r.g = item / ng;
