@@ -138,9 +138,9 @@ __device__ __forceinline__ bool clean_rows(char* tile, int r0, int r1, int lane)
 
 // By one warp: a tile's codes, which landed in its second slab (a row's 128 codes are
 // as long as half a row of fp16), into the fp16 tile, in place: a row is read by
-// eight lanes before any of them writes.  Rows from nk on are zero.  Infinities and NaN
-// in rows from d0 on are set to zero; whether there were any.
-template <int FMT>
+// eight lanes before any of them writes.  EDGE: rows from nk on are zero, and
+// infinities and NaN in rows from d0 on are set to zero; whether there were any.
+template <int FMT, bool EDGE>
 __device__ __forceinline__ bool expand(char* tile, int nk, int d0, int lane) {
     const int c = lane & 7, r4 = lane >> 3;
     uint32_t odd = 0;
@@ -159,21 +159,25 @@ __device__ __forceinline__ bool expand(char* tile, int nk, int d0, int lane) {
             codes_to_f16<FMT>(raw[i].y, lo.z, lo.w);
             codes_to_f16<FMT>(raw[i].z, hi.x, hi.y);
             codes_to_f16<FMT>(raw[i].w, hi.z, hi.w);
-            if (r >= nk) lo = hi = make_uint4(0, 0, 0, 0);
-            if (FMT == QF_CACHE_E4M3 && r >= d0) {
-                odd |= odd_pair<__half>(lo.x) | odd_pair<__half>(lo.y) | odd_pair<__half>(lo.z) |
-                       odd_pair<__half>(lo.w) | odd_pair<__half>(hi.x) | odd_pair<__half>(hi.y) |
-                       odd_pair<__half>(hi.z) | odd_pair<__half>(hi.w);
-                zero_not_finite<__half>(lo);
-                zero_not_finite<__half>(hi);
+            if constexpr (EDGE) {
+                if (r >= nk) lo = hi = make_uint4(0, 0, 0, 0);
+                if (FMT == QF_CACHE_E4M3 && r >= d0) {
+                    odd |= odd_pair<__half>(lo.x) | odd_pair<__half>(lo.y) | odd_pair<__half>(lo.z) |
+                           odd_pair<__half>(lo.w) | odd_pair<__half>(hi.x) | odd_pair<__half>(hi.y) |
+                           odd_pair<__half>(hi.z) | odd_pair<__half>(hi.w);
+                    zero_not_finite<__half>(lo);
+                    zero_not_finite<__half>(hi);
+                }
             }
             // (lanes of the second slab the odd chunk first: eight lanes, eight bank groups)
-            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + (c >> 2))) = c >> 2 ? hi : lo;
-            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + 1 - (c >> 2))) = c >> 2 ? lo : hi;
+            const bool second = c >> 2;
+            const uint4 one = second ? hi : lo, two = second ? lo : hi;
+            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + (c >> 2))) = one;
+            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + 1 - (c >> 2))) = two;
         }
         __syncwarp();
     }
-    return __any_sync(kFull, odd != 0);
+    return EDGE && __any_sync(kFull, odd != 0);
 }
 
 // q . k over the 128 dims on the CUDA cores, k a cache row.
@@ -225,6 +229,13 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
         "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(block), "r"(smem_u32(bar))
         : "memory");
+}
+
+// 8 consecutive columns of this thread's lane.
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 
 // One lane of a converged warp, known as such to the assembler: the products'
@@ -360,8 +371,30 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 if (Q8 && side == 0 && in) {
                     ks[x] = __ldg(a.ks + srow);
                     vs[x] = __ldg(a.vs + srow);
-                    // a scale of 0 (a row never written) stands for zeros, as good as at 2^-120
-                    if (vs[x] < kLeastScale) vs[x] = kLeastScale;
+                }
+            }
+        };
+        // The same scales for a block whose pages are all there, in two steps with the work
+        // on another block between them: the keys' pages, then the scales.
+        int page[4];
+        auto look_scales = [&](int j) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int key = sg.k_begin + j * kRows + x * 32 + lane;
+                page[x] = key < sg.k_end ? __ldg(bt + a.B.div(key)) : -1;
+            }
+        };
+        auto load_scales = [&](int j) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int key = sg.k_begin + j * kRows + x * 32 + lane;
+                ks[x] = 0.f;
+                vs[x] = 1.f;
+                if (page[x] >= 0 && page[x] < a.N) {
+                    const int64_t srow = (int64_t)page[x] * a.s0 + (int64_t)sg.g * a.s1 +
+                                         (int64_t)(key - a.B.div(key) * a.B.d) * a.s2;
+                    ks[x] = __ldg(a.ks + srow);
+                    vs[x] = __ldg(a.vs + srow);
                 }
             }
         };
@@ -372,6 +405,10 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         auto inform = [&](int slot, bool first) {
             if (lane == 0) *reinterpret_cast<uint4*>(valid[slot]) = make_uint4(ok[0], ok[1], ok[2], ok[3]);
             if constexpr (Q8) {
+                // a scale of 0 (a row never written) stands for zeros, as good as at 2^-120
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (vs[x] < kLeastScale) vs[x] = kLeastScale;
                 if (first) {
                     float top = 0.f;
 #pragma unroll
@@ -419,7 +456,13 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             ++seq_no;
             bt = a.bt + (int64_t)sg.s * a.bts;
             const int nblk = blocks_of(), k_end = sg.k_end;
-            if (box > 0 && nblk > 0) look(0);
+            if (box > 0 && nblk > 0) {
+                look(0);
+                if (Q8 && side == 0) {
+                    look_scales(0);
+                    load_scales(0);
+                }
+            }
             for (int j = 0; j < nblk; ++j, ++n) {
                 const int st = n % ST, kb = sg.k_begin + j * kRows, nk = min(kRows, k_end - kb);
                 char* tile = tiles + st * kTile;
@@ -451,11 +494,11 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                     }
                     if (j + 1 < nblk) look(j + 1);
                     if (side == 0) {  // meanwhile, what the softmax needs to know
-                        if (Q8) locate(j);
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
                             ok[x] = nk >= 32 * (x + 1) ? kFull : nk > 32 * x ? (1u << (nk - 32 * x)) - 1u : 0u;
                         inform(n % C::SLOTS, j == 0);
+                        if (Q8 && j + 1 < nblk) look_scales(j + 1);
                     }
                     if (!work) continue;
                     if (!__all_sync(kFull, mbar_wait(bar, raw++ & 1, nullptr))) {
@@ -466,11 +509,14 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                         for (int r = nk + hi; r < kRows; r += 2)
                             *reinterpret_cast<uint4*>(tile + tile_off(r, c)) = make_uint4(0, 0, 0, 0);
                 } else if constexpr (Q8) {  // row by row, 16 codes a lane
-                    if (box > 0 && j + 1 < nblk) look(j + 1);
+                    if (box > 0 && j + 1 < nblk) {
+                        look(j + 1);
+                        if (side == 0) look_scales(j + 1);
+                    }
                     const uint32_t dst = smem_u32(tile) + (uint32_t)(kSlab + (lane >> 3) * 128 + (lane & 7) * 16);
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
-#pragma unroll
+#pragma unroll 1
                         for (int i = 0; i < 8; ++i) {
                             const int r = 4 * i + (lane >> 3);
                             const int64_t o = __shfl_sync(kFull, off[x], r);
@@ -487,7 +533,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                     const char* from = src + c * 16;
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-#pragma unroll
+#pragma unroll 4
                         for (int i = 0; i < 16; ++i) {
                             const int64_t o = __shfl_sync(kFull, off[x], 2 * i + hi);
                             cp_async16_at(dst + (uint32_t)((x * 32 + 2 * i) * 128 + (((c & 7) ^ ((2 * i & 7) + hi)) << 4)),
@@ -500,12 +546,14 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                     __syncwarp();
                 }
                 if constexpr (Q8) {
-                    if (expand<FMT>(tile, side == 1 ? nk : kRows, side == 1 ? d0 : kRows, lane)) odd_v = seq_no;
+                    if (side == 0 || (nk == kRows && d0 >= kRows)) expand<FMT, false>(tile, nk, d0, lane);
+                    else if (expand<FMT, true>(tile, nk, d0, lane)) odd_v = seq_no;
                 } else {
                     if (work && d0 < nk && clean_rows<MT>(tile, d0, nk, lane)) odd_v = seq_no;
                 }
                 proxy_fence();
                 mbar_arrive(&full[st]);
+                if (Q8 && side == 0 && box > 0 && j + 1 < nblk) load_scales(j + 1);
             }
         }
         // every copy issued has landed before the CTA can leave
@@ -674,21 +722,47 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 for (int q = 0; q < 4; ++q)
                     see[q] = live ? see[q] & tree_bits32(mrow, a.words, kb + 32 * q - w.ctx) : 0u;
             const bool masked = __any_sync(kFull, (see[0] & see[1] & see[2] & see[3]) != kFull);
-            // the two halves of a block one after the other: the first's products run during
-            // the second's softmax
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-            const int c0 = 64 * h;
-            const uint32_t sh = sS + (uint32_t)c0;
             bool near = true;
             if constexpr (Q8) {
                 near = snear[slot] != 0;
-                if (j == 0 && h == 0) unscale = __int_as_float((127 - sexp[slot]) << 23);
+                if (j == 0) unscale = __int_as_float((127 - sexp[slot]) << 23);
             }
+            // the two halves of a block one after the other: the first's products run during
+            // the second's softmax (not unrolled: the roles share the instruction cache)
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+            const int c0 = 64 * h;
+            const uint32_t sh = sS + (uint32_t)c0;
+            const uint32_t see2[2] = {h ? see[2] : see[0], h ? see[3] : see[1]};
+            // The reference moves: O and l with it.
+            auto follow = [&](bool move, float mx) {
+                const float corr = move ? ex2(m - mx) : 1.f;
+                if (j > 0 || h > 0) {
+                    // O is between two products: those of the block before were done before this
+                    // block's S, the first half's are waited for, this half's wait for P
+                    if (h == 1) {
+                        got = __all_sync(kFull, mbar_wait(&bars.pv_done[t], (uses + (uint32_t)j) & 1, abort));
+                        if (!got) return;
+                        tc_fence_after();
+                    }
+#pragma unroll 1
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t o[32];
+                        tmem_ld32(sO + 32 * q, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                        tmem_st32(sO + 32 * q, o);
+                    }
+                }
+                l *= corr;
+                if (move) m = mx;
+            };
+            if (!Q8 || near) {
             // One pass over S against the reference m, P in registers, the half block's maximum
             // on the side.  While no row's maximum has grown past 2^8 (but for the first blocks,
-            // nearly always) P stands; else the reference moves, O and l with it, and
-            // the pass is made again over S, which P has not touched yet.
+            // nearly always) P stands; else the reference moves, and the pass is made again over
+            // S, which P has not touched yet.
             uint32_t pk[32];
             float sum;
             for (int turn = 0;; ++turn) {
@@ -715,75 +789,78 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                     if (masked) {  // (an unseen key's score may be anything)
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (!((see[2 * h + q] >> e) & 1)) xs[e] = __float_as_uint(-INFINITY);
+                            if (!((see2[q] >> e) & 1)) xs[e] = __float_as_uint(-INFINITY);
                     }
-                    if (!Q8 || near) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            float p[4];
-                            // raw maxima: rs > 0 (a negative scale's sign is in Q)
-                            mx0 = max3(mx0, __uint_as_float(xs[e]), __uint_as_float(xs[e + 1]));
-                            mx1 = max3(mx1, __uint_as_float(xs[e + 2]), __uint_as_float(xs[e + 3]));
-                            fma2(p[0], p[1], __uint_as_float(xs[e]), __uint_as_float(xs[e + 1]), rs, -mref);
-                            fma2(p[2], p[3], __uint_as_float(xs[e + 2]), __uint_as_float(xs[e + 3]), rs, -mref);
+                    for (int e = 0; e < 32; e += 4) {
+                        float p[4];
+                        // raw maxima: rs > 0 (a negative scale's sign is in Q)
+                        mx0 = max3(mx0, __uint_as_float(xs[e]), __uint_as_float(xs[e + 1]));
+                        mx1 = max3(mx1, __uint_as_float(xs[e + 2]), __uint_as_float(xs[e + 3]));
+                        fma2(p[0], p[1], __uint_as_float(xs[e]), __uint_as_float(xs[e + 1]), rs, -mref);
+                        fma2(p[2], p[3], __uint_as_float(xs[e + 2]), __uint_as_float(xs[e + 3]), rs, -mref);
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) p[x] = ex2(p[x]);
-                            add2(s0, s1, p[0], p[1]);
-                            add2(s2, s3, p[2], p[3]);
-                            if constexpr (Q8) {
-                                const float4 v4 = *reinterpret_cast<const float4*>(&sv[slot][cq + e]);
-                                mul2(p[0], p[1], v4.x, v4.y);
-                                mul2(p[2], p[3], v4.z, v4.w);
-                            }
-                            pk[16 * q + (e >> 1)] = MP::pack(p[0], p[1]);
-                            pk[16 * q + (e >> 1) + 1] = MP::pack(p[2], p[3]);
+                        for (int y = 0; y < 4; ++y) p[y] = ex2(p[y]);
+                        add2(s0, s1, p[0], p[1]);
+                        add2(s2, s3, p[2], p[3]);
+                        if constexpr (Q8) {
+                            const float4 v4 = *reinterpret_cast<const float4*>(&sv[slot][cq + e]);
+                            mul2(p[0], p[1], v4.x, v4.y);
+                            mul2(p[2], p[3], v4.z, v4.w);
                         }
-                    } else {  // V's scales in the exponent
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            const float x0 = __uint_as_float(xs[e]), x1 = __uint_as_float(xs[e + 1]);
-                            const float2 l2 = *reinterpret_cast<const float2*>(&sl[slot][cq + e]);
-                            const float t0 = x0 * rs, t1 = x1 * rs;
-                            const float u0 = x0 == -INFINITY ? x0 : t0 + l2.x, u1 = x1 == -INFINITY ? x1 : t1 + l2.y;
-                            mx0 = max3(mx0, u0, u1);
-                            s0 += ex2(t0 - mref);
-                            s1 += ex2(t1 - mref);
-                            pk[16 * q + (e >> 1)] = MP::pack(ex2(u0 - mref), ex2(u1 - mref));
-                        }
+                        pk[16 * q + (e >> 1)] = MP::pack(p[0], p[1]);
+                        pk[16 * q + (e >> 1) + 1] = MP::pack(p[2], p[3]);
                     }
                     if (q == 0) tmem_wait_ld();
                 }
                 sum = (s0 + s1) + (s2 + s3);
-                const float mx = fmaxf(mx0, mx1) * (near ? rs : 1.f);
+                const float mx = fmaxf(mx0, mx1) * rs;
                 const bool move = turn == 0 && (mx > m + kKeepLog2 || (m == -INFINITY && mx > -INFINITY));
                 if (!__any_sync(kFull, move)) break;
-                const float corr = move ? ex2(m - mx) : 1.f;
-                if (j > 0 || h > 0) {
-                    // O is between two products: those of the block before were done before this
-                    // block's S, the first half's are waited for, this half's wait for P
-                    if (h == 1) {
-                        got = mbar_wait(&bars.pv_done[t], (uses + (uint32_t)j) & 1, abort);
-                        if (!__all_sync(kFull, got)) break;
-                        tc_fence_after();
-                    }
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t o[32];
-                        tmem_ld32(sO + 32 * q, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                        tmem_st32(sO + 32 * q, o);
-                    }
-                }
-                l *= corr;
-                if (move) m = mx;
+                follow(move, mx);
+                if (!got) break;
             }
-            got = __all_sync(kFull, got);
             if (!got) break;
 #pragma unroll
             for (int q = 0; q < 2; ++q) tmem_st16(sh + 16 * q, pk + 16 * q);
             l += sum;
+            } else if constexpr (Q8) {
+            // V's scales in the exponent, in two passes and small steps (such blocks are rare)
+            auto quarter = [&](int c, float mref, float* mx, float* sum, uint32_t* pk) {
+                uint32_t x[16];
+                tmem_ld16(sh + c, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    float u[2], p[2];
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int cc = c + e + y;
+                        const bool ok = ((c & 32 ? see2[1] : see2[0]) >> ((c & 31) + e + y)) & 1;
+                        const float tt = ok ? __uint_as_float(x[e + y]) * sk[slot][c0 + cc] * rs : -INFINITY;
+                        u[y] = ok ? tt + sl[slot][c0 + cc] : -INFINITY;
+                        *mx = fmaxf(*mx, u[y]);
+                        *sum += ex2(tt - mref);
+                        p[y] = ex2(u[y] - mref);
+                    }
+                    pk[e >> 1] = MP::pack(p[0], p[1]);
+                }
+            };
+            float mx = -INFINITY, sum = 0.f;
+            uint32_t pk[8];
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 16) quarter(c, 0.f, &mx, &sum, pk);
+            const bool move = mx > m + kKeepLog2 || (m == -INFINITY && mx > -INFINITY);
+            if (__any_sync(kFull, move)) follow(move, mx);
+            if (!got) break;
+            sum = 0.f;
+#pragma unroll 1
+            for (int c = 0; c < 64; c += 16) {
+                quarter(c, m == -INFINITY ? 0.f : m, &mx, &sum, pk);
+                tmem_st8(sh + c / 2, pk);  // over columns read already
+            }
+            l += sum;
+            }
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&bars.p_full[t][h]);
@@ -804,9 +881,9 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             // there, then the warp whole rows (partials: half rows of 64 floats) to memory
             const int hi = lane >> 4, c = lane & 15, w0 = (warp & 3) * 32;
             const int64_t to = !live ? -1 : whole ? trow_q * a.ot + (int64_t)hq * a.oh : 0;
-#pragma unroll
+#pragma unroll 1
             for (int half = 0; half < 2; ++half) {
-#pragma unroll
+#pragma unroll 1
                 for (int q = 0; q < 2; ++q) {
                     uint32_t o[32];
                     tmem_ld32(sO + 64 * half + 32 * q, o);
