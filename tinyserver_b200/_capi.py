@@ -8,6 +8,7 @@ fails, every op raises -- there is no CPU or torch fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -246,6 +247,13 @@ def check(rc: int, what: str) -> None:
         err = lib().qf_last_cuda_error().decode()
         raise RuntimeError(f"{what}: CUDA launch failed: {err}")
     raise RuntimeError(f"{what}: error code {rc}")
+
+
+@functools.lru_cache(maxsize=4096)
+def strides_array(strides: tuple) -> ctypes.Array:
+    """A tensor's strides as the C side reads them, made once per distinct tuple (the
+    library takes const pointers, so calls may share one)."""
+    return (c_i64 * len(strides))(*strides)
 
 
 def i64_array(vals) -> ctypes.Array:

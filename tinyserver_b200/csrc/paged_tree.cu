@@ -72,6 +72,8 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const TreeDev a) {
     __shared__ int64_t scratch[34];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wr = warp % WR, wk = warp / WR;
+    pdl_wait();
+    pdl_trigger();
     TreeWalk<kF32Keys, NR, 4> walk;
     walk.begin(a, scratch);
     zero_unowned_rows<float, D>(a);
@@ -246,8 +248,7 @@ int launch_f32(const TreeDev& a, int ctas, cudaStream_t stream) {
     constexpr int smem = F32Tile<FMT, D, WR>::FLOATS * 4;
     const int rc = allow_smem<kernel>(smem);
     if (rc) return rc;
-    kernel<<<(unsigned)ctas, 128, smem, stream>>>(a);
-    return check_launch();
+    return launch_pdl(kernel, dim3((unsigned)ctas), 128, (size_t)smem, stream, a);
 }
 
 template <int FMT, int D>
@@ -356,6 +357,8 @@ int launch_merge(const TreeDev& a, int D, int rows, int ctas, cudaStream_t strea
 __global__ void __launch_bounds__(128)
     build_tree_mask_kernel(const void* parents, int index_type, const int32_t* cu, int S, int T,
                            int max_tree, int words, int64_t* mask, int32_t* depths, int32_t* status) {
+    pdl_wait();
+    pdl_trigger();
     const int s = blockIdx.x;
     const int b = min(max(__ldg(cu + s), 0), T), e = min(max(__ldg(cu + s + 1), b), T);
     auto empty = [&](int t0, int t1) {
@@ -408,7 +411,8 @@ struct TreePlan {
 
 // The kernel and its grid, by sizes alone (lengths are on the device; the block
 // tables bound them).  A cut costs a partial of (D + 2) floats a row, written and
-// read back, so a CTA's stretch is at least two blocks of 128 keys, or four of 64.
+// read back, so a CTA's stretch is at least two blocks of 128 keys, or four of 64;
+// and a second launch, so sequences of up to 768 keys stay whole.
 TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     TreePlan p{};
     const int64_t G = g.num_q_heads / g.num_kv_heads, rows = (g.cu_seqlens_q ? g.max_tree : 1) * G;
@@ -432,7 +436,7 @@ TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     const int64_t blocks = ceil_div(cap, keys);  // of the longest sequence
     const int64_t items = g.num_seqs * g.num_kv_heads * ceil_div(rows, p.rows);
     const int64_t slots = (int64_t)sm_count() * per_sm;
-    p.split = blocks > p.min_units;
+    p.split = blocks > 3 * p.min_units;
     p.ctas = (int)(items >= slots ? slots : std::min(slots, items * blocks));
     return p;
 }
@@ -579,8 +583,7 @@ extern "C" int qf_build_tree_mask(const void* parents, int index_type, const int
     if (num_seqs > INT32_MAX || num_nodes > INT32_MAX || max_tree > INT32_MAX ||
         mask_words > INT32_MAX)
         return QF_ERR_UNSUPPORTED;
-    qf::build_tree_mask_kernel<<<(unsigned)num_seqs, 128, 0, stream>>>(
-        parents, index_type, cu_seqlens, (int)num_seqs, (int)num_nodes, (int)max_tree,
-        (int)mask_words, mask, depths, status);
-    return qf::check_launch();
+    return qf::launch_pdl(qf::build_tree_mask_kernel, dim3((unsigned)num_seqs), 128, 0, stream, parents,
+                          index_type, cu_seqlens, (int)num_seqs, (int)num_nodes, (int)max_tree,
+                          (int)mask_words, mask, depths, status);
 }

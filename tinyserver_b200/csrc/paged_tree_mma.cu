@@ -99,6 +99,8 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
     const float sl2 = a.scale * 1.4426950408889634f;
     unsigned char* ring = smem + warp * R::WARP;
 
+    pdl_wait();
+    pdl_trigger();
     TreeWalk<kMmaKeys, NR, 4> walk;
     walk.begin(a, scratch);
     zero_unowned_rows<T, D>(a);
@@ -474,8 +476,7 @@ int launch_nr(const TreeDev& a, int ctas, cudaStream_t stream) {
     constexpr auto kernel = tree_mma_kernel<T, FMT, D, NR>;
     const int rc = allow_smem<kernel>(MmaRing<FMT, D>::SMEM);
     if (rc) return rc;
-    kernel<<<(unsigned)ctas, 32 * kWarps, MmaRing<FMT, D>::SMEM, stream>>>(a);
-    return check_launch();
+    return launch_pdl(kernel, dim3((unsigned)ctas), 32 * kWarps, (size_t)MmaRing<FMT, D>::SMEM, stream, a);
 }
 
 template <typename T, int FMT>

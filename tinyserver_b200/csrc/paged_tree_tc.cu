@@ -332,6 +332,9 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     const uint32_t tmem = tmem_slot;
     const float sl2 = a.scale * 1.4426950408889634f;
 
+    // launched with programmatic dependent launch: what is above overlaps the kernel before
+    pdl_wait();
+    pdl_trigger();
     // every role walks the same segments; barrier phases run on across them
     TreeWalk<kRows, NT * kRows, kItemBlocks> walk;
     walk.begin(a, scratch);
@@ -984,8 +987,8 @@ int launch_nt(const TreeDev& a, int ctas, cudaStream_t stream) {
     CUtensorMap tk{}, tv{};
     int box = std::min(a.B.d & -a.B.d, kRows);
     if (box < (Q8 ? 4 : 8) || !page_map(&tk, a.kc, a, type, box) || !page_map(&tv, a.vc, a, type, box)) box = 0;
-    kernel<<<(unsigned)ctas, TreeTc<NT>::THREADS, TreeTc<NT>::SMEM, stream>>>(a, tk, tv, box);
-    return check_launch();
+    return launch_pdl(kernel, dim3((unsigned)ctas), TreeTc<NT>::THREADS, (size_t)TreeTc<NT>::SMEM, stream, a, tk, tv,
+                      box);
 }
 
 template <typename T, int FMT>

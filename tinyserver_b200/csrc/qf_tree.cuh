@@ -147,24 +147,11 @@ struct TreeWalk {
     __device__ void begin(const TreeDev& a, int64_t* scratch) {
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
         const int nt = nw * 32;
-        int64_t mine = 0;
-        for (int i = tid; i < a.S; i += nt) mine += units(a, tree_seq(a, i, blockIdx.x == 0));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        if (lane == 0) scratch[warp] = mine;
-        __syncthreads();
-        int64_t total = 0;
-        for (int i = 0; i < nw; ++i) total += scratch[i];
-        per = max((int64_t)a.min_units, (total + gridDim.x - 1) / gridDim.x);
-        pos = min(total, per * blockIdx.x);
-        end = min(total, pos + per);
-        __syncthreads();
-        // the sequence with base <= pos < base + us, by scans of nt sequences
-        if (tid == 0) scratch[32] = -1;
-        int64_t before = 0;
-        for (int i0 = 0; i0 < a.S; i0 += nt) {
+        int64_t before = 0, u = 0, first = 0, total = 0;
+        // first: the units before sequence i0 + tid; all: of sequences [i0, i0 + nt)
+        auto scan = [&](int i0, bool report) -> int64_t {
             const int i = i0 + tid;
-            const int64_t u = i < a.S ? units(a, tree_seq(a, i, false)) : 0;
+            u = i < a.S ? units(a, tree_seq(a, i, report)) : 0;
             int64_t incl = u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -178,15 +165,24 @@ struct TreeWalk {
                 if (x < warp) warps += scratch[x];
                 all += scratch[x];
             }
-            const int64_t first = before + warps + incl - u;
+            __syncthreads();
+            first = before + warps + incl - u;
+            return all;
+        };
+        for (int i0 = 0; i0 < a.S; i0 += nt) total += scan(i0, blockIdx.x == 0);
+        per = max((int64_t)a.min_units, (total + gridDim.x - 1) / gridDim.x);
+        pos = min(total, per * blockIdx.x);
+        end = min(total, pos + per);
+        // the sequence with base <= pos < base + us (with up to nt sequences, scanned already)
+        for (int i0 = 0; i0 < a.S && before <= pos; i0 += nt) {
+            const int64_t all = a.S <= nt ? total : scan(i0, false);
             if (first <= pos && pos < first + u) {
-                scratch[32] = i;
+                scratch[32] = i0 + tid;
                 scratch[33] = first;
             }
             before += all;
-            __syncthreads();
-            if (before > pos) break;
         }
+        __syncthreads();
         if (pos < end) {
             base = scratch[33];
             enter(a, (int)scratch[32]);

@@ -36,7 +36,11 @@ def _mappings(what: str, block_mapping: torch.Tensor, slot_mapping: torch.Tensor
     index_tag(slot_mapping, f"{what} slot_mapping")
     if slot_mapping.dtype != block_mapping.dtype:
         slot_mapping = slot_mapping.to(block_mapping.dtype)
-    return block_mapping.contiguous(), slot_mapping.contiguous(), itag
+    if not block_mapping.is_contiguous():
+        block_mapping = block_mapping.contiguous()
+    if not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.contiguous()
+    return block_mapping, slot_mapping, itag
 
 
 def store_kv_cache_quantized(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: torch.Tensor,
@@ -67,7 +71,7 @@ def store_kv_cache_quantized(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: 
         raise ValueError(f"{what}: {bm.numel()} places for {T} tokens")
     tag = dtype_tag(k_src, what)
     dev = require_cuda(what, k_src, v_src, k_cache, v_cache, k_scale, v_scale, bm, sm)
-    i64 = _capi.i64_array
+    i64 = _capi.strides_array
     with on_device(dev):
         rc = _capi.lib().qf_kv_store_quantized(
             k_src.data_ptr(), i64(k_src.stride()), v_src.data_ptr(), i64(v_src.stride()),
@@ -95,10 +99,9 @@ def load_kv_cache_quantized(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scal
     N, H, B, D = k_cache.shape
     T = bm.numel()
     dev = require_cuda(what, k_cache, v_cache, k_scale, v_scale, bm, sm)
-    k = torch.empty((T, H, D), dtype=dtype, device=dev).transpose(0, 1)
-    v = torch.empty((T, H, D), dtype=dtype, device=dev).transpose(0, 1)
+    k, v = torch.empty((2, T, H, D), dtype=dtype, device=dev).transpose(1, 2).unbind(0)
     tag = dtype_tag(k, what)
-    i64 = _capi.i64_array
+    i64 = _capi.strides_array
     rows = i64((D, H * D, 1))
     with on_device(dev):
         rc = _capi.lib().qf_kv_load_quantized(

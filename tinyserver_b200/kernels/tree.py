@@ -18,6 +18,7 @@ The reference has no counterpart: it decodes one token per sequence and step.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -29,6 +30,13 @@ from .._runtime import (after_op, dtype_tag, index_tag, on_device, require_cuda,
 __all__ = ["build_tree_mask", "paged_tree_attention", "paged_tree_attention_workspace_bytes"]
 
 CACHE_FORMATS = {torch.float8_e4m3fn: _capi.QF_CACHE_E4M3, torch.int8: _capi.QF_CACHE_INT8}
+
+
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as contiguous int32, itself where it is that already."""
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def build_tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -56,8 +64,9 @@ def build_tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor,
     itag = index_tag(parents, "build_tree_mask parents")
     index_tag(cu_seqlens, "build_tree_mask cu_seqlens")
     dev = require_cuda("build_tree_mask", parents, cu_seqlens)
-    parents = parents.contiguous()
-    cu = cu_seqlens.to(torch.int32).contiguous()
+    if not parents.is_contiguous():
+        parents = parents.contiguous()
+    cu = _int32(cu_seqlens)
     n, words = parents.numel(), (max_tree + 63) // 64
     if n and cu.numel() < 2:
         raise ValueError(f"build_tree_mask: {n} nodes but no sequence")
@@ -72,20 +81,32 @@ def build_tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor,
     return mask, depths
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(num_tokens: int, num_seqs: int, max_tree: int, num_q_heads: int,
+                     num_kv_heads: int, head_dim: int, block_size: int, max_blocks_per_seq: int,
+                     tag: int, fmt: int, decode: bool) -> int:
+    a = _capi.PagedTreeAttentionArgs()
+    a.cu_seqlens_q = None if decode else 1  # (whether there is one is all that is read)
+    a.num_tokens, a.num_seqs, a.max_tree = num_tokens, num_seqs, max_tree
+    a.num_q_heads, a.num_kv_heads, a.head_dim = num_q_heads, num_kv_heads, head_dim
+    a.block_size, a.max_blocks_per_seq = block_size, max_blocks_per_seq
+    a.dtype, a.cache_format = tag, fmt
+    return int(_capi.lib().qf_paged_tree_attention_workspace_bytes(a))
+
+
 def paged_tree_attention_workspace_bytes(num_tokens: int, num_seqs: int, max_tree: int,
                                          num_q_heads: int, num_kv_heads: int, head_dim: int,
                                          block_size: int, max_blocks_per_seq: int,
                                          dtype: torch.dtype) -> int:
     """Bytes of fp32 scratch that let :func:`paged_tree_attention` split long
-    sequences over several CTAs (0 when nothing needs splitting); a decode call
-    (:func:`~tinyserver_b200.paged_attention_quantized`) counts as max_tree 1."""
-    a = _capi.PagedTreeAttentionArgs()
-    a.cu_seqlens_q = 1  # any address: only whether it is one is read
-    a.num_tokens, a.num_seqs, a.max_tree = num_tokens, num_seqs, max_tree
-    a.num_q_heads, a.num_kv_heads, a.head_dim = num_q_heads, num_kv_heads, head_dim
-    a.block_size, a.max_blocks_per_seq = block_size, max_blocks_per_seq
-    a.dtype = dtype_tag(torch.empty(0, dtype=dtype), "paged_tree_attention_workspace_bytes")
-    return int(_capi.lib().qf_paged_tree_attention_workspace_bytes(a))
+    sequences over several CTAs (0 when nothing needs splitting), for a cache of any
+    format; a decode call (:func:`~tinyserver_b200.paged_attention_quantized`) counts
+    as max_tree 1.  It depends on the GPU: ask with the call's device current."""
+    tag = dtype_tag(torch.empty(0, dtype=dtype), "paged_tree_attention_workspace_bytes")
+    sizes = (num_tokens, num_seqs, max_tree, num_q_heads, num_kv_heads, head_dim, block_size,
+             max_blocks_per_seq, tag)
+    return max(_workspace_bytes(*sizes, fmt, decode) for decode in {False, max_tree == 1}
+               for fmt in (_capi.QF_CACHE_PLAIN, *CACHE_FORMATS.values()))
 
 
 def check_quantized_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -157,34 +178,36 @@ def attend(what: str, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
     if bt.shape[1] > 1 and bt.stride(1) != 1:
         bt = bt.contiguous()
-    lens = lens.to(torch.int32).contiguous()
+    lens = _int32(lens)
     out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    a = _capi.PagedTreeAttentionArgs()
-    a.q, a.q_stride_token, a.q_stride_head = q.data_ptr(), sq[0], sq[1]
-    a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-    a.cache_strides[:] = strides
-    if k_scale is not None:
-        a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-        a.scale_strides[:] = k_scale.stride()
-    a.num_blocks, a.block_size = N, B
-    a.block_tables, a.block_tables_row_stride = bt.data_ptr(), bt.stride(0)
-    a.max_blocks_per_seq = bt.shape[1]
-    a.context_lens = lens.data_ptr()
+    cu = mask = None
     if cu_seqlens is not None:
-        cu = cu_seqlens.to(torch.int32).contiguous()
-        mask = tree_mask.contiguous()
-        a.cu_seqlens_q, a.tree_mask, a.mask_words = cu.data_ptr(), mask.data_ptr(), mask.shape[1]
-    a.num_seqs, a.num_tokens, a.max_tree = S, T, max_tree
-    a.num_q_heads, a.num_kv_heads, a.head_dim = Hq, Hkv, D
-    a.scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
-    a.out, a.out_stride_token, a.out_stride_head = out.data_ptr(), Hq * D, D
-    a.dtype, a.cache_format = tag, fmt
-    a.status = status_word(dev).data_ptr()
+        cu = _int32(cu_seqlens)
+        mask = tree_mask if tree_mask.is_contiguous() else tree_mask.contiguous()
+    arr = _capi.strides_array
+    scaled = k_scale is not None
+    # positional, in the struct's order: a third of the time of 40 assignments
+    a = _capi.PagedTreeAttentionArgs(
+        q.data_ptr(), sq[0], sq[1],
+        k_cache.data_ptr(), v_cache.data_ptr(), arr(strides),
+        k_scale.data_ptr() if scaled else None, v_scale.data_ptr() if scaled else None,
+        arr(k_scale.stride() if scaled else (0, 0, 0)),
+        N, B,
+        bt.data_ptr(), bt.stride(0), bt.shape[1],
+        lens.data_ptr(), cu.data_ptr() if cu is not None else None,
+        mask.data_ptr() if mask is not None else None, mask.shape[1] if mask is not None else 0,
+        S, T, max_tree, Hq, Hkv, D,
+        1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale),
+        out.data_ptr(), Hq * D, D,
+        None, 0,
+        tag, fmt,
+        status_word(dev).data_ptr())
     lib = _capi.lib()
     with on_device(dev):
         if split:
             if workspace is None:
-                need = lib.qf_paged_tree_attention_workspace_bytes(a)
+                need = _workspace_bytes(T, S, max_tree, Hq, Hkv, D, B, bt.shape[1], tag, fmt,
+                                        cu is None)
                 if need:
                     workspace = torch.empty(need // 4, dtype=torch.float32, device=dev)
             if workspace is not None:
