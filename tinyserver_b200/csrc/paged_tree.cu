@@ -412,7 +412,7 @@ struct TreePlan {
 // The kernel and its grid, by sizes alone (lengths are on the device; the block
 // tables bound them).  A cut costs a partial of (D + 2) floats a row, written and
 // read back, so a CTA's stretch is at least two blocks of 128 keys, or four of 64;
-// and a second launch, so sequences of up to 768 keys stay whole.
+// and a second launch, so sequences of up to 768 keys (256 of the mma.sync kernel's) stay whole.
 TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     TreePlan p{};
     const int64_t G = g.num_q_heads / g.num_kv_heads, rows = (g.cu_seqlens_q ? g.max_tree : 1) * G;
@@ -436,7 +436,7 @@ TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     const int64_t blocks = ceil_div(cap, keys);  // of the longest sequence
     const int64_t items = g.num_seqs * g.num_kv_heads * ceil_div(rows, p.rows);
     const int64_t slots = (int64_t)sm_count() * per_sm;
-    p.split = blocks > 3 * p.min_units;
+    p.split = blocks > (keys == 128 ? 6 : 4);
     p.ctas = (int)(items >= slots ? slots : std::min(slots, items * blocks));
     return p;
 }

@@ -25,7 +25,9 @@
 // definition.  Queries become fp16 after a power-of-two row factor that puts
 // their largest element in [2^14, 2^15): exact for every element within 2^-28 of it.
 // P goes in as a 16-bit high part and the rounded remainder, so the product
-// keeps 16 significant bits or more of p; sums and maxima are fp32.
+// keeps 16 significant bits or more of p; over codes and for bf16 outputs fp16's 11
+// bits, an eighth of the output's own rounding, are enough and the remainder is left
+// out.  Sums and maxima are fp32.
 #include <math.h>
 
 #include "qf_mma.cuh"
@@ -41,6 +43,12 @@ constexpr unsigned kAll = 0xffffffffu;
 __device__ __forceinline__ float pow2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float log2_of(float x) {  // of a normal number
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -62,7 +70,7 @@ struct MmaRing {
     static constexpr int NCH = ROW / 16;              // 16-byte chunks per row
     static constexpr int MAT = 16 * ROW;              // one tile of K or V
     static constexpr int STAGE = 2 * MAT + 128 + 16;  // K, V, 16 + 16 scales, valid bits
-    static constexpr int STAGES = MAT <= 2048 ? 4 : 3;
+    static constexpr int STAGES = MAT <= 1024 ? 4 : 3;
     static constexpr int WARP = STAGE * STAGES;
     static constexpr int SMEM = kWarps * WARP;
     // Byte offset of 16-byte chunk c of row r: the rows that a quarter of a warp
@@ -76,9 +84,23 @@ struct MmaRing {
 
 constexpr int kMmaKeys = 16 * kWarps;  // keys of a work unit
 
+// CTAs per SM: by the registers that a kernel needs (16 rows' accumulators, wide
+// heads and 16-bit fragments take more) and the rings' shared memory.
+constexpr int mma_ctas(bool plain, int D, int rows) {
+    return D == 256 ? (plain ? 1 : 2) : D == 128 ? (plain || rows == 16 ? 2 : 4) : plain ? 3 : 4;
+}
+static_assert(mma_ctas(true, 256, 8) * (MmaRing<QF_CACHE_PLAIN, 256>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(false, 256, 8) * (MmaRing<QF_CACHE_E4M3, 256>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(true, 128, 8) * (MmaRing<QF_CACHE_PLAIN, 128>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(false, 128, 8) * (MmaRing<QF_CACHE_E4M3, 128>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(true, 64, 8) * (MmaRing<QF_CACHE_PLAIN, 64>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(false, 64, 8) * (MmaRing<QF_CACHE_E4M3, 64>::SMEM + 2048) <= 233472,
+              "the rings of an SM's CTAs");
+
 template <typename T, int FMT, int D, int NR>
-__global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) {
+__global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D, NR)) tree_mma_kernel(const TreeDev a) {
     constexpr bool Q8 = FMT != QF_CACHE_PLAIN;
+    constexpr bool LO = !Q8 || std::is_same<T, __half>::value;  // P's remainder goes in too
     using MT = typename std::conditional<Q8, __half, T>::type;  // the products' operand type
     using MP = Packed<MT>;
     using R = MmaRing<FMT, D>;
@@ -106,6 +128,11 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
     zero_unowned_rows<T, D>(a);
     if (tid == 0) walk.record(a);
 
+    // a lane's first chunk of a tile within one page, and the way to its next
+    const bool one_page = a.B.d % 16 == 0;
+    const int64_t lane_off = (int64_t)(lane / R::NCH) * a.c2 * EB + (lane % R::NCH) * 16;
+    const int64_t row_step = (int64_t)(32 / R::NCH) * a.c2 * EB;
+
     TreeSeg sg;
     while (walk.next(a, sg)) {
         const TreeSeq& w = sg.w;
@@ -113,7 +140,8 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
         const int32_t* bt = a.bt + (int64_t)sg.s * a.bts;
         const int ntiles = (sg.k_end - sg.k_begin + 15) / 16;  // (0: no key at all)
 
-        // copies of tile i (of this warp: 4 i + warp) into its stage; one group each
+        // copies of tile i (of this warp: 4 i + warp) into its stage; one group each.  Where
+        // pages are multiples of 16 slots a tile lies in one, and its rows are c2 apart.
         int ahead_blk = 0;  // the block of this lane's key of the tile issued next
         auto look = [&](int i) {
             const int j = sg.k_begin + (i * kWarps + warp) * 16 + (lane & 15);
@@ -128,17 +156,23 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
                 ok = false;
             }
             const int slot = j - a.B.div(j) * a.B.d;
-            int64_t row = 0, srow = 0;
-            if (ok) {
-                row = (blk * a.c0 + (int64_t)g * a.c1 + (int64_t)slot * a.c2) * EB;
-                srow = blk * a.s0 + (int64_t)g * a.s1 + (int64_t)slot * a.s2;
-            }
+            const int64_t row = ok ? (blk * a.c0 + (int64_t)g * a.c1 + (int64_t)slot * a.c2) * EB : 0;
+            const int64_t srow = Q8 && ok ? blk * a.s0 + (int64_t)g * a.s1 + (int64_t)slot * a.s2 : 0;
             look(i + 1);
             const unsigned valid = __ballot_sync(kAll, ok) & 0xffffu;
             unsigned char* kt = ring + (i % ST) * R::STAGE;
             unsigned char* vt = kt + R::MAT;
-            if (valid) {
+            if (valid == 0xffffu && one_page) {
+                const int64_t first = __shfl_sync(kAll, row, 0) + lane_off;
 #pragma unroll
+                for (int x = 0; x < R::NCH / 2; ++x) {
+                    const int r = (x * 32 + lane) / R::NCH, c = (x * 32 + lane) % R::NCH;
+                    const int64_t o = first + x * row_step;
+                    cp_async16(kt + R::off(r, c), a.kc + o, 16);
+                    cp_async16(vt + R::off(r, c), a.vc + o, 16);
+                }
+            } else if (valid) {
+#pragma unroll 2
                 for (int x = 0; x < R::NCH / 2; ++x) {
                     const int idx = x * 32 + lane, r = idx / R::NCH, c = idx % R::NCH;
                     const int64_t o = __shfl_sync(kAll, row, r);
@@ -146,15 +180,13 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
                     cp_async16(kt + R::off(r, c), a.kc + o + c * 16, bytes);
                     cp_async16(vt + R::off(r, c), a.vc + o + c * 16, bytes);
                 }
-                if (Q8 && ok)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(
-                                     __cvta_generic_to_shared(kt + 2 * R::MAT + lane * 4))),
-                                 "l"((lane < 16 ? a.ks : a.vs) + srow)
-                                 : "memory");
-                if (lane == 0) *reinterpret_cast<unsigned*>(kt + 2 * R::MAT + 128) = valid;
-            } else if (lane == 0) {
-                *reinterpret_cast<unsigned*>(kt + 2 * R::MAT + 128) = 0u;
             }
+            if (Q8 && ok)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(
+                                 __cvta_generic_to_shared(kt + 2 * R::MAT + lane * 4))),
+                             "l"((lane < 16 ? a.ks : a.vs) + srow)
+                             : "memory");
+            if (lane == 0) *reinterpret_cast<unsigned*>(kt + 2 * R::MAT + 128) = valid;
             cp_async_commit();
         };
         look(0);
@@ -262,8 +294,8 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
                         const float2 v2 = *reinterpret_cast<const float2*>(sp + 16 + 8 * n + 2 * tig);
                         ksv[n][0] = k2.x, ksv[n][1] = k2.y;
                         // a scale of 0 (a row never written) stands for zeros, as good as at 2^-120
-                        lvv[n][0] = __log2f(v2.x < kLeastScale ? kLeastScale : v2.x);
-                        lvv[n][1] = __log2f(v2.y < kLeastScale ? kLeastScale : v2.y);
+                        lvv[n][0] = log2_of(v2.x < kLeastScale ? kLeastScale : v2.x);
+                        lvv[n][1] = log2_of(v2.y < kLeastScale ? kLeastScale : v2.y);
                     }
                 }
                 float pw[NRT][2][2];
@@ -305,7 +337,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
                         ph[nt][n] = MP::pack(pw[nt][n][0], pw[nt][n][1]);
-                        pl[nt][n] = MP::pack(pw[nt][n][0] - MP::lo(ph[nt][n]), pw[nt][n][1] - MP::hi(ph[nt][n]));
+                        if (LO) pl[nt][n] = MP::pack(pw[nt][n][0] - MP::lo(ph[nt][n]), pw[nt][n][1] - MP::hi(ph[nt][n]));
                     }
                 }
                 if (__any_sync(kAll, moved)) {
@@ -410,7 +442,7 @@ __global__ void __launch_bounds__(32 * kWarps) tree_mma_kernel(const TreeDev a) 
 #pragma unroll
                                 for (int nt = 0; nt < NRT; ++nt) {
                                     Mma<MT>::run(acc[nt][y], va, ph[nt][0], ph[nt][1]);
-                                    Mma<MT>::run(acc[nt][y], va, pl[nt][0], pl[nt][1]);
+                                    if (LO) Mma<MT>::run(acc[nt][y], va, pl[nt][0], pl[nt][1]);
                                 }
                             }
                         }
@@ -502,16 +534,7 @@ int launch_fmt(const TreeDev& a, int format, int D, int rows, int ctas, cudaStre
 
 }  // namespace
 
-// CTAs that fit on an SM: by the rings' shared memory, and by the registers,
-// which 16 rows' accumulators take more of.
-int tree_mma_ctas_per_sm(bool plain, int D, int rows) {
-    const int smem = plain ? (D == 64 ? MmaRing<QF_CACHE_PLAIN, 64>::SMEM
-                                      : D == 128 ? MmaRing<QF_CACHE_PLAIN, 128>::SMEM : MmaRing<QF_CACHE_PLAIN, 256>::SMEM)
-                           : (D == 64 ? MmaRing<QF_CACHE_E4M3, 64>::SMEM
-                                      : D == 128 ? MmaRing<QF_CACHE_E4M3, 128>::SMEM : MmaRing<QF_CACHE_E4M3, 256>::SMEM);
-    const int by_regs = D == 256 ? 2 : (D == 64 ? 4 : 3) - (rows == 16);
-    return std::max(1, std::min(by_regs, 232448 / (smem + 2048)));
-}
+int tree_mma_ctas_per_sm(bool plain, int D, int rows) { return mma_ctas(plain, D, rows); }
 
 int launch_tree_mma(const TreeDev& a, int dtype, int format, int D, int rows, int ctas,
                     cudaStream_t stream) {

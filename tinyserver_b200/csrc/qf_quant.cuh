@@ -27,23 +27,16 @@ __device__ __forceinline__ float code_top() {
     return FMT == QF_CACHE_E4M3 ? 448.f : 127.f;
 }
 
-// Two e4m3 codes (the low 16 bits of `w`) as two fp16 values: exact.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
-    uint32_t d;
-    asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}"
-        : "=r"(d)
-        : "r"(w));
-    return d;
-}
-
 // Four codes (a 32-bit word) as two fp16x2 registers, exact: {c0, c1}, {c2, c3}.
 // int8: the byte c + 128 under the high byte 0x64 is the fp16 number
 // 1024 + (c + 128); subtracting 1152 leaves c.
 template <int FMT>
 __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
     if constexpr (FMT == QF_CACHE_E4M3) {
-        lo = e4m3x2_to_f16x2(w);
-        hi = e4m3x2_to_f16x2(w >> 16);
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
     } else {
         const uint32_t u = w ^ 0x80808080u;
         lo = Packed<__half>::sub(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u);
