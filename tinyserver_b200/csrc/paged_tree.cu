@@ -268,75 +268,78 @@ int launch_f32(const TreeDev& a, int D, int rows, int ctas, cudaStream_t stream)
 // ---------------------------------------------------------------------------
 // Join the partials of the items that a CTA began and later ones went on with:
 // blockIdx.x + 1 is the item's second CTA, whose record has it.  WPR warps per row
-// share its partials (acc[D], reference in log2 units, sum), eight each in flight.
+// share its partials (acc[D], reference in log2 units, sum), eight each in flight: 8
+// warps for the few rows of a decode step, whose long sequences leave a partial in
+// every CTA, one for the many rows of a tree, which few CTAs share.
 template <typename T, int D, int WPR>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeDev a, int rows_per_item) {
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeDev a, int rows_per_item) {
+    constexpr int RPC = 8 / WPR, PER = D / 32;  // rows per CTA, columns per lane
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t ctas = gridDim.x + 1, cta = blockIdx.x + 1;
     const TreeRec rec = reinterpret_cast<const TreeRec*>(a.ws)[cta];
-    if (rec.last == 0) return;
-    const TreeSeq w = tree_seq(a, rec.s, false);
-    const int ri = blockIdx.y * (4 / WPR) + warp / WPR, sub = warp % WPR;
-    const int r = rec.rg * rows_per_item + ri;
-    const bool live = r < w.n * a.G;
-    if (WPR == 4 && !live) return;  // (the whole CTA)
-    constexpr int PER = D / 32;
-    float Ls = 0.f, acc[PER];
+    const int ri = blockIdx.y * RPC + warp / WPR, sub = warp % WPR, r = rec.r0 + ri;
+    if (rec.last == 0 || rec.r0 + (int)blockIdx.y * RPC >= rec.rows) return;  // (the whole CTA)
+    const int n = r < rec.rows ? rec.last - (int)cta + 2 : 0;
+    auto partial = [&](int p) -> const float* {
+        return tree_partial(a, ctas, cta - 1 + p, p == 0 ? 1 : 0, rows_per_item, ri, D);
+    };
+    // this warp's partials against their own largest reference
+    float M = -INFINITY, Ls = 0.f, acc[PER];
 #pragma unroll
     for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    if (live) {
-        const int n = rec.last - (int)cta + 2;
-        auto partial = [&](int p) -> const float* {
-            return tree_partial(a, ctas, cta - 1 + p, p == 0 ? 1 : 0, rows_per_item, ri, D);
-        };
-        float M = -INFINITY;
-        for (int p = lane; p < n; p += 32) M = fmaxf(M, partial(p)[D]);
-        M = warp_max(M);
+    for (int p = sub + WPR * lane; p < n; p += WPR * 32) M = fmaxf(M, partial(p)[D]);
+    M = warp_max(M);
+    const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll 8
-        for (int p = sub; p < n; p += WPR) {
-            const float* wp = partial(p);
-            const float2 ml = *reinterpret_cast<const float2*>(wp + D);
-            const float f = M == -INFINITY ? 0.f : exp2f(ml.x - M);
-            Ls += ml.y * f;
+    for (int p = sub; p < n; p += WPR) {
+        const float* wp = partial(p);
+        const float2 ml = *reinterpret_cast<const float2*>(wp + D);
+        const float f = exp2f(ml.x - base);
+        Ls += ml.y * f;
 #pragma unroll
-            for (int e = 0; e < PER; e += 2) {
-                const float2 v = *reinterpret_cast<const float2*>(wp + e * 32 + lane * 2);
-                acc[e] += v.x * f;
-                acc[e + 1] += v.y * f;
-            }
+        for (int e = 0; e < PER; e += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(wp + e * 32 + lane * 2);
+            acc[e] += v.x * f;
+            acc[e + 1] += v.y * f;
         }
     }
-    const int tok = r / a.G;
-    T* o = reinterpret_cast<T*>(a.out) + (int64_t)(w.q0 + tok) * a.ot +
+    __shared__ __align__(8) float part[8][D];
+    __shared__ float tops[8], sums[8];
+#pragma unroll
+    for (int e = 0; e < PER; e += 2)
+        *reinterpret_cast<float2*>(&part[warp][e * 32 + lane * 2]) = make_float2(acc[e], acc[e + 1]);
+    if (lane == 0) tops[warp] = M, sums[warp] = Ls;
+    if (WPR > 1) __syncthreads();
+    else __syncwarp();
+    if (n == 0) return;
+    // the row's warps share its columns
+    const int w0 = warp - sub, tok = r / a.G;
+    T* o = reinterpret_cast<T*>(a.out) + (int64_t)(rec.q0 + tok) * a.ot +
            (int64_t)(rec.g * a.G + r - tok * a.G) * a.oh;
-    if constexpr (WPR == 1) {
-        if (!live) return;
+    float top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < PER; ++e)
-            o[(e & ~1) * 32 + lane * 2 + (e & 1)] = Dt<T>::from_f(Ls == 0.f ? 0.f : acc[e] / Ls);
-    } else {
-        __shared__ __align__(8) float part[4][D];
-        __shared__ float sums[4];
+    for (int k = 0; k < WPR; ++k) top = fmaxf(top, tops[w0 + k]);
+    float f[WPR], total = 0.f;
 #pragma unroll
-        for (int e = 0; e < PER; e += 2)
-            *reinterpret_cast<float2*>(&part[warp][e * 32 + lane * 2]) = make_float2(acc[e], acc[e + 1]);
-        if (lane == 0) sums[warp] = Ls;
-        __syncthreads();
-        const float total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-        for (int d = threadIdx.x; d < D; d += 128) {
-            const float A = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
-            o[d] = Dt<T>::from_f(total == 0.f ? 0.f : A / total);
-        }
+    for (int k = 0; k < WPR; ++k) {
+        f[k] = top == -INFINITY ? 0.f : exp2f(tops[w0 + k] - top);
+        total += sums[w0 + k] * f[k];
+    }
+    for (int d = sub * 32 + lane; d < D; d += WPR * 32) {
+        float A = 0.f;
+#pragma unroll
+        for (int k = 0; k < WPR; ++k) A += part[w0 + k][d] * f[k];
+        o[d] = Dt<T>::from_f(total == 0.f ? 0.f : A / total);
     }
 }
 
 template <typename T, int D>
 int launch_merge(const TreeDev& a, int rows, int ctas, cudaStream_t stream) {
     if (rows <= 16)
-        return launch_pdl(tree_merge_kernel<T, D, 4>, dim3((unsigned)ctas - 1, (unsigned)rows), 128, 0, stream, a,
+        return launch_pdl(tree_merge_kernel<T, D, 8>, dim3((unsigned)ctas - 1, (unsigned)rows), 256, 0, stream, a,
                           rows);
-    return launch_pdl(tree_merge_kernel<T, D, 1>, dim3((unsigned)ctas - 1, (unsigned)rows / 4), 128, 0, stream, a,
+    return launch_pdl(tree_merge_kernel<T, D, 1>, dim3((unsigned)ctas - 1, (unsigned)rows / 8), 256, 0, stream, a,
                       rows);
 }
 

@@ -100,12 +100,15 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeDev& a, int s, bool report
 // a stretch of many short items is no longer than one of few long ones.
 // Without a workspace a CTA does whole items: those that begin in its stretch.
 struct TreeRec {
-    int s, g, rg;
-    int last;  // the last CTA of slot 0's item; 0 unless the CTA before this one began it
+    int last;     // the last CTA of slot 0's item; 0 unless the CTA before this one began it
+    int q0;       // the item's sequence's first query token
+    int g;        // its kv head
+    int r0, rows;  // its first row, and the sequence's rows per kv head
+    int unused[3];
 };
 
 struct TreeWs {  // workspace: records, then [CTA][2][ROWS][D + 2] floats: acc, reference, sum
-    __host__ __device__ static int64_t rec_floats(int64_t ctas) { return (ctas * 4 + 63) / 64 * 64; }
+    __host__ __device__ static int64_t rec_floats(int64_t ctas) { return (ctas * 8 + 63) / 64 * 64; }
     __host__ __device__ static int64_t floats(int64_t ctas, int64_t rows, int64_t d) {
         return rec_floats(ctas) + ctas * 2 * rows * (d + 2);
     }
@@ -222,15 +225,16 @@ struct TreeWalk {
     // By one thread, before the walk: the record of this CTA.
     __device__ __forceinline__ void record(const TreeDev& a) const {
         if (!a.ws) return;
-        TreeRec r{0, 0, 0, 0};
+        TreeRec r{};
         if (pos < end && pos > base) {
             const int64_t rel = pos - base;
             const int item = (int)(rel / (EXTRA + nb)), b0 = (int)(rel - (int64_t)item * (EXTRA + nb)) - EXTRA;
             const int64_t first = pos - b0;  // the unit of the item's first block
             if (b0 > 0 && first >= pos - per) {
-                r.s = s;
+                r.q0 = w.q0;
                 r.g = item / ng;
-                r.rg = item - r.g * ng;
+                r.r0 = (item - r.g * ng) * ROWS;
+                r.rows = w.n * a.G;
                 r.last = (int)((first + nb - 1) / per);
             }
         }
