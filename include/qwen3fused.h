@@ -334,7 +334,8 @@ int qf_kv_load_quantized(const void* k_cache, const int64_t k_cache_strides[4],
  * contiguous, rows 16-byte aligned (`cache_format` says what they hold); scales
  * (N, Hkv, B), equal strides, for the quantised formats; block_tables int32
  * rows; context_lens, cu_seqlens_q int32; tree_mask (T, mask_words) int64.
- * head_dim 64, 128 or 256; any Hq / Hkv; block tables of at most 2^30 keys a row.
+ * head_dim 64, 128 or 256; any Hq / Hkv; block tables of at most 2^30 keys a row, and
+ * sequences x kv heads x the longest table's blocks of 64 keys below 2^31.
  * A block index outside the cache leaves its keys out (QF_FLAG_BAD_BLOCK);
  * context + drafts longer than the block table's row, a negative length, or
  * cu_seqlens_q that leave [0, num_tokens] are cut (QF_FLAG_BAD_TABLE); drafted

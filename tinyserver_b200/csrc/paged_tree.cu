@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(128) tree_f32_kernel(const TreeDev a) {
     float* corr = ps + FT::PS;  // [4 warps][4 rows]
     int* kval = reinterpret_cast<int*>(corr + 16);
 
-    __shared__ int64_t scratch[34];
+    __shared__ int scratch[34];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wr = warp % WR, wk = warp / WR;
     pdl_wait();
@@ -410,6 +410,7 @@ struct TreePlan {
     int ctas;       // persistent CTAs: as many as fit, or one per unit of work if that is fewer
     int min_units;  // least stretch of a CTA
     bool split;     // whether sequences may be cut
+    bool fits;      // whether the work has fewer than 2^31 units
 };
 
 // The kernel and its grid, by sizes alone (lengths are on the device; the block
@@ -441,6 +442,7 @@ TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     const int64_t slots = (int64_t)sm_count() * per_sm;
     p.split = blocks > (keys == 128 ? 6 : 4);
     p.ctas = (int)(items >= slots ? slots : std::min(slots, items * blocks));
+    p.fits = items <= INT32_MAX / (blocks + 8);
     return p;
 }
 
@@ -519,6 +521,7 @@ extern "C" int qf_paged_tree_attention(const qf_paged_tree_attention_args* p, cu
     int rc = qf::check_tree_args(g);
     if (rc || g.num_tokens == 0) return rc;
     const qf::TreePlan plan = qf::make_plan(g);
+    if (!plan.fits) return QF_ERR_UNSUPPORTED;
     const size_t need = qf::plan_bytes(g, plan);
     if (need > 0 && g.workspace) {
         if (g.workspace_bytes < 0 || (size_t)g.workspace_bytes < need) return QF_ERR_INVALID;

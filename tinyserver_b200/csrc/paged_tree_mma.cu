@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
     static_assert(kWarps * NR * (D + 2) * 4 <= R::SMEM, "merge area");
 
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int64_t scratch[34];
+    __shared__ int scratch[34];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
     const float sl2 = a.scale * 1.4426950408889634f;
     unsigned char* ring = smem + warp * R::WARP;

@@ -184,6 +184,7 @@ __device__ __forceinline__ bool expand(char* tile, int nk, int d0, int lane) {
 template <typename T, int FMT>
 __device__ float dot_row(const T* q, const char* k) {
     float acc = 0.f;
+#pragma unroll 4
     for (int d = 0; d < kD; ++d) {
         float x;
         if constexpr (FMT == QF_CACHE_PLAIN) x = Dt<T>::to_f(reinterpret_cast<const T*>(k)[d]);
@@ -206,6 +207,7 @@ __device__ __noinline__ void add_not_finite(const TreeDev& a, const int32_t* bt,
         int64_t row, srow;
         if (!key_place(a, bt, g, j, row, srow)) continue;
         float p = -1.f;
+#pragma unroll 1
         for (int d = 0; d < kD; ++d) {
             float v;
             if constexpr (FMT == QF_CACHE_PLAIN) v = Dt<T>::to_f(reinterpret_cast<const T*>(a.vc)[row + d]);
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     __shared__ TreeBars<NT> bars;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, odd_v;  // odd_v: the last segment whose drafted V was not finite, from 1
-    __shared__ int64_t scratch[34];
+    __shared__ int scratch[34];
     __shared__ __align__(16) uint32_t valid[C::SLOTS][4];
     // of a block's keys: k-scale, v-scale * 2^x, log2 of that; whether the block's all are
     // near 1; x
@@ -667,38 +669,46 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             // 2 i + lane / 16), into the tile.  (The segment before is done with Q: its O,
             // which this thread has read, was final.)
             using P = Packed<T>;
-            const int hi = lane >> 4, c = lane & 15;
+            const int hi = lane >> 4, c = lane & 15, w0 = (warp & 3) * 32;
             const int64_t at = live ? trow_q * a.qt + (int64_t)hq * a.qh : -1;
-            // rs > 0: a negative scale's sign goes to Q, and 0 becomes as good as 0
-            const uint32_t flip = sl2 < 0.f ? 0x80008000u : 0u;
-            const float sl_abs = fabsf(sl2) < 1e-30f ? 1e-30f : fabsf(sl2);
-            if (!Q8) rs = sl_abs;
-            uint4 v[16];  // all in flight
-#pragma unroll
+#pragma unroll 4
             for (int i = 0; i < 16; ++i) {
                 const int64_t o = __shfl_sync(kFull, at, 2 * i + hi);
-                v[i] = o >= 0 ? ld_stream16(reinterpret_cast<const T*>(a.q) + o + 8 * c) : make_uint4(0, 0, 0, 0);
+                cp_async16_at(smem_u32(qtile) + tile_off(w0 + 2 * i + hi, c),
+                              reinterpret_cast<const T*>(a.q) + (o < 0 ? 0 : o) + 8 * c, o < 0 ? 0 : 16);
             }
+            cp_async_commit();
+            cp_async_wait<0>();
+            __syncwarp();
+            // rs > 0: a negative scale's sign goes to Q, and 0 becomes as good as 0
+            const uint32_t flip = sl2 < 0.f ? 0x80008000u : 0u;
+            rs = fabsf(sl2) < 1e-30f ? 1e-30f : fabsf(sl2);
+            if (Q8 || flip) {
+                int er = 0;  // this thread's own row's exponent
+#pragma unroll 2
+                for (int i = 0; i < 16; ++i) {
+                    uint4* cell = reinterpret_cast<uint4*>(qtile + tile_off(w0 + 2 * i + hi, c));
+                    uint4 v = *cell;
+                    if constexpr (Q8) {  // a power-of-two factor brings the row's largest element to [2^14, 2^15)
+                        uint32_t mx = 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if constexpr (Q8) {  // a power-of-two factor brings the row's largest element to [2^14, 2^15)
-                    uint32_t mx = 0;
+                        for (int x = 0; x < 4; ++x)
+                            mx = max(mx, max(__float_as_uint(P::lo(word(v, x))) & 0x7fffffffu,
+                                             __float_as_uint(P::hi(word(v, x))) & 0x7fffffffu));
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        mx = max(mx, max(__float_as_uint(P::lo(word(v[i], x))) & 0x7fffffffu,
-                                         __float_as_uint(P::hi(word(v[i], x))) & 0x7fffffffu));
+                        for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
+                        const int e = min(max((int)(mx >> 23) - 127, -100), 127);
+                        const float f = __int_as_float((127 + 14 - e) << 23);
 #pragma unroll
-                    for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
-                    const int e = min(max((int)(mx >> 23) - 127, -100), 127);
-                    const float f = __int_as_float((127 + 14 - e) << 23);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        set_word(v[i], x, MP::pack(P::lo(word(v[i], x)) * f, P::hi(word(v[i], x)) * f));
-                    const int er = __shfl_sync(kFull, e, (lane & 1) * 16);  // lane's own row's, if it is one of these
-                    if ((lane >> 1) == i) rs = fmaxf(sl_abs * __int_as_float((127 - 14 + er) << 23), 1.2e-38f);
+                        for (int x = 0; x < 4; ++x)
+                            set_word(v, x, MP::pack(P::lo(word(v, x)) * f, P::hi(word(v, x)) * f));
+                        const int mine = __shfl_sync(kFull, e, (lane & 1) * 16);  // the row's, if it is one of these
+                        if ((lane >> 1) == i) er = mine;
+                    }
+                    v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+                    *cell = v;
                 }
-                v[i].x ^= flip, v[i].y ^= flip, v[i].z ^= flip, v[i].w ^= flip;
-                *reinterpret_cast<uint4*>(qtile + tile_off((warp & 3) * 32 + 2 * i + hi, c)) = v[i];
+                if constexpr (Q8) rs = fmaxf(rs * __int_as_float((127 - 14 + er) << 23), 1.2e-38f);
             }
             proxy_fence();
             mbar_arrive(&bars.q_full);

@@ -123,18 +123,19 @@ struct TreeSeg {
 
 template <int KB, int ROWS, int EXTRA>
 struct TreeWalk {
-    int64_t pos, end, base, us;  // this CTA's stretch; the current sequence's first unit and units
-    int64_t per;                 // units of a stretch
-    int s, nb, ng;               // the current sequence, its key blocks and groups per head
-                                 // (an item: EXTRA + nb units)
+    // (the launcher sees to it that all units are fewer than 2^31)
+    int pos, end, base, us;  // this CTA's stretch; the current sequence's first unit and units
+    int per;                 // units of a stretch
+    int s, nb, ng;           // the current sequence, its key blocks and groups per head
+                             // (an item: EXTRA + nb units)
     TreeSeq w;
 
     __device__ __forceinline__ static int blocks(const TreeSeq& w) { return max(1, (w.L + KB - 1) / KB); }
     __device__ __forceinline__ static int groups(const TreeDev& a, const TreeSeq& w) {
-        return (int)(((int64_t)w.n * a.G + ROWS - 1) / ROWS);
+        return (w.n * a.G + ROWS - 1) / ROWS;
     }
-    __device__ __forceinline__ static int64_t units(const TreeDev& a, const TreeSeq& w) {
-        return (int64_t)(EXTRA + blocks(w)) * groups(a, w) * a.Hkv;
+    __device__ __forceinline__ static int units(const TreeDev& a, const TreeSeq& w) {
+        return (EXTRA + blocks(w)) * groups(a, w) * a.Hkv;
     }
     __device__ __forceinline__ void enter(const TreeDev& a, int seq) {
         s = seq;
@@ -144,26 +145,27 @@ struct TreeWalk {
         us = units(a, w);
     }
 
-    // By all threads of the CTA (`scratch`: 34 int64 of shared memory): the units
+    // By all threads of the CTA (`scratch`: 34 words of shared memory): the units
     // of all sequences, this CTA's stretch, and the sequence it begins in.  CTA 0
     // reports what had to be cut.
-    __device__ void begin(const TreeDev& a, int64_t* scratch) {
+    __device__ __forceinline__ void begin(const TreeDev& a, int* scratch) {
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
         const int nt = nw * 32;
-        int64_t before = 0, u = 0, first = 0, total = 0;
+        int before = 0, u = 0, first = 0, total = 0;
         // first: the units before sequence i0 + tid; all: of sequences [i0, i0 + nt)
-        auto scan = [&](int i0, bool report) -> int64_t {
+        auto scan = [&](int i0, bool report) -> int {
             const int i = i0 + tid;
             u = i < a.S ? units(a, tree_seq(a, i, report)) : 0;
-            int64_t incl = u;
+            int incl = u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += v;
             }
             if (lane == 31) scratch[warp] = incl;
             __syncthreads();
-            int64_t warps = 0, all = 0;
+            int warps = 0, all = 0;
+#pragma unroll 1
             for (int x = 0; x < nw; ++x) {
                 if (x < warp) warps += scratch[x];
                 all += scratch[x];
@@ -172,13 +174,16 @@ struct TreeWalk {
             first = before + warps + incl - u;
             return all;
         };
+#pragma unroll 1
         for (int i0 = 0; i0 < a.S; i0 += nt) total += scan(i0, blockIdx.x == 0);
-        per = max((int64_t)a.min_units, (total + gridDim.x - 1) / gridDim.x);
-        pos = min(total, per * blockIdx.x);
-        end = min(total, pos + per);
+        const int ctas = (int)gridDim.x;
+        per = max(a.min_units, (total - 1) / ctas + 1);
+        pos = (int)min((int64_t)total, (int64_t)per * blockIdx.x);
+        end = total - pos > per ? pos + per : total;
         // the sequence with base <= pos < base + us (with up to nt sequences, scanned already)
+#pragma unroll 1
         for (int i0 = 0; i0 < a.S && before <= pos; i0 += nt) {
-            const int64_t all = a.S <= nt ? total : scan(i0, false);
+            const int all = a.S <= nt ? total : scan(i0, false);
             if (first <= pos && pos < first + u) {
                 scratch[32] = i0 + tid;
                 scratch[33] = first;
@@ -188,7 +193,7 @@ struct TreeWalk {
         __syncthreads();
         if (pos < end) {
             base = scratch[33];
-            enter(a, (int)scratch[32]);
+            enter(a, scratch[32]);
         }
         __syncthreads();
     }
@@ -200,9 +205,8 @@ struct TreeWalk {
                 enter(a, s + 1);
                 continue;
             }
-            const int64_t rel = pos - base;
-            const int item = (int)(rel / (EXTRA + nb)), u0 = (int)(rel - (int64_t)item * (EXTRA + nb));
-            const int u1 = (int)min((int64_t)(EXTRA + nb), u0 + (end - pos));
+            const int rel = pos - base, item = rel / (EXTRA + nb), u0 = rel - item * (EXTRA + nb);
+            const int u1 = min(EXTRA + nb, u0 + (end - pos));
             if (!a.ws && u0 > 0) {  // an item of the CTA before
                 pos += EXTRA + nb - u0;
                 continue;
@@ -227,15 +231,14 @@ struct TreeWalk {
         if (!a.ws) return;
         TreeRec r{};
         if (pos < end && pos > base) {
-            const int64_t rel = pos - base;
-            const int item = (int)(rel / (EXTRA + nb)), b0 = (int)(rel - (int64_t)item * (EXTRA + nb)) - EXTRA;
-            const int64_t first = pos - b0;  // the unit of the item's first block
+            const int rel = pos - base, item = rel / (EXTRA + nb), b0 = rel - item * (EXTRA + nb) - EXTRA;
+            const int first = pos - b0;  // the unit of the item's first block
             if (b0 > 0 && first >= pos - per) {
                 r.q0 = w.q0;
                 r.g = item / ng;
                 r.r0 = (item - r.g * ng) * ROWS;
                 r.rows = w.n * a.G;
-                r.last = (int)((first + nb - 1) / per);
+                r.last = (first + nb - 1) / per;
             }
         }
         reinterpret_cast<TreeRec*>(a.ws)[blockIdx.x] = r;
@@ -282,18 +285,20 @@ __device__ __forceinline__ uint32_t tree_bits32(const int64_t* row, int words, i
 template <typename T, int D>
 __device__ __forceinline__ void zero_unowned_rows(const TreeDev& a) {
     if (!a.cu) return;
-    constexpr int CH = D * (int)sizeof(T) / 16;
+    const int chunks = a.Hq * (D * (int)sizeof(T) / 16);  // 16-byte pieces of a query token
     auto zero = [&](int t0, int t1) {
-        const int64_t n = (int64_t)max(0, t1 - t0) * a.Hq * CH;
-        for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
-            const int64_t r = i / CH;
-            char* o = a.out + ((t0 + r / a.Hq) * a.ot + (r % a.Hq) * a.oh) * (int64_t)sizeof(T);
-            st16(o + (i - r * CH) * 16, make_uint4(0, 0, 0, 0));
-        }
+#pragma unroll 1
+        for (int t = t0; t < t1; ++t)
+#pragma unroll 1
+            for (int i = threadIdx.x; i < chunks; i += blockDim.x) {
+                const int h = i / (D * (int)sizeof(T) / 16), c = i % (D * (int)sizeof(T) / 16);
+                st16(a.out + (t * a.ot + h * a.oh) * (int64_t)sizeof(T) + c * 16, make_uint4(0, 0, 0, 0));
+            }
     };
     auto row = [&](int s) { return min(max(__ldg(a.cu + s), 0), a.T); };
     if (blockIdx.x == 0) zero(0, row(0));
     if (blockIdx.x == gridDim.x - 1) zero(max(row(a.S - 1), row(a.S)), a.T);
+#pragma unroll 1
     for (int s = blockIdx.x; s < a.S; s += gridDim.x) {
         const int b = row(s), e = max(b, row(s + 1));
         if (e - b > a.max_tree) zero(b + a.max_tree, e);
