@@ -138,11 +138,13 @@ __device__ __forceinline__ bool clean_rows(char* tile, int r0, int r1, int lane)
 
 // By one warp: a tile's codes, which landed in its second slab (a row's 128 codes are
 // as long as half a row of fp16), into the fp16 tile, in place: a row is read by
-// eight lanes before any of them writes.  EDGE: rows from nk on are zero, and
-// infinities and NaN in rows from d0 on are set to zero; whether there were any.
+// eight lanes before any of them writes.  (The lanes of a row's second half take the
+// row beside it, whose swizzle puts their chunks in other banks.)  EDGE: rows from nk
+// on are zero, and infinities and NaN in rows from d0 on are set to zero; whether
+// there were any.
 template <int FMT, bool EDGE>
 __device__ __forceinline__ bool expand(char* tile, int nk, int d0, int lane) {
-    const int c = lane & 7, r4 = lane >> 3;
+    const int c = lane & 7, r4 = (lane >> 3) ^ (c >> 2);
     uint32_t odd = 0;
 #pragma unroll 1
     for (int i0 = 0; i0 < 32; i0 += 8) {
@@ -169,11 +171,8 @@ __device__ __forceinline__ bool expand(char* tile, int nk, int d0, int lane) {
                     zero_not_finite<__half>(hi);
                 }
             }
-            // (lanes of the second slab the odd chunk first: eight lanes, eight bank groups)
-            const bool second = c >> 2;
-            const uint4 one = second ? hi : lo, two = second ? lo : hi;
-            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + (c >> 2))) = one;
-            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + 1 - (c >> 2))) = two;
+            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c)) = lo;
+            *reinterpret_cast<uint4*>(tile + tile_off(r, 2 * c + 1)) = hi;
         }
         __syncwarp();
     }
@@ -782,13 +781,15 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                 const float mref = m == -INFINITY ? 0.f : m;
                 float mx0 = -INFINITY, mx1 = -INFINITY;
                 float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-                uint32_t x[2][32];
+                // the second quarter's load in flight meanwhile, where registers allow
+                constexpr int NX = Q8 && NT == 1 ? 1 : 2;
+                uint32_t x[NX][32];
                 tmem_ld32(sh, x[0]);
                 tmem_wait_ld();
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    if (q == 0) tmem_ld32(sh + 32, x[1]);  // in flight meanwhile
-                    uint32_t* xs = x[q];
+                    if (NX == 2 && q == 0) tmem_ld32(sh + 32, x[NX - 1]);
+                    uint32_t* xs = x[NX == 2 ? q : 0];
                     const int cq = c0 + 32 * q;
                     if constexpr (Q8) {
 #pragma unroll
@@ -824,6 +825,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                         pk[16 * q + (e >> 1)] = MP::pack(p[0], p[1]);
                         pk[16 * q + (e >> 1) + 1] = MP::pack(p[2], p[3]);
                     }
+                    if (NX == 1 && q == 0) tmem_ld32(sh + 32, x[0]);
                     if (q == 0) tmem_wait_ld();
                 }
                 sum = (s0 + s1) + (s2 + s3);
