@@ -285,35 +285,33 @@ size_t qf_paged_attention_noalloc_capacity(void);
  * in fp32, Q = 448 for QF_CACHE_E4M3 (codes are e4m3 bytes), 127 for
  * QF_CACHE_INT8 (signed bytes).  A row with an infinity or a NaN is stored as
  * codes 0 and scale NaN: it reads back as NaN.
- * k_src/v_src: (Hkv, T, D) of `dtype`; caches (N, Hkv, B, D) bytes; scales
- * (N, Hkv, B) fp32; all strides in elements, any values.  The (block, slot)
- * pairs of one call must be distinct: of two tokens sent to one slot, the row
- * and its scale may come from different ones.  Rows of 64, 128 or 256 that
- * start on 16-byte boundaries take the vector path. */
-int qf_kv_store_quantized(const void* k_src, const int64_t k_src_strides[3],
-                          const void* v_src, const int64_t v_src_strides[3],
-                          void* k_cache, const int64_t k_cache_strides[4],
-                          void* v_cache, const int64_t v_cache_strides[4],
-                          float* k_scale, const int64_t k_scale_strides[3],
-                          float* v_scale, const int64_t v_scale_strides[3],
-                          const void* block_mapping, const void* slot_mapping, int index_type,
-                          int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
-                          int64_t num_blocks, int64_t block_size, int dtype, int format,
-                          int32_t* status, cudaStream_t stream);
+ * k_rows/v_rows: (Hkv, T, D) of `dtype` (a load writes them); caches
+ * (N, Hkv, B, D) bytes; scales (N, Hkv, B) fp32; all strides in elements, any
+ * values.  The (block, slot) pairs of one store must be distinct: of two tokens
+ * sent to one slot, the row and its scale may come from different ones.  Rows of
+ * 64, 128 or 256 that start on 16-byte boundaries take the vector path. */
+typedef struct {
+    void* k_rows; int64_t k_row_strides[3];
+    void* v_rows; int64_t v_row_strides[3];
+    void* k_cache; int64_t k_cache_strides[4];
+    void* v_cache; int64_t v_cache_strides[4];
+    float* k_scale; int64_t k_scale_strides[3];
+    float* v_scale; int64_t v_scale_strides[3];
+    const void* block_mapping; const void* slot_mapping;
+    int64_t num_tokens, num_kv_heads, head_dim, num_blocks, block_size;
+    int index_type, dtype, format;
+    int32_t* status;
+} qf_kv_quantized_args;
 
-/* The rows back: k_out/v_out[h, t, :] = rnd(code * scale) of the row at
+int qf_kv_store_quantized(const qf_kv_quantized_args* args, cudaStream_t stream);
+
+/* The rows back: k_rows/v_rows[h, t, :] = rnd(code * scale) of the row at
  * (block_mapping[t], slot_mapping[t]), in `dtype`.  A place outside the cache
  * reads as a zero row and is flagged. */
-int qf_kv_load_quantized(const void* k_cache, const int64_t k_cache_strides[4],
-                         const void* v_cache, const int64_t v_cache_strides[4],
-                         const float* k_scale, const int64_t k_scale_strides[3],
-                         const float* v_scale, const int64_t v_scale_strides[3],
-                         const void* block_mapping, const void* slot_mapping, int index_type,
-                         void* k_out, const int64_t k_out_strides[3],
-                         void* v_out, const int64_t v_out_strides[3],
-                         int64_t num_tokens, int64_t num_kv_heads, int64_t head_dim,
-                         int64_t num_blocks, int64_t block_size, int dtype, int format,
-                         int32_t* status, cudaStream_t stream);
+int qf_kv_load_quantized(const qf_kv_quantized_args* args, cudaStream_t stream);
+
+/* sizeof(qf_kv_quantized_args) as compiled into the library. */
+size_t qf_kv_quantized_args_size(void);
 
 /* ---------------------------------------------------------------------- */
 /* Attention of several new tokens per sequence over the paged cache, for the
@@ -379,9 +377,20 @@ size_t qf_paged_tree_attention_args_size(void);
  * rounded up; depths int32.  A parent that is no earlier node is read as -1, nodes past max_tree
  * get an empty mask and depth 0 (QF_FLAG_BAD_TREE); nodes outside every sequence likewise
  * (unflagged: a padded batch). */
-int qf_build_tree_mask(const void* parents, int index_type, const int32_t* cu_seqlens,
-                       int64_t num_seqs, int64_t num_nodes, int64_t max_tree, int64_t mask_words,
-                       int64_t* mask, int32_t* depths, int32_t* status, cudaStream_t stream);
+typedef struct {
+    const void* parents;
+    const int32_t* cu_seqlens;
+    int64_t num_seqs, num_nodes, max_tree, mask_words;
+    int64_t* mask;
+    int32_t* depths;
+    int index_type;
+    int32_t* status;
+} qf_tree_mask_args;
+
+int qf_build_tree_mask(const qf_tree_mask_args* args, cudaStream_t stream);
+
+/* sizeof(qf_tree_mask_args) as compiled into the library. */
+size_t qf_tree_mask_args_size(void);
 
 /* ---------------------------------------------------------------------- */
 /* Prefill attention over variable-length packed sequences.  Replaces

@@ -278,6 +278,56 @@ def test_strided_inputs_scale_and_layer_views():
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("fmt", ref.FORMATS)
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("n,hq", [(8, 2), (12, 16), (40, 16)])
+def test_scales_over_eight_decades_and_none(fmt, dtype, n, hq):
+    """V's row scales from 1e-6 to 1e2 beside each other (none brings them all near 1), whole pages of one
+    size, and scales of 0 (rows never written, which stand for zeros but have their weight)."""
+    sizes, contexts = [n, 3], [1500, 130]
+    q, k, v, ks, vs, bt, mask = _case(sizes, contexts, hq, 2, 128, 16, dtype, fmt, 21)
+    g = torch.Generator().manual_seed(3)
+    vs *= (10.0 ** torch.randint(-4, 5, vs.shape, generator=g)).to(DEV)
+    vs[bt[0, 8:24].long()] = 0.02
+    ks[bt[0, 40].long()] = 0.0
+    vs[bt[0, 40].long()] = 0.0
+    out, bound = ref.attention(q, k, v, bt, 16, contexts, sizes, mask, ks, vs, p_type=torch.float16)
+    for split in (True, False):
+        got = _run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes, split=split)
+        tsb.check_errors()
+        ref.assert_within(got, out, bound, f"split={split}")
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_negative_and_zero_softmax_scale(dtype, scale):
+    """The definition holds for any scale: least scores first, and a plain mean of the seen values."""
+    for hq, fmt in ((2, None), (20, None), (20, E4M3)):
+        q, k, v, ks, vs, bt, mask = _case([9, 40], [300, 0], hq, 1, 128, 16, dtype, fmt, 8)
+        out, bound = ref.attention(q, k, v, bt, 16, [300, 0], [9, 40], mask, ks, vs, scale=scale,
+                                   p_type=torch.float16 if fmt else None)
+        ref.assert_within(_run(q, k, v, ks, vs, bt, mask, 16, [300, 0], [9, 40], softmax_scale=scale), out, bound)
+
+
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (32, 2), (64, 2)])
+def test_many_sequences_of_every_length(hq, hkv):
+    """More sequences than a CTA has threads, empty ones among them: each CTA's stretch of the work begins and
+    ends where it should; twice, with the same bits."""
+    g = torch.Generator().manual_seed(5)
+    n = 400
+    sizes = torch.randint(0, 6, (n,), generator=g).tolist()
+    contexts = [int(x) if i % 7 else 0 for i, x in enumerate(torch.randint(0, 300, (n,), generator=g))]
+    contexts[77], contexts[399] = 5000, 2222
+    for fmt in (None, E4M3):
+        q, k, v, ks, vs, bt, mask = _case(sizes, contexts, hq, hkv, 128, 16, torch.bfloat16, fmt, 3)
+        out, bound = ref.attention(q, k, v, bt, 16, contexts, sizes, mask, ks, vs,
+                                   p_type=torch.float16 if fmt else None)
+        got = _run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes)
+        tsb.check_errors()
+        ref.assert_within(got, out, bound)
+        assert torch.equal(got, _run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes))
+
+
 def test_two_graphs_share_nothing():
     sizes, contexts = [30, 8], [2000, 700]
     cases = [_case(sizes, contexts, 16, 2, 128, 16, torch.bfloat16, f, 4) for f in (None, E4M3)]
@@ -316,3 +366,42 @@ def test_large_scores_and_minus_infinity():
         got = _run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes)
         clean = [t for t in range(12) if not (int(mask[t, 0]) >> 2) & 1]
         ref.assert_within(got[clean], out[clean], bound[clean])
+
+
+def test_registered_ops_match_their_fakes_and_run_in_a_graph():
+    """opcheck on real launches, and one verification step under torch.compile, caches included."""
+    Q = torch.ops.qwen3fused
+    sizes, contexts, B = [4, 3], [30, 9], 16
+    q, k, v, ks, vs, bt, mask = _case(sizes, contexts, 8, 2, 128, B, torch.bfloat16, E4M3, 15)
+    g = torch.Generator().manual_seed(2)
+    parents, cu = ref.random_parents(sizes, g).to(DEV), _cu(sizes)
+    lens = torch.tensor(contexts, dtype=torch.int32, device=DEV)
+    kn, vn = (torch.randn(2, 7, 128, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    of = torch.tensor([0] * 4 + [1] * 3, device=DEV)
+    at = lens[of].long() + torch.tensor([0, 1, 2, 3, 0, 1, 2], device=DEV)
+    bm, sm = bt[of, at // B].long(), at % B
+    checks = ("test_schema", "test_faketensor")
+    i8 = torch.zeros(k.shape[0], 2, B, 128, dtype=torch.int8, device=DEV)
+    sc = torch.ones(k.shape[0], 2, B, device=DEV)
+    torch.library.opcheck(Q.store_kv_cache_quantized, (kn, vn, i8, i8.clone(), sc, sc.clone(), bm, sm),
+                          test_utils=checks)
+    torch.library.opcheck(Q.load_kv_cache_quantized, (i8, i8.clone(), sc, sc.clone(), bm, sm, torch.float16),
+                          test_utils=checks)
+    torch.library.opcheck(Q.build_tree_mask, (parents, cu, 5), test_utils=checks)
+    torch.library.opcheck(Q.paged_attention_quantized, (q[:2], i8, i8.clone(), sc, sc.clone(), bt, B, lens),
+                          test_utils=checks)
+    torch.library.opcheck(Q.paged_tree_attention, (q, i8, i8.clone(), bt, B, lens, cu, mask, 4, sc, sc.clone()),
+                          test_utils=checks)
+
+    def step(q, kn, vn, k, v, ks, vs):
+        m, _ = Q.build_tree_mask(parents, cu, 4)
+        Q.store_kv_cache_quantized(kn, vn, k, v, ks, vs, bm, sm)
+        return Q.paged_tree_attention(q, k, v, bt, B, lens, cu, m, 4, ks, vs) * 2
+
+    caches = [[x.clone() for x in (k, v, ks, vs)] for _ in range(2)]
+    want = step(q, kn, vn, *caches[0])
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(q, kn, vn, *caches[1])
+    tsb.check_errors()
+    assert torch.equal(got, want)
+    for a, b in zip(*caches):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))

@@ -8,8 +8,8 @@ fails, every op raises -- there is no CPU or torch fallback.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
+import struct
 import threading
 
 from . import build as _build
@@ -80,26 +80,57 @@ class PagedAttentionArgs(ctypes.Structure):
     ]
 
 
-class PagedTreeAttentionArgs(ctypes.Structure):
-    """Mirror of qf_paged_tree_attention_args (field order and types must match)."""
+class PackedArgs:
+    """An argument struct of the C side as bytes, packed by position in one call (a few
+    microseconds less than a ctypes Structure's fields).  Native sizes and alignment:
+    the order and the types must match the header; NULL is 0."""
 
-    _fields_ = [
-        ("q", c_vp), ("q_stride_token", c_i64), ("q_stride_head", c_i64),
-        ("k_cache", c_vp), ("v_cache", c_vp), ("cache_strides", c_i64 * 4),
-        ("k_scale", c_vp), ("v_scale", c_vp), ("scale_strides", c_i64 * 3),
-        ("num_blocks", c_i64), ("block_size", c_i64),
-        ("block_tables", c_vp), ("block_tables_row_stride", c_i64),
-        ("max_blocks_per_seq", c_i64),
-        ("context_lens", c_vp), ("cu_seqlens_q", c_vp),
-        ("tree_mask", c_vp), ("mask_words", c_i64),
-        ("num_seqs", c_i64), ("num_tokens", c_i64), ("max_tree", c_i64),
-        ("num_q_heads", c_i64), ("num_kv_heads", c_i64), ("head_dim", c_i64),
-        ("scale", c_float),
-        ("out", c_vp), ("out_stride_token", c_i64), ("out_stride_head", c_i64),
-        ("workspace", c_vp), ("workspace_bytes", c_i64),
-        ("dtype", c_int), ("cache_format", c_int),
-        ("status", c_vp),
-    ]
+    def __init__(self, *fields: tuple[str, str]):
+        self.names = tuple(name for name, code in fields for _ in range(int(code[:-1] or 1)))
+        # "0q" at the end: padded to the size of its widest member
+        self._struct = struct.Struct("@" + "".join(code for _, code in fields) + "0q")
+        self.pack = self._struct.pack
+        self.size = self._struct.size
+
+    def named(self, **values) -> bytes:
+        """Packed from names, the rest 0 (a name of several members takes a tuple)."""
+        left = {k: list(v) if isinstance(v, tuple) else [v] for k, v in values.items()}
+        return self.pack(*(left[n].pop(0) if left.get(n) else 0 for n in self.names))
+
+
+# qf_kv_quantized_args
+KvQuantizedArgs = PackedArgs(
+    ("k_rows", "q"), ("k_row_strides", "3q"), ("v_rows", "q"), ("v_row_strides", "3q"),
+    ("k_cache", "q"), ("k_cache_strides", "4q"), ("v_cache", "q"), ("v_cache_strides", "4q"),
+    ("k_scale", "q"), ("k_scale_strides", "3q"), ("v_scale", "q"), ("v_scale_strides", "3q"),
+    ("block_mapping", "q"), ("slot_mapping", "q"),
+    ("num_tokens", "q"), ("num_kv_heads", "q"), ("head_dim", "q"), ("num_blocks", "q"),
+    ("block_size", "q"),
+    ("index_type", "i"), ("dtype", "i"), ("format", "i"),
+    ("status", "q"))
+
+# qf_tree_mask_args
+TreeMaskArgs = PackedArgs(
+    ("parents", "q"), ("cu_seqlens", "q"), ("num_seqs", "q"), ("num_nodes", "q"),
+    ("max_tree", "q"), ("mask_words", "q"), ("mask", "q"), ("depths", "q"), ("index_type", "i"),
+    ("status", "q"))
+
+# qf_paged_tree_attention_args
+PagedTreeAttentionArgs = PackedArgs(
+    ("q", "q"), ("q_stride_token", "q"), ("q_stride_head", "q"),
+    ("k_cache", "q"), ("v_cache", "q"), ("cache_strides", "4q"),
+    ("k_scale", "q"), ("v_scale", "q"), ("scale_strides", "3q"),
+    ("num_blocks", "q"), ("block_size", "q"),
+    ("block_tables", "q"), ("block_tables_row_stride", "q"), ("max_blocks_per_seq", "q"),
+    ("context_lens", "q"), ("cu_seqlens_q", "q"),
+    ("tree_mask", "q"), ("mask_words", "q"),
+    ("num_seqs", "q"), ("num_tokens", "q"), ("max_tree", "q"),
+    ("num_q_heads", "q"), ("num_kv_heads", "q"), ("head_dim", "q"),
+    ("scale", "f"),
+    ("out", "q"), ("out_stride_token", "q"), ("out_stride_head", "q"),
+    ("workspace", "q"), ("workspace_bytes", "q"),
+    ("dtype", "i"), ("cache_format", "i"),
+    ("status", "q"))
 
 
 class VarlenAttentionArgs(ctypes.Structure):
@@ -162,16 +193,14 @@ SIGNATURES: dict[str, list] = {
     "qf_paged_attention_args_size": [],
     "qf_paged_attention_decode_noalloc": [ctypes.POINTER(PagedAttentionArgs), c_vp],
     "qf_paged_attention_noalloc_capacity": [],
-    "qf_kv_store_quantized": [c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp,
-                              I64P, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_int,
-                              c_int, c_vp, c_vp],
-    "qf_kv_load_quantized": [c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp, I64P, c_vp, c_vp, c_int,
-                             c_vp, I64P, c_vp, I64P, c_i64, c_i64, c_i64, c_i64, c_i64, c_int,
-                             c_int, c_vp, c_vp],
-    "qf_paged_tree_attention": [ctypes.POINTER(PagedTreeAttentionArgs), c_vp],
-    "qf_paged_tree_attention_workspace_bytes": [ctypes.POINTER(PagedTreeAttentionArgs)],
+    "qf_kv_store_quantized": [c_vp, c_vp],
+    "qf_kv_load_quantized": [c_vp, c_vp],
+    "qf_kv_quantized_args_size": [],
+    "qf_paged_tree_attention": [c_vp, c_vp],
+    "qf_paged_tree_attention_workspace_bytes": [c_vp],
     "qf_paged_tree_attention_args_size": [],
-    "qf_build_tree_mask": [c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp],
+    "qf_build_tree_mask": [c_vp, c_vp],
+    "qf_tree_mask_args_size": [],
     "qf_varlen_attention": [ctypes.POINTER(VarlenAttentionArgs), c_vp],
     "qf_varlen_attention_args_size": [],
     "qf_sample_tokens": [ctypes.POINTER(SampleArgs), c_vp],
@@ -188,6 +217,8 @@ RESTYPES = {"qf_last_cuda_error": ctypes.c_char_p, "qf_version": ctypes.c_char_p
             "qf_paged_attention_workspace_bytes": ctypes.c_size_t,
             "qf_paged_tree_attention_workspace_bytes": ctypes.c_size_t,
             "qf_paged_tree_attention_args_size": ctypes.c_size_t,
+            "qf_kv_quantized_args_size": ctypes.c_size_t,
+            "qf_tree_mask_args_size": ctypes.c_size_t,
             "qf_paged_attention_noalloc_capacity": ctypes.c_size_t,
             "qf_sample_workspace_bytes": c_i64,
             "qf_varlen_attention_args_size": ctypes.c_size_t,
@@ -220,13 +251,19 @@ def lib() -> ctypes.CDLL:
                 fn.restype = RESTYPES.get(name, c_int)
             for fn, mirror in (("qf_qk_norm_rope_args_size", QkNormRopeArgs),
                                ("qf_paged_attention_args_size", PagedAttentionArgs),
-                               ("qf_paged_tree_attention_args_size", PagedTreeAttentionArgs),
                                ("qf_varlen_attention_args_size", VarlenAttentionArgs),
                                ("qf_sample_args_size", SampleArgs)):
                 size = getattr(handle, fn)()
                 if size != ctypes.sizeof(mirror):
                     raise RuntimeError(f"{fn}: ABI mismatch, library {size} bytes, binding "
                                        f"{ctypes.sizeof(mirror)} bytes")
+            for fn, packed in (("qf_kv_quantized_args_size", KvQuantizedArgs),
+                               ("qf_tree_mask_args_size", TreeMaskArgs),
+                               ("qf_paged_tree_attention_args_size", PagedTreeAttentionArgs)):
+                size = getattr(handle, fn)()
+                if size != packed.size:
+                    raise RuntimeError(f"{fn}: ABI mismatch, library {size} bytes, binding "
+                                       f"{packed.size} bytes")
             _lib = handle
     return _lib
 
@@ -247,13 +284,6 @@ def check(rc: int, what: str) -> None:
         err = lib().qf_last_cuda_error().decode()
         raise RuntimeError(f"{what}: CUDA launch failed: {err}")
     raise RuntimeError(f"{what}: error code {rc}")
-
-
-@functools.lru_cache(maxsize=4096)
-def strides_array(strides: tuple) -> ctypes.Array:
-    """A tensor's strides as the C side reads them, made once per distinct tuple (the
-    library takes const pointers, so calls may share one)."""
-    return (c_i64 * len(strides))(*strides)
 
 
 def i64_array(vals) -> ctypes.Array:

@@ -58,6 +58,27 @@ def require_cuda(what: str, *tensors: torch.Tensor | None) -> torch.device:
     return dev
 
 
+def device_index(what: str, *tensors: torch.Tensor | None) -> int:
+    """:func:`require_cuda` as the device's index, without a device object per tensor."""
+    first = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != first:
+            first = -1
+            break
+    if first < 0:
+        require_cuda(what, *tensors)
+    return first
+
+
+def launch(index: int, fn, packed: bytes) -> int:
+    """``fn(packed arguments, the device's current stream)`` with that device current."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        return fn(packed, stream)
+    with torch.cuda.device(index):
+        return fn(packed, stream)
+
+
 def stream_ptr(device: torch.device) -> int:
     idx = device.index
     # the handle itself, without the Stream object around it (~1.5 us a call)
@@ -76,6 +97,17 @@ def on_device(device: torch.device):
     if idx is None or idx == torch.cuda.current_device():
         return _SAME_DEVICE
     return torch.cuda.device(idx)
+
+
+def status_ptr(index: int) -> int:
+    """The address of :func:`status_word` of a device, by its index."""
+    w = _status_words.get(index)
+    return (w if w is not None else status_word(torch.device("cuda", index))).data_ptr()
+
+
+def after_launch(index: int) -> None:
+    if SYNC_CHECK:
+        check_errors(index)
 
 
 def status_word(device: torch.device) -> torch.Tensor:

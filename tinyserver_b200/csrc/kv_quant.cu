@@ -205,57 +205,56 @@ int launch(const QuantKv& a, bool fast, cudaStream_t stream) {
 }
 
 template <bool STORE>
-int run(const void* k_rows, const int64_t* ks, const void* v_rows, const int64_t* vs, const void* k_cache,
-        const int64_t* kc, const void* v_cache, const int64_t* vc, const void* k_scale,
-        const int64_t* kss, const void* v_scale, const int64_t* vss, const void* block_mapping,
-        const void* slot_mapping, int index_type, int64_t T, int64_t Hkv, int64_t D, int64_t N,
-        int64_t B, int dtype, int format, int32_t* status, cudaStream_t stream) {
-    if (T < 0 || Hkv < 0 || D < 0 || N < 0 || B < 0) return QF_ERR_INVALID;
-    if (index_type != QF_I32 && index_type != QF_I64) return QF_ERR_INVALID;
-    if (dtype != QF_F32 && dtype != QF_F16 && dtype != QF_BF16) return QF_ERR_INVALID;
-    if (format != QF_CACHE_E4M3 && format != QF_CACHE_INT8) return QF_ERR_INVALID;
-    if (T == 0 || Hkv == 0 || D == 0) return QF_OK;
-    if (!k_rows || !v_rows || !k_cache || !v_cache || !k_scale || !v_scale || !block_mapping ||
-        !slot_mapping || !ks || !vs || !kc || !vc || !kss || !vss)
+int run(const qf_kv_quantized_args* p, cudaStream_t stream) {
+    if (!p) return QF_ERR_INVALID;
+    const qf_kv_quantized_args& g = *p;
+    if (g.num_tokens < 0 || g.num_kv_heads < 0 || g.head_dim < 0 || g.num_blocks < 0 ||
+        g.block_size < 0)
         return QF_ERR_INVALID;
-    if (T > ((int64_t)1 << 31) || Hkv > 65535) return QF_ERR_UNSUPPORTED;
+    if (g.index_type != QF_I32 && g.index_type != QF_I64) return QF_ERR_INVALID;
+    if (g.dtype != QF_F32 && g.dtype != QF_F16 && g.dtype != QF_BF16) return QF_ERR_INVALID;
+    if (g.format != QF_CACHE_E4M3 && g.format != QF_CACHE_INT8) return QF_ERR_INVALID;
+    const int64_t D = g.head_dim;
+    if (g.num_tokens == 0 || g.num_kv_heads == 0 || D == 0) return QF_OK;
+    if (!g.k_rows || !g.v_rows || !g.k_cache || !g.v_cache || !g.k_scale || !g.v_scale ||
+        !g.block_mapping || !g.slot_mapping)
+        return QF_ERR_INVALID;
+    if (g.num_tokens > ((int64_t)1 << 31) || g.num_kv_heads > 65535) return QF_ERR_UNSUPPORTED;
     QuantKv a{};
-    a.k_src = static_cast<const char*>(k_rows);
-    a.v_src = static_cast<const char*>(v_rows);
-    a.k_dst = static_cast<char*>(const_cast<void*>(k_rows));
-    a.v_dst = static_cast<char*>(const_cast<void*>(v_rows));
-    a.k_cache = static_cast<uint8_t*>(const_cast<void*>(k_cache));
-    a.v_cache = static_cast<uint8_t*>(const_cast<void*>(v_cache));
-    a.k_scale = static_cast<float*>(const_cast<void*>(k_scale));
-    a.v_scale = static_cast<float*>(const_cast<void*>(v_scale));
-    const int64_t es = dtype == QF_F32 ? 4 : 2;
+    a.k_src = a.k_dst = static_cast<char*>(g.k_rows);
+    a.v_src = a.v_dst = static_cast<char*>(g.v_rows);
+    a.k_cache = static_cast<uint8_t*>(g.k_cache);
+    a.v_cache = static_cast<uint8_t*>(g.v_cache);
+    a.k_scale = g.k_scale;
+    a.v_scale = g.v_scale;
+    const int64_t es = g.dtype == QF_F32 ? 4 : 2;
     // 16-byte accesses: whole rows contiguous, every row start a multiple of 16 bytes
-    bool fast = (D == 64 || D == 128 || D == 256) && aligned16(k_rows) && aligned16(v_rows) &&
-                aligned16(k_cache) && aligned16(v_cache) && ks[2] == 1 && vs[2] == 1 &&
-                kc[3] == 1 && vc[3] == 1;
+    bool fast = (D == 64 || D == 128 || D == 256) && aligned16(g.k_rows) && aligned16(g.v_rows) &&
+                aligned16(g.k_cache) && aligned16(g.v_cache) && g.k_row_strides[2] == 1 &&
+                g.v_row_strides[2] == 1 && g.k_cache_strides[3] == 1 && g.v_cache_strides[3] == 1;
     for (int i = 0; i < 3; ++i) {
-        a.ks[i] = ks[i];
-        a.vs[i] = vs[i];
-        a.kss[i] = kss[i];
-        a.vss[i] = vss[i];
-        if (i < 2) fast = fast && (ks[i] * es) % 16 == 0 && (vs[i] * es) % 16 == 0;
+        a.ks[i] = g.k_row_strides[i];
+        a.vs[i] = g.v_row_strides[i];
+        a.kss[i] = g.k_scale_strides[i];
+        a.vss[i] = g.v_scale_strides[i];
+        if (i < 2) fast = fast && (a.ks[i] * es) % 16 == 0 && (a.vs[i] * es) % 16 == 0;
     }
     for (int i = 0; i < 4; ++i) {
-        a.kc[i] = kc[i];
-        a.vc[i] = vc[i];
-        if (i < 3) fast = fast && kc[i] % 16 == 0 && vc[i] % 16 == 0;
+        a.kc[i] = g.k_cache_strides[i];
+        a.vc[i] = g.v_cache_strides[i];
+        if (i < 3) fast = fast && a.kc[i] % 16 == 0 && a.vc[i] % 16 == 0;
     }
-    a.block_mapping = block_mapping;
-    a.slot_mapping = slot_mapping;
-    a.index_type = index_type;
-    a.T = T;
-    a.Hkv = Hkv;
+    a.block_mapping = g.block_mapping;
+    a.slot_mapping = g.slot_mapping;
+    a.index_type = g.index_type;
+    a.T = g.num_tokens;
+    a.Hkv = g.num_kv_heads;
     a.D = D;
-    a.N = N;
-    a.B = B;
-    a.status = status;
-    const bool e4m3 = format == QF_CACHE_E4M3;
-    switch (dtype) {
+    a.N = g.num_blocks;
+    a.B = g.block_size;
+    a.status = g.status;
+    const bool e4m3 = g.format == QF_CACHE_E4M3;
+    switch (g.dtype) {
     case QF_F32:
         return e4m3 ? launch<float, QF_CACHE_E4M3, STORE>(a, fast, stream)
                     : launch<float, QF_CACHE_INT8, STORE>(a, fast, stream);
@@ -271,32 +270,12 @@ int run(const void* k_rows, const int64_t* ks, const void* v_rows, const int64_t
 }  // namespace
 }  // namespace qf
 
-extern "C" int qf_kv_store_quantized(
-    const void* k_src, const int64_t k_src_strides[3], const void* v_src,
-    const int64_t v_src_strides[3], void* k_cache, const int64_t k_cache_strides[4], void* v_cache,
-    const int64_t v_cache_strides[4], float* k_scale, const int64_t k_scale_strides[3],
-    float* v_scale, const int64_t v_scale_strides[3], const void* block_mapping,
-    const void* slot_mapping, int index_type, int64_t num_tokens, int64_t num_kv_heads,
-    int64_t head_dim, int64_t num_blocks, int64_t block_size, int dtype, int format,
-    int32_t* status, cudaStream_t stream) {
-    return qf::run<true>(k_src, k_src_strides, v_src, v_src_strides, k_cache, k_cache_strides,
-                         v_cache, v_cache_strides, k_scale, k_scale_strides, v_scale,
-                         v_scale_strides, block_mapping, slot_mapping, index_type, num_tokens,
-                         num_kv_heads, head_dim, num_blocks, block_size, dtype, format, status,
-                         stream);
+extern "C" int qf_kv_store_quantized(const qf_kv_quantized_args* args, cudaStream_t stream) {
+    return qf::run<true>(args, stream);
 }
 
-extern "C" int qf_kv_load_quantized(
-    const void* k_cache, const int64_t k_cache_strides[4], const void* v_cache,
-    const int64_t v_cache_strides[4], const float* k_scale, const int64_t k_scale_strides[3],
-    const float* v_scale, const int64_t v_scale_strides[3], const void* block_mapping,
-    const void* slot_mapping, int index_type, void* k_out, const int64_t k_out_strides[3],
-    void* v_out, const int64_t v_out_strides[3], int64_t num_tokens, int64_t num_kv_heads,
-    int64_t head_dim, int64_t num_blocks, int64_t block_size, int dtype, int format,
-    int32_t* status, cudaStream_t stream) {
-    return qf::run<false>(k_out, k_out_strides, v_out, v_out_strides, k_cache, k_cache_strides,
-                          v_cache, v_cache_strides, k_scale, k_scale_strides, v_scale,
-                          v_scale_strides, block_mapping, slot_mapping, index_type, num_tokens,
-                          num_kv_heads, head_dim, num_blocks, block_size, dtype, format, status,
-                          stream);
+extern "C" int qf_kv_load_quantized(const qf_kv_quantized_args* args, cudaStream_t stream) {
+    return qf::run<false>(args, stream);
 }
+
+extern "C" size_t qf_kv_quantized_args_size(void) { return sizeof(qf_kv_quantized_args); }

@@ -471,7 +471,7 @@ int check_tree_args(const qf_paged_tree_attention_args& g) {
         return QF_ERR_INVALID;
     if (g.cu_seqlens_q) {
         if (g.max_tree < 1 || !g.tree_mask || g.mask_words < 1) return QF_ERR_INVALID;
-        if (g.mask_words < (g.max_tree + 63) / 64) return QF_ERR_INVALID;
+        if (g.mask_words < g.max_tree / 64 + (g.max_tree % 64 != 0)) return QF_ERR_INVALID;
     } else if (g.num_tokens != g.num_seqs) {
         return QF_ERR_INVALID;
     }
@@ -577,19 +577,20 @@ extern "C" int qf_paged_tree_attention(const qf_paged_tree_attention_args* p, cu
     }
 }
 
-extern "C" int qf_build_tree_mask(const void* parents, int index_type, const int32_t* cu_seqlens,
-                                  int64_t num_seqs, int64_t num_nodes, int64_t max_tree,
-                                  int64_t mask_words, int64_t* mask, int32_t* depths, int32_t* status,
-                                  cudaStream_t stream) {
-    if (num_seqs < 0 || num_nodes < 0 || max_tree < 1 || mask_words < 1) return QF_ERR_INVALID;
-    if (index_type != QF_I32 && index_type != QF_I64) return QF_ERR_INVALID;
-    if (mask_words < (max_tree + 63) / 64) return QF_ERR_INVALID;
-    if (num_nodes == 0) return QF_OK;
-    if (num_seqs == 0 || !parents || !cu_seqlens || !mask || !depths) return QF_ERR_INVALID;
-    if (num_seqs > INT32_MAX || num_nodes > INT32_MAX || max_tree > INT32_MAX ||
-        mask_words > INT32_MAX)
+extern "C" int qf_build_tree_mask(const qf_tree_mask_args* p, cudaStream_t stream) {
+    if (!p) return QF_ERR_INVALID;
+    const qf_tree_mask_args& g = *p;
+    if (g.num_seqs < 0 || g.num_nodes < 0 || g.max_tree < 1 || g.mask_words < 1) return QF_ERR_INVALID;
+    if (g.index_type != QF_I32 && g.index_type != QF_I64) return QF_ERR_INVALID;
+    if (g.mask_words < g.max_tree / 64 + (g.max_tree % 64 != 0)) return QF_ERR_INVALID;
+    if (g.num_nodes == 0) return QF_OK;
+    if (g.num_seqs == 0 || !g.parents || !g.cu_seqlens || !g.mask || !g.depths) return QF_ERR_INVALID;
+    if (g.num_seqs > INT32_MAX || g.num_nodes > INT32_MAX || g.max_tree > INT32_MAX ||
+        g.mask_words > INT32_MAX)
         return QF_ERR_UNSUPPORTED;
-    return qf::launch_pdl(qf::build_tree_mask_kernel, dim3((unsigned)num_seqs), 128, 0, stream, parents,
-                          index_type, cu_seqlens, (int)num_seqs, (int)num_nodes, (int)max_tree,
-                          (int)mask_words, mask, depths, status);
+    return qf::launch_pdl(qf::build_tree_mask_kernel, dim3((unsigned)g.num_seqs), 128, 0, stream, g.parents,
+                          g.index_type, g.cu_seqlens, (int)g.num_seqs, (int)g.num_nodes, (int)g.max_tree,
+                          (int)g.mask_words, g.mask, g.depths, g.status);
 }
+
+extern "C" size_t qf_tree_mask_args_size(void) { return sizeof(qf_tree_mask_args); }

@@ -21,8 +21,7 @@ from __future__ import annotations
 import torch
 
 from .. import _capi
-from .._runtime import (after_op, dtype_tag, index_tag, on_device, require_cuda, status_word,
-                        stream_ptr)
+from .._runtime import after_launch, device_index, dtype_tag, index_tag, launch, status_ptr
 from .tree import attend, check_quantized_cache
 
 __all__ = ["load_kv_cache_quantized", "paged_attention_quantized", "store_kv_cache_quantized"]
@@ -70,17 +69,16 @@ def store_kv_cache_quantized(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: 
     if bm.numel() != T:
         raise ValueError(f"{what}: {bm.numel()} places for {T} tokens")
     tag = dtype_tag(k_src, what)
-    dev = require_cuda(what, k_src, v_src, k_cache, v_cache, k_scale, v_scale, bm, sm)
-    i64 = _capi.strides_array
-    with on_device(dev):
-        rc = _capi.lib().qf_kv_store_quantized(
-            k_src.data_ptr(), i64(k_src.stride()), v_src.data_ptr(), i64(v_src.stride()),
-            k_cache.data_ptr(), i64(k_cache.stride()), v_cache.data_ptr(), i64(v_cache.stride()),
-            k_scale.data_ptr(), i64(k_scale.stride()), v_scale.data_ptr(), i64(v_scale.stride()),
-            bm.data_ptr(), sm.data_ptr(), itag, T, H, D, k_cache.shape[0], k_cache.shape[2], tag,
-            fmt, status_word(dev).data_ptr(), stream_ptr(dev))
-    _capi.check(rc, what)
-    after_op(dev)
+    dev = device_index(what, k_src, v_src, k_cache, v_cache, k_scale, v_scale, bm, sm)
+    N, _, B, _ = k_cache.shape
+    rc = launch(dev, _capi.lib().qf_kv_store_quantized, _capi.KvQuantizedArgs.pack(
+        k_src.data_ptr(), *k_src.stride(), v_src.data_ptr(), *v_src.stride(),
+        k_cache.data_ptr(), *k_cache.stride(), v_cache.data_ptr(), *v_cache.stride(),
+        k_scale.data_ptr(), *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride(),
+        bm.data_ptr(), sm.data_ptr(), T, H, D, N, B, itag, tag, fmt, status_ptr(dev)))
+    if rc:
+        _capi.check(rc, what)
+    after_launch(dev)
 
 
 def load_kv_cache_quantized(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -98,19 +96,18 @@ def load_kv_cache_quantized(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scal
     bm, sm, itag = _mappings(what, block_mapping, slot_mapping)
     N, H, B, D = k_cache.shape
     T = bm.numel()
-    dev = require_cuda(what, k_cache, v_cache, k_scale, v_scale, bm, sm)
-    k, v = torch.empty((2, T, H, D), dtype=dtype, device=dev).transpose(1, 2).unbind(0)
+    dev = device_index(what, k_cache, v_cache, k_scale, v_scale, bm, sm)
+    k = torch.empty_strided((H, T, D), (D, H * D, 1), dtype=dtype, device=k_cache.device)
+    v = torch.empty_strided((H, T, D), (D, H * D, 1), dtype=dtype, device=k_cache.device)
     tag = dtype_tag(k, what)
-    i64 = _capi.strides_array
-    rows = i64((D, H * D, 1))
-    with on_device(dev):
-        rc = _capi.lib().qf_kv_load_quantized(
-            k_cache.data_ptr(), i64(k_cache.stride()), v_cache.data_ptr(), i64(v_cache.stride()),
-            k_scale.data_ptr(), i64(k_scale.stride()), v_scale.data_ptr(), i64(v_scale.stride()),
-            bm.data_ptr(), sm.data_ptr(), itag, k.data_ptr(), rows, v.data_ptr(), rows, T, H, D, N,
-            B, tag, fmt, status_word(dev).data_ptr(), stream_ptr(dev))
-    _capi.check(rc, what)
-    after_op(dev)
+    rc = launch(dev, _capi.lib().qf_kv_load_quantized, _capi.KvQuantizedArgs.pack(
+        k.data_ptr(), D, H * D, 1, v.data_ptr(), D, H * D, 1,
+        k_cache.data_ptr(), *k_cache.stride(), v_cache.data_ptr(), *v_cache.stride(),
+        k_scale.data_ptr(), *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride(),
+        bm.data_ptr(), sm.data_ptr(), T, H, D, N, B, itag, tag, fmt, status_ptr(dev)))
+    if rc:
+        _capi.check(rc, what)
+    after_launch(dev)
     return k, v
 
 

@@ -24,8 +24,7 @@ import math
 import torch
 
 from .. import _capi
-from .._runtime import (after_op, dtype_tag, index_tag, on_device, require_cuda, status_word,
-                        stream_ptr)
+from .._runtime import (after_launch, device_index, dtype_tag, index_tag, launch, status_ptr)
 
 __all__ = ["build_tree_mask", "paged_tree_attention", "paged_tree_attention_workspace_bytes"]
 
@@ -63,21 +62,21 @@ def build_tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor,
         raise ValueError(f"max_tree must be >= 1, got {max_tree}")
     itag = index_tag(parents, "build_tree_mask parents")
     index_tag(cu_seqlens, "build_tree_mask cu_seqlens")
-    dev = require_cuda("build_tree_mask", parents, cu_seqlens)
+    dev = device_index("build_tree_mask", parents, cu_seqlens)
     if not parents.is_contiguous():
         parents = parents.contiguous()
     cu = _int32(cu_seqlens)
-    n, words = parents.numel(), (max_tree + 63) // 64
-    if n and cu.numel() < 2:
+    n, words, seqs = parents.numel(), (max_tree + 63) // 64, cu.numel() - 1
+    if n and seqs < 1:
         raise ValueError(f"build_tree_mask: {n} nodes but no sequence")
-    mask = torch.empty(n, words, dtype=torch.int64, device=dev)
-    depths = torch.empty(n, dtype=torch.int32, device=dev)
-    with on_device(dev):
-        rc = _capi.lib().qf_build_tree_mask(
-            parents.data_ptr(), itag, cu.data_ptr(), cu.numel() - 1, n, max_tree, words,
-            mask.data_ptr(), depths.data_ptr(), status_word(dev).data_ptr(), stream_ptr(dev))
-    _capi.check(rc, "build_tree_mask")
-    after_op(dev)
+    mask = torch.empty((n, words), dtype=torch.int64, device=parents.device)
+    depths = torch.empty((n,), dtype=torch.int32, device=parents.device)
+    rc = launch(dev, _capi.lib().qf_build_tree_mask, _capi.TreeMaskArgs.pack(
+        parents.data_ptr(), cu.data_ptr(), seqs, n, max_tree, words, mask.data_ptr(),
+        depths.data_ptr(), itag, status_ptr(dev)))
+    if rc:
+        _capi.check(rc, "build_tree_mask")
+    after_launch(dev)
     return mask, depths
 
 
@@ -85,13 +84,12 @@ def build_tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor,
 def _workspace_bytes(num_tokens: int, num_seqs: int, max_tree: int, num_q_heads: int,
                      num_kv_heads: int, head_dim: int, block_size: int, max_blocks_per_seq: int,
                      tag: int, fmt: int, decode: bool) -> int:
-    a = _capi.PagedTreeAttentionArgs()
-    a.cu_seqlens_q = None if decode else 1  # (whether there is one is all that is read)
-    a.num_tokens, a.num_seqs, a.max_tree = num_tokens, num_seqs, max_tree
-    a.num_q_heads, a.num_kv_heads, a.head_dim = num_q_heads, num_kv_heads, head_dim
-    a.block_size, a.max_blocks_per_seq = block_size, max_blocks_per_seq
-    a.dtype, a.cache_format = tag, fmt
-    return int(_capi.lib().qf_paged_tree_attention_workspace_bytes(a))
+    return int(_capi.lib().qf_paged_tree_attention_workspace_bytes(
+        _capi.PagedTreeAttentionArgs.named(
+            cu_seqlens_q=0 if decode else 1,  # (whether there is one is all that is read)
+            num_tokens=num_tokens, num_seqs=num_seqs, max_tree=max_tree, num_q_heads=num_q_heads,
+            num_kv_heads=num_kv_heads, head_dim=head_dim, block_size=block_size,
+            max_blocks_per_seq=max_blocks_per_seq, dtype=tag, cache_format=fmt)))
 
 
 def paged_tree_attention_workspace_bytes(num_tokens: int, num_seqs: int, max_tree: int,
@@ -167,55 +165,53 @@ def attend(what: str, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         raise ValueError(f"{what}: block_tables must be (num_seqs, max_blocks) and the lengths "
                          f"(num_seqs,), got {tuple(block_tables.shape)} and {tuple(lens.shape)}")
     tag = dtype_tag(query, what)
-    dev = require_cuda(what, query, k_cache, v_cache, block_tables, lens, k_scale, v_scale,
+    dev = device_index(what, query, k_cache, v_cache, block_tables, lens, k_scale, v_scale,
                        cu_seqlens, tree_mask, workspace)
     q = query
     es = q.element_size()
     sq = q.stride()
     if sq[2] != 1 or (sq[0] * es) % 16 or (sq[1] * es) % 16 or q.data_ptr() % 16:
-        q = torch.empty(q.shape, dtype=q.dtype, device=dev).copy_(q)  # the kernels' alignment
+        q = torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q)  # the kernels' alignment
         sq = q.stride()
     bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
-    if bt.shape[1] > 1 and bt.stride(1) != 1:
+    max_blocks = bt.shape[1]
+    if max_blocks > 1 and bt.stride(1) != 1:
         bt = bt.contiguous()
     lens = _int32(lens)
-    out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     cu = mask = None
+    words = 0
     if cu_seqlens is not None:
         cu = _int32(cu_seqlens)
         mask = tree_mask if tree_mask.is_contiguous() else tree_mask.contiguous()
-    arr = _capi.strides_array
+        words = mask.shape[1]
+    space = 0
+    if split:
+        if workspace is None:
+            space = _workspace_bytes(T, S, max_tree, Hq, Hkv, D, B, max_blocks, tag, fmt, cu is None)
+            if space:
+                workspace = torch.empty(space // 4, dtype=torch.float32, device=q.device)
+        else:
+            space = workspace.numel() * workspace.element_size()
     scaled = k_scale is not None
-    # positional, in the struct's order: a third of the time of 40 assignments
-    a = _capi.PagedTreeAttentionArgs(
+    rc = launch(dev, _capi.lib().qf_paged_tree_attention, _capi.PagedTreeAttentionArgs.pack(
         q.data_ptr(), sq[0], sq[1],
-        k_cache.data_ptr(), v_cache.data_ptr(), arr(strides),
-        k_scale.data_ptr() if scaled else None, v_scale.data_ptr() if scaled else None,
-        arr(k_scale.stride() if scaled else (0, 0, 0)),
+        k_cache.data_ptr(), v_cache.data_ptr(), *strides,
+        k_scale.data_ptr() if scaled else 0, v_scale.data_ptr() if scaled else 0,
+        *(k_scale.stride() if scaled else (0, 0, 0)),
         N, B,
-        bt.data_ptr(), bt.stride(0), bt.shape[1],
-        lens.data_ptr(), cu.data_ptr() if cu is not None else None,
-        mask.data_ptr() if mask is not None else None, mask.shape[1] if mask is not None else 0,
+        bt.data_ptr(), bt.stride(0), max_blocks,
+        lens.data_ptr(), 0 if cu is None else cu.data_ptr(),
+        0 if mask is None else mask.data_ptr(), words,
         S, T, max_tree, Hq, Hkv, D,
         1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale),
         out.data_ptr(), Hq * D, D,
-        None, 0,
+        workspace.data_ptr() if space else 0, space,
         tag, fmt,
-        status_word(dev).data_ptr())
-    lib = _capi.lib()
-    with on_device(dev):
-        if split:
-            if workspace is None:
-                need = _workspace_bytes(T, S, max_tree, Hq, Hkv, D, B, bt.shape[1], tag, fmt,
-                                        cu is None)
-                if need:
-                    workspace = torch.empty(need // 4, dtype=torch.float32, device=dev)
-            if workspace is not None:
-                a.workspace = workspace.data_ptr()
-                a.workspace_bytes = workspace.numel() * workspace.element_size()
-        rc = lib.qf_paged_tree_attention(a, stream_ptr(dev))
-    _capi.check(rc, what)
-    after_op(dev)
+        status_ptr(dev)))
+    if rc:
+        _capi.check(rc, what)
+    after_launch(dev)
     return out
 
 
