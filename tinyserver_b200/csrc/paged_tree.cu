@@ -23,6 +23,11 @@ namespace qf {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// Rows per kv head that the mma.sync kernel takes at head_dim 128 (it reads the cache
+// once per 16 of them, the tcgen05 kernel once per 256).  32 trees at 4096 context
+// keys, 8 kv heads, mma.sync | tcgen05: bf16, 8 rows 105 | 109 us, 16 rows 110 | 110 us,
+// 24 rows 188 | 111 us; e4m3, 16 rows 100 | 167 us, 24 rows 169 | 169 us, 64 rows 323 |
+// 154 us; 2 trees at 700 keys, bf16, 16 rows 16.2 | 17.3 us, 24 rows 19.5 | 17.2 us.
 constexpr int kMmaRows = 16;
 constexpr int kF32Keys = 64;  // keys of a work unit of the fp32 kernel
 
@@ -416,7 +421,11 @@ struct TreePlan {
 // The kernel and its grid, by sizes alone (lengths are on the device; the block
 // tables bound them).  A cut costs a partial of (D + 2) floats a row, written and
 // read back, so a CTA's stretch is at least two blocks of 128 keys, or four of 64;
-// and a second launch, so sequences of up to 768 keys (256 of the mma.sync kernel's) stay whole.
+// and a second launch, so sequences of up to 768 keys (256 of the mma.sync kernel's)
+// stay whole.  Whole | cut: a tree of 16 nodes x 4 heads, 8 kv heads, at 500 keys 15.3 |
+// 16.9 us, at 1000 18.3 | 17.1, at 2000 26.7 | 18.7; 8 of them at 500 keys 16.4 | 22.9;
+// decode of 4 sequences over e4m3 at 200 keys 9.0 | 10.1 us, at 500 13.6 | 11.4, at 1000
+// 23.7 | 13.6.
 TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     TreePlan p{};
     const int64_t G = g.num_q_heads / g.num_kv_heads, rows = (g.cu_seqlens_q ? g.max_tree : 1) * G;
@@ -429,7 +438,7 @@ TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     } else if (g.head_dim == 128 && rows > kMmaRows) {
         p.tiles = rows > 128 ? 2 : 1;
         p.rows = 128 * p.tiles;
-        per_sm = p.tiles == 1 ? 2 : 1;
+        per_sm = 1;
         keys = 128;
         p.min_units = 2;
     } else {

@@ -1,30 +1,43 @@
 // Paged attention for many query rows per kv head (a tree's tokens x G), 16-bit
 // queries, head_dim 128, on the 5th-generation tensor cores.
 //
-// A CTA takes NT tiles of 128 rows of one (sequence, kv head) and a partition of
+// A CTA takes NT tiles of 128 rows of one (sequence, kv head) and a stretch of
 // the keys in blocks of 128.  Both products run on tcgen05.mma with S, P and O in
 // tensor memory, P over the S it came from:
-//   S_t = Q_t K_j^T     Q, K in shared memory (128-byte swizzle)
-//   softmax of row r by thread r of the tile's warpgroup, whose tensor-memory
-//   lane the row is; P_t back over the first half of S_t
-//   O_t += P_t V_j      A = P_t from tensor memory, V in shared memory
+//   S_t = Q K_j^T     Q, K in shared memory (128-byte swizzle)
+//   softmax of row r by thread r of warpgroup t, whose tensor-memory lane the row
+//   is; P_t back over the first half of S_t
+//   O_t += P_t V_j    A = P_t from tensor memory, V in shared memory
+// There are two S, two O and two softmax warpgroups.  NT = 2 (more than 128 rows):
+// warpgroup t has tile t; K and V meet 256 rows, and tile 0's softmax overlaps tile
+// 1's products.  NT = 1: the warpgroups take turns at the one tile's blocks, each
+// with a maximum, a sum and an O of its own, which the end of the item joins; so one
+// block's products and copies overlap the softmax of the block before.
 // P goes back by halves of a block: the first half's products run during the
 // second's softmax.  (Scores by halves too, taking turns in S_t, overlap better on
 // paper, but 64 columns cost the tensor core as much as 128: 511 cycles for a tile's
 // eight steps against 515.)
-// Roles: 4 NT softmax warps, one MMA thread, a warp that brings K and one that
-// brings V.  16-bit pages come by TMA, one box per lane, where a block's keys are
-// all context; else (the drafted keys, the tail, pages whose size is no multiple of
-// 8) row by row with cp.async.  8-bit rows land in half of their tile and are
-// converted to fp16 (exact) in place.
+// Roles: 8 softmax warps, one MMA thread, and loaders: one warp each for K and V, or
+// two (NT = 1), every other block one's.  16-bit pages come by TMA, one box per
+// lane, where a block's keys are all context; else (the drafted keys, the tail, pages
+// whose size is no multiple of 8) row by row with cp.async.  8-bit rows land in half
+// of their tile and are converted to fp16 (exact) in place.
 //
-// What bounds it: a block is 64 KB of 16-bit K and V, ~2900 cycles of an SM's
+// What bounds it: a block is 64 KB of 16-bit K and V, ~2800 cycles of an SM's
 // share of HBM; a tile's softmax is 16384 exponentials, 1024 cycles of the MUFU,
-// and its products 1024 cycles of the tensor core.  One tile (up to 128 rows):
-// bound by HBM if something is always in flight, hence two CTAs per SM, each with
-// one K and one V buffer that refill while the other product and the softmax run.
-// Two tiles (more rows): one CTA per SM with two-deep rings; K and V meet 256 rows,
-// and tile 0's softmax overlaps tile 1's products.
+// and its products 1024 cycles of the tensor core.
+//  * Up to 128 rows, 16-bit rows: by HBM's latency, with 128 KB of K and V stages per
+//    SM: 32 trees of 16 nodes x 4 heads at 4096 context keys, 8 kv heads: 113 us, 4.85
+//    TB/s (two CTAs per SM with one stage each and halves of a block in turn: 127 us).
+//  * 8-bit rows: by the softmax warps' dependent instructions (two warps per scheduler;
+//    36% of the issue slots used): a half block takes 2300 cycles, against 1100 over
+//    16-bit rows, for the scales' loads and products.  The same trees over e4m3: 154 us
+//    (182 us); 32 trees of 32 nodes at up to 8191 context keys: 220 us.
+//  * More than 128 rows: by the chain of products and softmax, ~4100 cycles a block of
+//    two tiles; 64 trees of 64 nodes x 4 heads at up to 8191 context keys: 350 us, 870
+//    TFLOP/s (as single tiles, which read K and V twice: 445 us).
+// Registers moved from the loaders to the softmax (88 and 168 a thread instead of 128)
+// cost more in the loaders than they gained: 154 -> 206 us.
 //
 // Quantised rows: the codes go into the products as they are.  K's scale multiplies
 // the score, V's (times 2^x, x of the segment's first block) the probability before
@@ -51,31 +64,45 @@ namespace {
 
 constexpr int kD = 128;
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kItemBlocks = 4;      // what beginning and ending an item costs, in blocks
+// What beginning and ending an item costs, in blocks.  64 trees of 64, 16 of 16 over
+// 16-bit rows, 32 of 32 over e4m3: 347, 48.7, 214 us; with 2: 370, 53.5, 234; 8: 357, 51.9, 213.
+constexpr int kItemBlocks = 4;
 constexpr float kKeepLog2 = 8.f;    // the reference maximum moves when the row's has grown by 2^8
 constexpr float kScaleLog2 = 6.f;   // log2 of the v-scales (times 2^x) that a probability is multiplied by
 
 
 template <int NT>
 struct TreeTc {
-    static constexpr int ST = NT;                   // K and V stages
-    static constexpr int SOFT = 128 * NT;           // softmax threads
-    static constexpr int MMA_WARP = 4 * NT, LOAD_WARP = MMA_WARP + 1;  // K, then V
-    static constexpr int THREADS = SOFT + 32 + 64;
-    static constexpr int SLOTS = 2 * ST;            // blocks whose scales and valid bits are kept
+    static constexpr int ST = 2;              // K and V stages
+    static constexpr int LW = NT == 1 ? 2 : 1;  // loader warps of K, and of V: block n is warp n % LW's
+    static constexpr int SOFT = 256;          // softmax threads
+    static constexpr int MMA_WARP = 8, LOAD_WARP = 9;  // K's, then V's
+    static constexpr int THREADS = SOFT + 32 + 64 * LW;
+    static constexpr int SLOTS = 2 * ST;      // blocks whose scales and valid bits are kept
     static constexpr int SMEM = (NT + 2 * ST) * kTile + 1024;
-    static constexpr uint32_t COLS = 256 * NT;      // tensor memory: S_t at 128 t, O_t behind them
 };
+constexpr uint32_t kCols = 512;  // tensor memory: S_t at 128 t, O_t at 256 + 128 t
 
-template <int NT>
 struct TreeBars {
     uint64_t q_full;
-    uint64_t k_full[NT], v_full[NT], k_empty[NT], v_empty[NT];
-    uint64_t info_full[2 * NT];  // a block's valid bits and scales
-    uint64_t s_full[NT], p_full[NT][2];  // P by halves of a block
-    uint64_t pv_done[NT], o_full, drain;
-    uint64_t raw[2];  // a K, a V tile that its loader still works on has landed
+    uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];
+    uint64_t info_full[4];  // a block's valid bits and scales
+    uint64_t s_full[2], p_full[2][2];  // P by halves of a block
+    uint64_t pv_done[2], o_full, drain;
+    uint64_t raw[4];  // a tile that its loader still works on has landed
 };
+
+// By the softmax warps, all together: whether `ok` holds in every thread.
+__device__ __forceinline__ bool soft_all(bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)ok)
+        : "memory");
+    return all != 0;
+}
 
 __device__ __forceinline__ void proxy_fence() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -196,18 +223,18 @@ __device__ float dot_row(const T* q, const char* k) {
 // A drafted block's V held an infinity or a NaN, which went into the product as
 // zero so that rows that do not see the key stay clean: the rows that do see it
 // get p * v added to what they wrote (the sum is an infinity or a NaN whatever the
-// finite part was).  Keys [j0, k_end), one row per thread.
+// finite part was).  Keys [j0, k_end), one row per thread, its columns [d0, d1).
 template <typename T, int FMT, typename O>
 __device__ __noinline__ void add_not_finite(const TreeDev& a, const int32_t* bt, int g, int ctx,
                                             const int64_t* mrow, const T* q, float sl2, float mref,
-                                            int j0, int k_end, O* out) {
+                                            int j0, int k_end, int d0, int d1, O* out) {
     for (int j = j0; j < k_end; ++j) {
         if (!((tree_bits32(mrow, a.words, j - ctx)) & 1u)) continue;
         int64_t row, srow;
         if (!key_place(a, bt, g, j, row, srow)) continue;
         float p = -1.f;
 #pragma unroll 1
-        for (int d = 0; d < kD; ++d) {
+        for (int d = d0; d < d1; ++d) {
             float v;
             if constexpr (FMT == QF_CACHE_PLAIN) v = Dt<T>::to_f(reinterpret_cast<const T*>(a.vc)[row + d]);
             else v = code_to_float<FMT>(reinterpret_cast<const uint8_t*>(a.vc)[row + d]);
@@ -270,19 +297,21 @@ __device__ __forceinline__ void issue_scores(uint32_t d, uint32_t q, uint32_t k,
 }
 
 template <typename T, int FMT, int NT>
-__global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
     tree_tc_kernel(const TreeDev a, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv, int box) {
     using C = TreeTc<NT>;
     constexpr bool Q8 = FMT != QF_CACHE_PLAIN;
     using MT = typename std::conditional<Q8, __half, T>::type;
     using MP = Packed<MT>;
-    constexpr int ST = C::ST;
+    constexpr int ST = C::ST, LW = C::LW;
+    constexpr bool TURNS = NT == 1;  // the warpgroups take turns at one tile's blocks
+    constexpr int STEP = TURNS ? 2 : 1;  // between a warpgroup's blocks
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     extern __shared__ __align__(1024) char dsm[];
-    __shared__ TreeBars<NT> bars;
+    __shared__ TreeBars bars;
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, odd_v;  // odd_v: the last segment whose drafted V was not finite, from 1
     __shared__ int scratch[34];
@@ -292,6 +321,8 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     __shared__ __align__(16) float sk[Q8 ? C::SLOTS : 1][Q8 ? kRows : 4], sv[Q8 ? C::SLOTS : 1][Q8 ? kRows : 4],
         sl[Q8 ? C::SLOTS : 1][Q8 ? kRows : 4];
     __shared__ int snear[C::SLOTS], sexp[C::SLOTS];
+    __shared__ float stat[TURNS ? 3 : 1][TURNS ? 256 : 1];  // m, l, 2^-x of the softmax threads
+    __shared__ uint32_t qtop[TURNS && Q8 ? 256 : 1];        // largest magnitude in a row of Q's slab
     volatile int* abort = &abort_flag;
 
     const uint32_t raw = smem_u32(dsm);
@@ -299,7 +330,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     char* const kbase = base + NT * kTile;
     char* const vbase = kbase + ST * kTile;
     if (tid == 0) {
-        mbar_init(&bars.q_full, kRows * NT);
+        mbar_init(&bars.q_full, C::SOFT);
         for (int i = 0; i < ST; ++i) {
             mbar_init(&bars.k_full[i], 32);
             mbar_init(&bars.v_full[i], 32);
@@ -307,15 +338,14 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             mbar_init(&bars.v_empty[i], 1);
         }
         for (int i = 0; i < C::SLOTS; ++i) mbar_init(&bars.info_full[i], 32);
-        for (int t = 0; t < NT; ++t) {
+        for (int t = 0; t < 2; ++t) {
             mbar_init(&bars.s_full[t], 1);
             for (int h = 0; h < 2; ++h) mbar_init(&bars.p_full[t][h], kRows);
             mbar_init(&bars.pv_done[t], 1);
         }
         mbar_init(&bars.o_full, 1);
         mbar_init(&bars.drain, 1);
-        mbar_init(&bars.raw[0], 1);
-        mbar_init(&bars.raw[1], 1);
+        for (int i = 0; i < 2 * LW; ++i) mbar_init(&bars.raw[i], 1);
         abort_flag = 0;
         odd_v = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -323,7 +353,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     if (warp == C::MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(&tmem_slot)),
-                     "r"(C::COLS)
+                     "r"(kCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -350,8 +380,8 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     auto draft_of = [&](int nblk) { return a.cu ? max(0, (sg.w.ctx - sg.k_begin) / kRows) : nblk; };
 
     if (warp >= C::LOAD_WARP) {
-        // ---- loaders: one warp K, one warp V
-        const int side = warp - C::LOAD_WARP;
+        // ---- loaders: K's warps, then V's; every LW-th block of all segments is one's
+        const int side = (warp - C::LOAD_WARP) / LW, turn = (warp - C::LOAD_WARP) % LW;
         const char* src = side ? a.vc : a.kc;
         char* const tiles = side ? vbase : kbase;
         uint64_t* full = side ? bars.v_full : bars.k_full;
@@ -447,7 +477,9 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         const int hi = lane >> 4, c = lane & 15;
         // this lane's piece of a block: `box` slots of one page, 64 dims of them or all codes
         const int pc = Q8 ? lane : lane >> 1;
-        int n = 0, raw = 0;  // blocks, worked-on tiles of all segments
+        int n0 = 0, last = -1;  // the segment's first block of all segments', and the last one begun here
+        int raw = 0;            // tiles worked on
+        uint64_t* const landed = &bars.raw[warp - C::LOAD_WARP];
         int blk = 0, slot0 = 0;
         auto look = [&](int j) {  // the page and first slot of this lane's piece of block j
             const int kb = sg.k_begin + j * kRows;
@@ -460,15 +492,16 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             ++seq_no;
             bt = a.bt + (int64_t)sg.s * a.bts;
             const int nblk = blocks_of(), k_end = sg.k_end;
-            if (box > 0 && nblk > 0) {
-                look(0);
+            const int j0 = LW == 1 ? 0 : (turn + n0) & 1;
+            if (box > 0 && j0 < nblk) {
+                look(j0);
                 if (Q8 && side == 0) {
-                    look_scales(0);
-                    load_scales(0);
+                    look_scales(j0);
+                    load_scales(j0);
                 }
             }
-            for (int j = 0; j < nblk; ++j, ++n) {
-                const int st = n % ST, kb = sg.k_begin + j * kRows, nk = min(kRows, k_end - kb);
+            for (int j = j0; j < nblk; j += LW) {
+                const int n = n0 + j, st = n % ST, kb = sg.k_begin + j * kRows, nk = min(kRows, k_end - kb);
                 char* tile = tiles + st * kTile;
                 // rows of V that some query row may not see
                 const int d0 = a.cu ? max(0, sg.w.ctx - kb) : kRows;
@@ -480,11 +513,12 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                     go = false;
                     break;
                 }
+                last = n;
                 // whether this warp works on the tile before the tensor core may have it
                 const bool work = Q8 || (side == 1 && (nk < kRows || d0 < nk));
                 if (bulk) {
                     // (K behind the last key may hold anything: those columns are masked)
-                    uint64_t* bar = work ? &bars.raw[side] : &full[st];
+                    uint64_t* bar = work ? landed : &full[st];
                     const uint32_t bytes = (uint32_t)((nk + box - 1) / box * box) * (Q8 ? 128u : 256u);
                     if (lane == 0) mbar_expect_tx(bar, bytes);
                     else if (!work) mbar_arrive(bar);
@@ -496,13 +530,13 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                             tma_page(tile + (lane & 1) * kSlab + pc * box * 128, map, (lane & 1) * 64, slot0, sg.g, blk,
                                      bar);
                     }
-                    if (j + 1 < nblk) look(j + 1);
+                    if (j + LW < nblk) look(j + LW);
                     if (side == 0) {  // meanwhile, what the softmax needs to know
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
                             ok[x] = nk >= 32 * (x + 1) ? kFull : nk > 32 * x ? (1u << (nk - 32 * x)) - 1u : 0u;
-                        inform(n % C::SLOTS, j == 0);
-                        if (Q8 && j + 1 < nblk) look_scales(j + 1);
+                        inform(n % C::SLOTS, j == j0);
+                        if (Q8 && j + LW < nblk) look_scales(j + LW);
                     }
                     if (!work) continue;
                     if (!__all_sync(kFull, mbar_wait(bar, raw++ & 1, nullptr))) {
@@ -513,9 +547,9 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                         for (int r = nk + hi; r < kRows; r += 2)
                             *reinterpret_cast<uint4*>(tile + tile_off(r, c)) = make_uint4(0, 0, 0, 0);
                 } else if constexpr (Q8) {  // row by row, 16 codes a lane
-                    if (box > 0 && j + 1 < nblk) {
-                        look(j + 1);
-                        if (side == 0) look_scales(j + 1);
+                    if (box > 0 && j + LW < nblk) {
+                        look(j + LW);
+                        if (side == 0) look_scales(j + LW);
                     }
                     const uint32_t dst = smem_u32(tile) + (uint32_t)(kSlab + (lane >> 3) * 128 + (lane & 7) * 16);
 #pragma unroll
@@ -528,11 +562,11 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                                           (ok[x] >> r) & 1 ? 16 : 0);
                         }
                     cp_async_commit();
-                    if (side == 0) inform(n % C::SLOTS, j == 0);
+                    if (side == 0) inform(n % C::SLOTS, j == j0);
                     cp_async_wait<0>();
                     __syncwarp();
                 } else {  // chunk c of rows 2 i + hi; the swizzle repeats every four i
-                    if (box > 0 && j + 1 < nblk) look(j + 1);
+                    if (box > 0 && j + LW < nblk) look(j + LW);
                     const uint32_t dst = smem_u32(tile) + (uint32_t)((c >> 3) * kSlab + hi * 128);
                     const char* from = src + c * 16;
 #pragma unroll
@@ -545,23 +579,25 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
                         }
                     }
                     cp_async_commit();
-                    if (side == 0) inform(n % C::SLOTS, j == 0);
+                    if (side == 0) inform(n % C::SLOTS, j == j0);
                     cp_async_wait<0>();
                     __syncwarp();
                 }
                 if constexpr (Q8) {
                     if (side == 0 || (nk == kRows && d0 >= kRows)) expand<FMT, false>(tile, nk, d0, lane);
-                    else if (expand<FMT, true>(tile, nk, d0, lane)) odd_v = seq_no;
+                    else if (expand<FMT, true>(tile, nk, d0, lane)) atomicMax(&odd_v, seq_no);
                 } else {
-                    if (work && d0 < nk && clean_rows<MT>(tile, d0, nk, lane)) odd_v = seq_no;
+                    if (work && d0 < nk && clean_rows<MT>(tile, d0, nk, lane)) atomicMax(&odd_v, seq_no);
                 }
                 proxy_fence();
                 mbar_arrive(&full[st]);
-                if (Q8 && side == 0 && box > 0 && j + 1 < nblk) load_scales(j + 1);
+                if (Q8 && side == 0 && box > 0 && j + LW < nblk) load_scales(j + LW);
             }
+            n0 += nblk;
         }
         // every copy issued has landed before the CTA can leave
-        for (int d = max(0, n - ST); d < n; ++d) mbar_wait(&full[d % ST], (d / ST) & 1, nullptr);
+        for (int d = last - (ST - LW); d <= last; d += LW)
+            if (d >= 0) mbar_wait(&full[d % ST], (d / ST) & 1, nullptr);
     } else if (warp == C::MMA_WARP) {
         // ---- MMA issue, the warp together and one lane for it: S_t,0 | PV_t,j by the two
         // halves of P, S_t,j+1 | ...
@@ -575,51 +611,54 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             tc_fence_after();
         };
         uint32_t n = 0, seg = 0;  // blocks, segments with keys so far
-        uint32_t uses[NT] = {};   // blocks of each tile so far
+        uint32_t uses[2] = {};    // blocks of each tile so far (turns: n / 2)
         while (go && walk.next(a, sg)) {
-            const int nblk = blocks_of(), ntile = tiles_of();
+            const int nblk = blocks_of(), ntile = TURNS ? 1 : tiles_of();
             if (nblk == 0) continue;
             wait(&bars.q_full, seg);
-            wait(&bars.k_full[n % ST], n / ST);
-            if (!go) break;
-            // scores of block bn; K's stage is free once the last tile's have been issued
+            // scores of block bn into S_t; K's stage is free once the last tile's have been issued
             auto scores = [&](uint32_t bn, int t) {
+                if (TURNS || t == 0) wait(&bars.k_full[bn % ST], bn / ST);
+                if (!go) return;
                 if (elect_one()) {
-                    issue_scores(tmem + (uint32_t)(t * kRows), qa + t * (kTile >> 4), ka + (bn % ST) * (kTile >> 4), id_qk);
+                    issue_scores(tmem + (uint32_t)(t * kRows), qa + (TURNS ? 0 : t * (kTile >> 4)),
+                                 ka + (bn % ST) * (kTile >> 4), id_qk);
                     mma_commit(&bars.s_full[t]);
-                    if (t == ntile - 1) mma_commit(&bars.k_empty[bn % ST]);
+                    if (TURNS || t == ntile - 1) mma_commit(&bars.k_empty[bn % ST]);
                 }
                 __syncwarp();
             };
-            for (int t = 0; t < ntile; ++t) scores(n, t);
+            if constexpr (TURNS) {
+                scores(n, (int)(n & 1));
+                if (nblk > 1) scores(n + 1, (int)(~n & 1));
+            } else {
+                for (int t = 0; t < ntile; ++t) scores(n, t);
+            }
             for (int j = 0; go && j < nblk; ++j, ++n) {
                 const uint32_t st = n % ST;
                 wait(&bars.v_full[st], n / ST);
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if (!go || t >= ntile) break;
+                for (int i = 0; i < NT; ++i) {
+                    if (!go || i >= ntile) break;
+                    const int t = TURNS ? (int)(n & 1) : i;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        wait(&bars.p_full[t][h], uses[t] + (uint32_t)j);
+                        wait(&bars.p_full[t][h], TURNS ? n >> 1 : uses[i] + (uint32_t)j);
                         if (!go) break;
                         if (elect_one()) {
-                            const uint32_t o = tmem + (uint32_t)((NT + t) * kRows);
+                            const uint32_t o = tmem + (uint32_t)((2 + t) * kRows);
                             const uint32_t pt = tmem + (uint32_t)(t * kRows + h * 64);
                             const uint32_t v = va + st * (kTile >> 4) + h * (8192 >> 4);
 #pragma unroll
                             for (int k = 0; k < 4; ++k)  // keys in steps of 16
                                 mma_ts(o, pt + 8u * k, desc_of(v + k * (2048 >> 4)), id_pv,
-                                       (j > 0 || h > 0 || k > 0) ? 1u : 0u);
+                                       (j >= STEP || h > 0 || k > 0) ? 1u : 0u);
                             if (h == 0) mma_commit(&bars.pv_done[t]);
-                            else if (t == ntile - 1) mma_commit(&bars.v_empty[st]);
+                            else if (i == ntile - 1) mma_commit(&bars.v_empty[st]);
                         }
                         __syncwarp();
                     }
-                    if (go && j + 1 < nblk) {
-                        if (t == 0) wait(&bars.k_full[(n + 1) % ST], (n + 1) / ST);
-                        if (!go) break;
-                        scores(n + 1, t);
-                    }
+                    if (go && j + STEP < nblk) scores(n + STEP, t);
                 }
             }
             if (elect_one()) mma_commit(&bars.o_full);
@@ -633,7 +672,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         __syncwarp();
         mbar_wait(&bars.drain, 0, nullptr);
     } else {
-        // ---- softmax of tile t, one row per thread
+        // ---- softmax, one row per thread: warpgroup t has tile t, or every other block (S_t, O_t)
         const int t = warp >> 2, r = tid & (kRows - 1);
         bool got = true;
         uint32_t n0 = 0, seg = 0;                // blocks, segments with keys so far
@@ -641,10 +680,10 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         int seq_no = 0;                    // segments
         while (got && walk.next(a, sg)) {
         ++seq_no;
-        const int nblk = blocks_of(), ntile = tiles_of(), first_draft = draft_of(nblk);
+        const int nblk = blocks_of(), ntile = TURNS ? 2 : tiles_of(), first_draft = draft_of(nblk);
         const TreeSeq& w = sg.w;
         const int32_t* bt = a.bt + (int64_t)sg.s * a.bts;
-        const int rows = w.n * a.G, trow = sg.rg * NT * kRows + tid, k_begin = sg.k_begin, k_end = sg.k_end;
+        const int rows = w.n * a.G, trow = sg.rg * NT * kRows + (TURNS ? r : tid), k_begin = sg.k_begin, k_end = sg.k_end;
         const bool live = trow < rows;
         const int tok = live ? trow / a.G : 0;
         const int hq = sg.g * a.G + (live ? trow - tok * a.G : 0);
@@ -658,24 +697,29 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         }
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t sS = tmem + lanes + (uint32_t)(t * kRows);
-        const uint32_t sO = tmem + lanes + (uint32_t)((NT + t) * kRows);
+        const uint32_t sO = tmem + lanes + (uint32_t)((2 + t) * kRows);
+        const bool idle = !__any_sync(kFull, live);  // none of the warp's rows is one
         const T* qrow = reinterpret_cast<const T*>(a.q) + trow_q * a.qt + (int64_t)hq * a.qh;
         const int64_t* mrow = a.mask + trow_q * a.words;
         float rs = sl2;
-        char* const qtile = base + t * kTile;
+        char* const qtile = base + (TURNS ? 0 : t * kTile);
+        // the slabs of Q's tile that are this warpgroup's to fill and, at the end, to use for O
+        const int slab0 = TURNS ? t : 0, slab1 = TURNS ? t + 1 : 2;
+        const int hi = lane >> 3, c = lane & 7, w0 = (warp & 3) * 32;
         {
-            // The warp's 32 rows of Q, two at a time and whole (lane: chunk lane % 16 of row
-            // 2 i + lane / 16), into the tile.  (The segment before is done with Q: its O,
-            // which this thread has read, was final.)
+            // The warp's 32 rows of Q, four at a time (lane: chunk lane % 8 of a slab of row
+            // 4 i + lane / 8), into the tile.  (The segment before is done with Q: its O was
+            // final, and left through slabs of these rows that this warp alone fills.)
             using P = Packed<T>;
-            const int hi = lane >> 4, c = lane & 15, w0 = (warp & 3) * 32;
             const int64_t at = live ? trow_q * a.qt + (int64_t)hq * a.qh : -1;
+#pragma unroll 1
+            for (int sb = slab0; sb < slab1; ++sb)
 #pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-                const int64_t o = __shfl_sync(kFull, at, 2 * i + hi);
-                cp_async16_at(smem_u32(qtile) + tile_off(w0 + 2 * i + hi, c),
-                              reinterpret_cast<const T*>(a.q) + (o < 0 ? 0 : o) + 8 * c, o < 0 ? 0 : 16);
-            }
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t o = __shfl_sync(kFull, at, 4 * i + hi);
+                    cp_async16_at(smem_u32(qtile) + tile_off(w0 + 4 * i + hi, 8 * sb + c),
+                                  reinterpret_cast<const T*>(a.q) + (o < 0 ? 0 : o) + 64 * sb + 8 * c, o < 0 ? 0 : 16);
+                }
             cp_async_commit();
             cp_async_wait<0>();
             __syncwarp();
@@ -683,47 +727,71 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             const uint32_t flip = sl2 < 0.f ? 0x80008000u : 0u;
             rs = fabsf(sl2) < 1e-30f ? 1e-30f : fabsf(sl2);
             if (Q8 || flip) {
-                int er = 0;  // this thread's own row's exponent
+                // codes: a power-of-two factor brings the row's largest element to [2^14, 2^15)
+                int er = 14;  // this thread's own row's exponent
+                if constexpr (Q8) {
+                    uint32_t top = 0;
+#pragma unroll 1
+                    for (int sb = slab0; sb < slab1; ++sb)
 #pragma unroll 2
-                for (int i = 0; i < 16; ++i) {
-                    uint4* cell = reinterpret_cast<uint4*>(qtile + tile_off(w0 + 2 * i + hi, c));
-                    uint4 v = *cell;
-                    if constexpr (Q8) {  // a power-of-two factor brings the row's largest element to [2^14, 2^15)
-                        uint32_t mx = 0;
+                        for (int i = 0; i < 8; ++i) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(qtile + tile_off(w0 + 4 * i + hi, 8 * sb + c));
+                            uint32_t mx = 0;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            mx = max(mx, max(__float_as_uint(P::lo(word(v, x))) & 0x7fffffffu,
-                                             __float_as_uint(P::hi(word(v, x))) & 0x7fffffffu));
+                            for (int x = 0; x < 4; ++x)
+                                mx = max(mx, max(__float_as_uint(P::lo(word(v, x))) & 0x7fffffffu,
+                                                 __float_as_uint(P::hi(word(v, x))) & 0x7fffffffu));
 #pragma unroll
-                        for (int o = 8; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
-                        const int e = min(max((int)(mx >> 23) - 127, -100), 127);
-                        const float f = __int_as_float((127 + 14 - e) << 23);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            set_word(v, x, MP::pack(P::lo(word(v, x)) * f, P::hi(word(v, x)) * f));
-                        const int mine = __shfl_sync(kFull, e, (lane & 1) * 16);  // the row's, if it is one of these
-                        if ((lane >> 1) == i) er = mine;
+                            for (int o = 4; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(kFull, mx, o));
+                            mx = __shfl_sync(kFull, mx, (lane & 3) * 8);  // the thread's row, if it is one of these
+                            if ((lane >> 2) == i) top = max(top, mx);
+                        }
+                    if constexpr (TURNS) {  // the other half of the row is the other warpgroup's
+                        qtop[tid] = top;
+                        soft_all(true);
+                        top = max(top, qtop[tid ^ kRows]);
                     }
-                    v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                    *cell = v;
+                    er = min(max((int)(top >> 23) - 127, -100), 127);
+                    rs = fmaxf(rs * __int_as_float((127 - 14 + er) << 23), 1.2e-38f);
                 }
-                if constexpr (Q8) rs = fmaxf(rs * __int_as_float((127 - 14 + er) << 23), 1.2e-38f);
+#pragma unroll 1
+                for (int sb = slab0; sb < slab1; ++sb)
+#pragma unroll 2
+                    for (int i = 0; i < 8; ++i) {
+                        uint4* cell = reinterpret_cast<uint4*>(qtile + tile_off(w0 + 4 * i + hi, 8 * sb + c));
+                        uint4 v = *cell;
+                        if constexpr (Q8) {
+                            const float f = __int_as_float((127 + 14 - __shfl_sync(kFull, er, 4 * i + hi)) << 23);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                set_word(v, x, MP::pack(P::lo(word(v, x)) * f, P::hi(word(v, x)) * f));
+                        }
+                        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+                        *cell = v;
+                    }
             }
             proxy_fence();
             mbar_arrive(&bars.q_full);
         }
         float m = -INFINITY, l = 0.f;  // reference maximum and the sum against it
         float unscale = 1.f;           // 2^-x
-        for (int j = 0; t < ntile && j < nblk; ++j) {
-            const uint32_t nb = n0 + (uint32_t)j;
+        for (int j = TURNS ? (int)((t + n0) & 1u) : 0; t < ntile && j < nblk; j += STEP) {
+            const uint32_t nb = n0 + (uint32_t)j, phase = TURNS ? nb >> 1 : uses + (uint32_t)j;
+            const bool first = j < STEP;
             const int slot = (int)(nb % C::SLOTS), kb = k_begin + j * kRows;
             got = mbar_wait(&bars.info_full[slot], (nb / C::SLOTS) & 1, abort) &&
-                  mbar_wait(&bars.s_full[t], (uses + (uint32_t)j) & 1, abort);
+                  mbar_wait(&bars.s_full[t], phase & 1, abort);
             if (!__all_sync(kFull, got)) {
                 got = false;
                 break;
             }
             tc_fence_after();
+            if (idle) {  // what is in its rows of P reaches no other row of O
+                tc_fence_before();
+                mbar_arrive(&bars.p_full[t][0]);
+                mbar_arrive(&bars.p_full[t][1]);
+                continue;
+            }
             uint32_t see[4];
             {
                 const uint4 v = *reinterpret_cast<const uint4*>(valid[slot]);
@@ -737,7 +805,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             bool near = true;
             if constexpr (Q8) {
                 near = snear[slot] != 0;
-                if (j == 0) unscale = __int_as_float((127 - sexp[slot]) << 23);
+                if (first) unscale = __int_as_float((127 - sexp[slot]) << 23);
             }
             // the two halves of a block one after the other: the first's products run during
             // the second's softmax (not unrolled: the roles share the instruction cache)
@@ -749,11 +817,11 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
             // The reference moves: O and l with it.
             auto follow = [&](bool move, float mx) {
                 const float corr = move ? ex2(m - mx) : 1.f;
-                if (j > 0 || h > 0) {
+                if (!first || h > 0) {
                     // O is between two products: those of the block before were done before this
                     // block's S, the first half's are waited for, this half's wait for P
                     if (h == 1) {
-                        got = __all_sync(kFull, mbar_wait(&bars.pv_done[t], (uses + (uint32_t)j) & 1, abort));
+                        got = __all_sync(kFull, mbar_wait(&bars.pv_done[t], phase & 1, abort));
                         if (!got) return;
                         tc_fence_after();
                     }
@@ -884,73 +952,100 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
         }
         got = got && mbar_wait(&bars.o_full, seg & 1, abort);
         got = __all_sync(kFull, got);
+        const bool whole = sg.slot < 0;
+        float own = unscale, other = 0.f;  // what O_t, and the other warpgroup's, are multiplied by
+        bool both = false;                 // whether there is the other's
+        if constexpr (TURNS) {
+            // one row's two sums against the larger reference
+            stat[0][tid] = m, stat[1][tid] = l, stat[2][tid] = unscale;
+            got = soft_all(got);
+            const float m2 = stat[0][tid ^ kRows], top = fmaxf(m, m2);
+            const float f = m == -INFINITY ? 0.f : ex2(m - top), f2 = m2 == -INFINITY ? 0.f : ex2(m2 - top);
+            both = nblk > 1;
+            own *= f;
+            other = stat[2][tid ^ kRows] * f2;
+            l = l * f + stat[1][tid ^ kRows] * f2;
+            m = top;
+        }
+        if (whole) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            own *= inv, other *= inv;
+        }
+        // of one block only one warpgroup has an O
+        const uint32_t sA = TURNS && !both ? tmem + lanes + (uint32_t)((2 + (n0 & 1u)) * kRows) : sO;
+        const uint32_t sB = tmem + lanes + (uint32_t)((2 + (t ^ 1)) * kRows);
+        if (TURNS && !both && (n0 & 1u) != (uint32_t)t) own = other;
         ++seg;
         n0 += (uint32_t)nblk;
         if (t < ntile) uses += (uint32_t)nblk;
-        if (got && t < ntile) {
+        if (got && t < ntile && !idle) {
             tc_fence_after();
-            const bool whole = sg.slot < 0;
-            const float inv = unscale * (!whole ? 1.f : l == 0.f ? 0.f : 1.f / l);
-            float* part = whole ? nullptr : tree_partial(a, gridDim.x, blockIdx.x, sg.slot, NT * kRows, tid, kD);
-            // O leaves through Q's tile, which nothing reads any more: each thread its row
-            // there, then the warp whole rows (partials: half rows of 64 floats) to memory
-            const int hi = lane >> 4, c = lane & 15, w0 = (warp & 3) * 32;
+            float* part = whole ? nullptr : tree_partial(a, gridDim.x, blockIdx.x, sg.slot, NT * kRows, TURNS ? r : tid, kD);
+            // O leaves through Q's tile, which nothing reads any more: each thread its row of a
+            // slab there, then the warp's rows, 128 bytes at a time, to memory
             const int64_t to = !live ? -1 : whole ? trow_q * a.ot + (int64_t)hq * a.oh : 0;
-#pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-#pragma unroll 1
-                for (int q = 0; q < 2; ++q) {
-                    uint32_t o[32];
-                    tmem_ld32(sO + 64 * half + 32 * q, o);
-                    tmem_wait_ld();
-                    if (whole) {
-                        using P = Packed<T>;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            uint4 v;
-                            v.x = P::pack(__uint_as_float(o[8 * x]) * inv, __uint_as_float(o[8 * x + 1]) * inv);
-                            v.y = P::pack(__uint_as_float(o[8 * x + 2]) * inv, __uint_as_float(o[8 * x + 3]) * inv);
-                            v.z = P::pack(__uint_as_float(o[8 * x + 4]) * inv, __uint_as_float(o[8 * x + 5]) * inv);
-                            v.w = P::pack(__uint_as_float(o[8 * x + 6]) * inv, __uint_as_float(o[8 * x + 7]) * inv);
-                            *reinterpret_cast<uint4*>(qtile + tile_off(r, 8 * half + 4 * q + x)) = v;
-                        }
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 8; ++x)
-                            *reinterpret_cast<uint4*>(qtile + tile_off(r, 8 * q + x)) =
-                                make_uint4(__float_as_uint(__uint_as_float(o[4 * x]) * inv),
-                                           __float_as_uint(__uint_as_float(o[4 * x + 1]) * inv),
-                                           __float_as_uint(__uint_as_float(o[4 * x + 2]) * inv),
-                                           __float_as_uint(__uint_as_float(o[4 * x + 3]) * inv));
-                    }
-                }
-                if (whole && half == 0) continue;
+            auto leave = [&](int sb, int col) {  // (col: of the row's floats, for partials)
                 __syncwarp();
 #pragma unroll 4
-                for (int i = 0; i < 16; ++i) {
-                    const int rr = 2 * i + hi;
+                for (int i = 0; i < 8; ++i) {
+                    const int rr = 4 * i + hi;
                     const int64_t row = __shfl_sync(kFull, to, rr);
-                    const uint4 v = *reinterpret_cast<const uint4*>(qtile + tile_off(w0 + rr, c));
+                    const uint4 v = *reinterpret_cast<const uint4*>(qtile + tile_off(w0 + rr, 8 * sb + c));
                     if (row >= 0) {
                         if (whole) {
-                            st16(reinterpret_cast<T*>(a.out) + row + 8 * c, v);
+                            st16(reinterpret_cast<T*>(a.out) + row + 64 * sb + 8 * c, v);
                         } else {  // (rows of D + 2 floats: 8-byte aligned)
                             float* dst = tree_partial(a, gridDim.x, blockIdx.x, sg.slot, NT * kRows,
-                                                      t * kRows + w0 + rr, kD) + 64 * half + 4 * c;
+                                                      (TURNS ? 0 : t * kRows) + w0 + rr, kD) + col + 4 * c;
                             *reinterpret_cast<uint2*>(dst) = make_uint2(v.x, v.y);
                             *reinterpret_cast<uint2*>(dst + 2) = make_uint2(v.z, v.w);
                         }
                     }
                 }
                 __syncwarp();
+            };
+#pragma unroll 1
+            for (int sb = slab0; sb < slab1; ++sb) {
+#pragma unroll 1
+                for (int q = 0; q < 2; ++q) {
+                    float o[32];
+                    {
+                        uint32_t x[32];
+                        tmem_ld32(sA + 64 * sb + 32 * q, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(x[e]) * own;
+                        if (TURNS && both) {
+                            tmem_ld32(sB + 64 * sb + 32 * q, x);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = fmaf(__uint_as_float(x[e]), other, o[e]);
+                        }
+                    }
+                    if (whole) {
+                        using P = Packed<T>;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            *reinterpret_cast<uint4*>(qtile + tile_off(r, 8 * sb + 4 * q + x)) =
+                                make_uint4(P::pack(o[8 * x], o[8 * x + 1]), P::pack(o[8 * x + 2], o[8 * x + 3]),
+                                           P::pack(o[8 * x + 4], o[8 * x + 5]), P::pack(o[8 * x + 6], o[8 * x + 7]));
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            *reinterpret_cast<float4*>(qtile + tile_off(r, 8 * sb + x)) =
+                                make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                        leave(sb, 64 * sb + 32 * q);
+                    }
+                }
+                if (whole) leave(sb, 0);
             }
-            if (live && !whole) *reinterpret_cast<float2*>(part + kD) = make_float2(m, l);
+            if (live && !whole && (!TURNS || t == 0)) *reinterpret_cast<float2*>(part + kD) = make_float2(m, l);
             // (set before the last v_full, which o_full follows; the next segment's can only raise
             // it, and makes this one look where nothing is to be found)
             if (live && *static_cast<volatile int*>(&odd_v) >= seq_no) {
                 const int j0 = k_begin + min(first_draft, nblk) * kRows;
-                if (whole) add_not_finite<T, FMT, T>(a, bt, sg.g, w.ctx, mrow, qrow, sl2, m, j0, k_end, orow);
-                else add_not_finite<T, FMT, float>(a, bt, sg.g, w.ctx, mrow, qrow, sl2, m, j0, k_end, part);
+                if (whole) add_not_finite<T, FMT, T>(a, bt, sg.g, w.ctx, mrow, qrow, sl2, m, j0, k_end, 64 * slab0, 64 * slab1, orow);
+                else add_not_finite<T, FMT, float>(a, bt, sg.g, w.ctx, mrow, qrow, sl2, m, j0, k_end, 64 * slab0, 64 * slab1, part);
             }
             __syncwarp();
             tc_fence_before();  // O is read: the next segment's products follow q_full, or p_full
@@ -963,7 +1058,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, NT == 1 ? 2 : 1)
     if (tid == 0 && abort_flag) flag(a.status, QF_FLAG_TIMEOUT);
     if (warp == C::MMA_WARP) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols)
                      : "memory");
     }
 }
