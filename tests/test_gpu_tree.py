@@ -328,6 +328,20 @@ def test_many_sequences_of_every_length(hq, hkv):
         assert torch.equal(got, _run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes))
 
 
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (16, 2), (64, 2)])
+def test_one_long_sequence_among_short_ones(dtype, hq, hkv):
+    """The long one is shared by most CTAs, however few a sequence gets on average."""
+    sizes = [1 + i % 3 for i in range(150)]
+    contexts = [i % 20 for i in range(150)]
+    contexts[40] = 30000
+    for fmt in (None, E4M3):
+        q, k, v, ks, vs, bt, mask = _case(sizes, contexts, hq, hkv, 128, 16, dtype, fmt, 6)
+        out, bound = ref.attention(q, k, v, bt, 16, contexts, sizes, mask, ks, vs,
+                                   p_type=torch.float16 if fmt and dtype != torch.float32 else None)
+        ref.assert_within(_run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes), out, bound)
+
+
 def test_two_graphs_share_nothing():
     sizes, contexts = [30, 8], [2000, 700]
     cases = [_case(sizes, contexts, 16, 2, 128, 16, torch.bfloat16, f, 4) for f in (None, E4M3)]

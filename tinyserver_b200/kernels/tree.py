@@ -81,15 +81,16 @@ def build_tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor,
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(num_tokens: int, num_seqs: int, max_tree: int, num_q_heads: int,
+def _workspace_bytes(dev: int, num_tokens: int, num_seqs: int, max_tree: int, num_q_heads: int,
                      num_kv_heads: int, head_dim: int, block_size: int, max_blocks_per_seq: int,
                      tag: int, fmt: int, decode: bool) -> int:
-    return int(_capi.lib().qf_paged_tree_attention_workspace_bytes(
-        _capi.PagedTreeAttentionArgs.named(
-            cu_seqlens_q=0 if decode else 1,  # (whether there is one is all that is read)
-            num_tokens=num_tokens, num_seqs=num_seqs, max_tree=max_tree, num_q_heads=num_q_heads,
-            num_kv_heads=num_kv_heads, head_dim=head_dim, block_size=block_size,
-            max_blocks_per_seq=max_blocks_per_seq, dtype=tag, cache_format=fmt)))
+    args = _capi.PagedTreeAttentionArgs.named(
+        cu_seqlens_q=0 if decode else 1,  # (whether there is one is all that is read)
+        num_tokens=num_tokens, num_seqs=num_seqs, max_tree=max_tree, num_q_heads=num_q_heads,
+        num_kv_heads=num_kv_heads, head_dim=head_dim, block_size=block_size,
+        max_blocks_per_seq=max_blocks_per_seq, dtype=tag, cache_format=fmt)
+    with torch.cuda.device(dev):  # (its number of SMs counts; dev < 0: no GPU, no switch)
+        return int(_capi.lib().qf_paged_tree_attention_workspace_bytes(args))
 
 
 def paged_tree_attention_workspace_bytes(num_tokens: int, num_seqs: int, max_tree: int,
@@ -101,7 +102,8 @@ def paged_tree_attention_workspace_bytes(num_tokens: int, num_seqs: int, max_tre
     format; a decode call (:func:`~tinyserver_b200.paged_attention_quantized`) counts
     as max_tree 1.  It depends on the GPU: ask with the call's device current."""
     tag = dtype_tag(torch.empty(0, dtype=dtype), "paged_tree_attention_workspace_bytes")
-    sizes = (num_tokens, num_seqs, max_tree, num_q_heads, num_kv_heads, head_dim, block_size,
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    sizes = (dev, num_tokens, num_seqs, max_tree, num_q_heads, num_kv_heads, head_dim, block_size,
              max_blocks_per_seq, tag)
     return max(_workspace_bytes(*sizes, fmt, decode) for decode in {False, max_tree == 1}
                for fmt in (_capi.QF_CACHE_PLAIN, *CACHE_FORMATS.values()))
@@ -188,7 +190,7 @@ def attend(what: str, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     space = 0
     if split:
         if workspace is None:
-            space = _workspace_bytes(T, S, max_tree, Hq, Hkv, D, B, max_blocks, tag, fmt, cu is None)
+            space = _workspace_bytes(dev, T, S, max_tree, Hq, Hkv, D, B, max_blocks, tag, fmt, cu is None)
             if space:
                 workspace = torch.empty(space // 4, dtype=torch.float32, device=q.device)
         else:
