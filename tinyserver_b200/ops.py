@@ -6,9 +6,9 @@ errors and results are exactly those.  What the registration adds:
 
 - the ops appear as single nodes in FX / ``torch.compile`` / ``torch.export``
   graphs instead of being traced into;
-- the stores declare their in-place writes to ``k_cache`` / ``v_cache``
-  (``mutates_args``), so a compiled graph orders them against the caches'
-  other uses;
+- the stores declare their in-place writes to ``k_cache`` / ``v_cache`` and
+  to a quantised cache's scales (``mutates_args``), so a compiled graph
+  orders them against the caches' other uses;
 - every op has a fake (meta) implementation that gives the output shapes,
   dtypes and strides of the real one without launching anything, so graphs
   can be traced with fake or meta tensors.
