@@ -120,6 +120,18 @@ def test_decode_refuses_other_lengths():
         _attend(True, lens=torch.zeros(3, dtype=torch.int32), block_tables=torch.zeros(3, 3, dtype=torch.int32))
 
 
+@pytest.mark.parametrize("workspace", [torch.zeros(1).expand(1 << 20), torch.zeros(64)[::2]])
+def test_workspace_in_one_piece(workspace):
+    q, lens, bt = torch.zeros(1, 4, 128, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32), \
+        torch.zeros(1, 3, dtype=torch.int32)
+    cu, mask = torch.zeros(2, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int64)
+    with pytest.raises(ValueError, match="contiguous"):
+        tsb.paged_tree_attention(q, PLAIN, PLAIN, bt, 8, lens, cu, mask, 1, workspace=workspace)
+    codes, scales = _cache()
+    with pytest.raises(ValueError, match="contiguous"):
+        tsb.paged_attention_quantized(q, codes, codes, scales, scales, bt, 8, lens, workspace=workspace)
+
+
 def test_mask_refusals():
     p, cu = torch.zeros(3, dtype=torch.int32), torch.tensor([0, 3])
     for bad, match in (((p[None], cu, 3), "parents must"), ((p, cu, 0), "max_tree"), ((p.float(), cu, 3), "index dtype"),

@@ -112,20 +112,23 @@ def paged_tree_attention_workspace_bytes(num_tokens: int, num_seqs: int, max_tre
 def check_quantized_cache(what: str, k_cache: torch.Tensor, v_cache: torch.Tensor,
                           k_scale: torch.Tensor, v_scale: torch.Tensor) -> int:
     """The cache format of a quantised cache; ValueError unless codes and scales fit."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+    shape, dtype = k_cache.shape, k_cache.dtype
+    fmt, rows = CACHE_FORMATS.get(dtype), shape[:3]
+    if (fmt is not None and len(shape) == 4 and v_cache.shape == shape and v_cache.dtype == dtype
+            and k_scale.shape == rows and v_scale.shape == rows
+            and k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32):
+        return fmt
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError(f"{what}: k_cache/v_cache must be (num_blocks, num_kv_heads, block_size, "
                          f"head_dim), got {tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    fmt = CACHE_FORMATS.get(k_cache.dtype)
-    if fmt is None or v_cache.dtype != k_cache.dtype:
+    if fmt is None or v_cache.dtype != dtype:
         raise ValueError(f"{what}: a quantised cache holds float8_e4m3fn or int8 rows, got "
                          f"{k_cache.dtype} and {v_cache.dtype}")
-    if k_scale.shape != k_cache.shape[:3] or v_scale.shape != k_cache.shape[:3]:
+    if k_scale.shape != rows or v_scale.shape != rows:
         raise ValueError(f"{what}: k_scale/v_scale must be (num_blocks, num_kv_heads, block_size) "
-                         f"= {tuple(k_cache.shape[:3])}, got {tuple(k_scale.shape)} and "
+                         f"= {tuple(rows)}, got {tuple(k_scale.shape)} and "
                          f"{tuple(v_scale.shape)}")
-    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
-        raise ValueError(f"{what}: scales must be float32, got {k_scale.dtype} and {v_scale.dtype}")
-    return fmt
+    raise ValueError(f"{what}: scales must be float32, got {k_scale.dtype} and {v_scale.dtype}")
 
 
 def attend(what: str, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -137,6 +140,8 @@ def attend(what: str, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     """The call both public forms make (``cu_seqlens`` None: decode)."""
     if query.dim() != 3:
         raise ValueError(f"{what}: query must be a 3D tensor, but got shape {tuple(query.shape)}")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous, got strides {workspace.stride()}")
     if (k_scale is None) != (v_scale is None):
         raise ValueError(f"{what}: k_scale and v_scale come together")
     if k_scale is not None:
