@@ -779,8 +779,22 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
             const uint32_t nb = n0 + (uint32_t)j, phase = TURNS ? nb >> 1 : uses + (uint32_t)j;
             const bool first = j < STEP;
             const int slot = (int)(nb % C::SLOTS), kb = k_begin + j * kRows;
-            got = mbar_wait(&bars.info_full[slot], (nb / C::SLOTS) & 1, abort) &&
-                  mbar_wait(&bars.s_full[t], phase & 1, abort);
+            // what the rows see: over 16-bit rows found while S is on its way (64 trees of 64
+            // 348 -> 343 us), over codes, with more to hold, behind it (32 of 32 221 -> 214)
+            uint32_t see[4];
+            bool masked, near = true;
+            auto look = [&]() {
+                const uint4 v = *reinterpret_cast<const uint4*>(valid[slot]);
+                see[0] = v.x, see[1] = v.y, see[2] = v.z, see[3] = v.w;
+                if (j >= first_draft || !live)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        see[q] = live ? see[q] & tree_bits32(mrow, a.words, kb + 32 * q - w.ctx) : 0u;
+                masked = __any_sync(kFull, (see[0] & see[1] & see[2] & see[3]) != kFull);
+            };
+            got = mbar_wait(&bars.info_full[slot], (nb / C::SLOTS) & 1, abort);
+            if constexpr (!Q8) look();
+            got = got && mbar_wait(&bars.s_full[t], phase & 1, abort);
             if (!__all_sync(kFull, got)) {
                 got = false;
                 break;
@@ -792,18 +806,8 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
                 mbar_arrive(&bars.p_full[t][1]);
                 continue;
             }
-            uint32_t see[4];
-            {
-                const uint4 v = *reinterpret_cast<const uint4*>(valid[slot]);
-                see[0] = v.x, see[1] = v.y, see[2] = v.z, see[3] = v.w;
-            }
-            if (j >= first_draft || !live)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    see[q] = live ? see[q] & tree_bits32(mrow, a.words, kb + 32 * q - w.ctx) : 0u;
-            const bool masked = __any_sync(kFull, (see[0] & see[1] & see[2] & see[3]) != kFull);
-            bool near = true;
             if constexpr (Q8) {
+                look();
                 near = snear[slot] != 0;
                 if (first) unscale = __int_as_float((127 - sexp[slot]) << 23);
             }
