@@ -87,6 +87,8 @@ __device__ __forceinline__ uint4 quantise16(const float* f, float& scale) {
 
 template <typename T, int D, int FMT>
 __global__ void __launch_bounds__(256) quant_store_kernel(const QuantKv a) {
+    pdl_wait();
+    pdl_trigger();
     constexpr int LPR = D / 16;     // lanes per row
     constexpr int TT = 256 / LPR;   // tokens per CTA
     constexpr int64_t ES = sizeof(T);
@@ -126,6 +128,8 @@ __device__ __forceinline__ void dequantise16(char* dst, const uint4& c, float sc
 
 template <typename T, int D, int FMT>
 __global__ void __launch_bounds__(256) quant_load_kernel(const QuantKv a) {
+    pdl_wait();
+    pdl_trigger();
     constexpr int LPR = D / 16, TT = 256 / LPR;
     constexpr int64_t ES = sizeof(T);
     const int c = threadIdx.x % LPR, r = threadIdx.x / LPR;
@@ -193,9 +197,8 @@ int launch(const QuantKv& a, bool fast, cudaStream_t stream) {
         const dim3 grid((unsigned)ceil_div(a.T, tt), (unsigned)a.Hkv);
 #define QF_QUANT_CASE(DD)                                                            \
     case DD:                                                                         \
-        if constexpr (STORE) quant_store_kernel<T, DD, FMT><<<grid, 256, 0, stream>>>(a); \
-        else quant_load_kernel<T, DD, FMT><<<grid, 256, 0, stream>>>(a);             \
-        return check_launch();
+        if constexpr (STORE) return launch_pdl(quant_store_kernel<T, DD, FMT>, grid, 256, 0, stream, a); \
+        else return launch_pdl(quant_load_kernel<T, DD, FMT>, grid, 256, 0, stream, a);
         switch (a.D) {
             QF_QUANT_CASE(64)
             QF_QUANT_CASE(128)

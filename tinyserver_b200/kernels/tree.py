@@ -69,8 +69,9 @@ def build_tree_mask(parents: torch.Tensor, cu_seqlens: torch.Tensor,
     n, words, seqs = parents.numel(), (max_tree + 63) // 64, cu.numel() - 1
     if n and seqs < 1:
         raise ValueError(f"build_tree_mask: {n} nodes but no sequence")
-    mask = torch.empty((n, words), dtype=torch.int64, device=parents.device)
-    depths = torch.empty((n,), dtype=torch.int32, device=parents.device)
+    # (empty_strided: a microsecond less a call than empty)
+    mask = torch.empty_strided((n, words), (words, 1), dtype=torch.int64, device=parents.device)
+    depths = torch.empty_strided((n,), (1,), dtype=torch.int32, device=parents.device)
     rc = launch(dev, _capi.lib().qf_build_tree_mask, _capi.TreeMaskArgs.pack(
         parents.data_ptr(), cu.data_ptr(), seqs, n, max_tree, words, mask.data_ptr(),
         depths.data_ptr(), itag, status_ptr(dev)))
@@ -197,7 +198,8 @@ def attend(what: str, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         if workspace is None:
             space = _workspace_bytes(dev, T, S, max_tree, Hq, Hkv, D, B, max_blocks, tag, fmt, cu is None)
             if space:
-                workspace = torch.empty(space // 4, dtype=torch.float32, device=q.device)
+                workspace = torch.empty_strided((space // 4,), (1,), dtype=torch.float32,
+                                                device=q.device)
         else:
             space = workspace.numel() * workspace.element_size()
     scaled = k_scale is not None
