@@ -14,9 +14,9 @@
 // sectors.  Rows of other widths, strides or alignments take one warp per row
 // and element-wise accesses.
 //
-// 8 heads of 128, bf16 <-> e4m3, pages of 16 slots: 8192 tokens stored in 8.9 us (5.7
-// TB/s), 16411 loaded in 19.6 us (5.2 TB/s); over int8, 256 tokens stored in 2.6 us and
-// 484 loaded in 3.4 us, a launch's own time.
+// 8 heads of 128, bf16 <-> e4m3, pages of 16 slots: 8192 tokens stored in 8.8 us (5.8
+// TB/s), 16411 loaded in 19.0 us (5.4 TB/s); over int8, 256 tokens stored in 2.4 us and
+// 484 loaded in 3.0 us, a launch's own time (0.3 us less by programmatic dependent launch).
 #include "qf_quant.cuh"
 
 namespace qf {

@@ -27,15 +27,15 @@
 // share of HBM; a tile's softmax is 16384 exponentials, 1024 cycles of the MUFU,
 // and its products 1024 cycles of the tensor core.
 //  * Up to 128 rows, 16-bit rows: by HBM's latency, with 128 KB of K and V stages per
-//    SM: 32 trees of 16 nodes x 4 heads at 4096 context keys, 8 kv heads: 113 us, 4.85
+//    SM: 32 trees of 16 nodes x 4 heads at 4096 context keys, 8 kv heads: 109 us, 5.0
 //    TB/s (two CTAs per SM with one stage each and halves of a block in turn: 127 us).
 //  * 8-bit rows: by the softmax warps' dependent instructions (two warps per scheduler;
 //    36% of the issue slots used): a half block takes 2300 cycles, against 1100 over
 //    16-bit rows, for the scales' loads and products.  The same trees over e4m3: 154 us
-//    (182 us); 32 trees of 32 nodes at up to 8191 context keys: 220 us.
+//    (182 us); 32 trees of 32 nodes at up to 8191 context keys: 213 us.
 //  * More than 128 rows: by the chain of products and softmax, ~4100 cycles a block of
-//    two tiles; 64 trees of 64 nodes x 4 heads at up to 8191 context keys: 350 us, 870
-//    TFLOP/s (as single tiles, which read K and V twice: 445 us).
+//    two tiles; 64 trees of 64 nodes x 4 heads at up to 8191 context keys: 329 us, 925
+//    TFLOP/s (as single tiles, which read K and V twice, 445 us against 350 then).
 // Registers moved from the loaders to the softmax (88 and 168 a thread instead of 128)
 // cost more in the loaders than they gained: 154 -> 206 us.
 //
