@@ -342,6 +342,26 @@ def test_one_long_sequence_among_short_ones(dtype, hq, hkv):
         ref.assert_within(_run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes), out, bound)
 
 
+@pytest.mark.parametrize("fmt,block", [(None, 16), (None, 12), (E4M3, 16), (E4M3, 6)])
+def test_caches_past_32_bit_offsets(fmt, block):
+    """Rows by TMA boxes and one by one, from blocks more than 2^31 elements behind the first."""
+    sizes, contexts = [3, 40], [50, 200]
+    q, k, v, ks, vs, bt, mask = _case(sizes, contexts, 8, 2, 128, block, torch.bfloat16, fmt, 8)
+    first = (1 << 31) // (2 * block * 128) + 1
+
+    def far(t):
+        if t is None:
+            return None
+        big = torch.empty((first + t.shape[0], *t.shape[1:]), dtype=t.dtype, device=DEV)
+        big[first:] = t
+        return big
+    out, bound = ref.attention(q, k, v, bt, block, contexts, sizes, mask, ks, vs,
+                               p_type=torch.float16 if fmt else None)
+    got = _run(q, far(k), far(v), far(ks), far(vs), bt + first, mask, block, contexts, sizes)
+    tsb.check_errors()
+    ref.assert_within(got, out, bound)
+
+
 def test_two_graphs_share_nothing():
     sizes, contexts = [30, 8], [2000, 700]
     cases = [_case(sizes, contexts, 16, 2, 128, 16, torch.bfloat16, f, 4) for f in (None, E4M3)]
