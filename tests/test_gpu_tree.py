@@ -298,6 +298,23 @@ def test_scales_over_eight_decades_and_none(fmt, dtype, n, hq):
         ref.assert_within(got, out, bound, f"split={split}")
 
 
+@pytest.mark.parametrize("fmt", ref.FORMATS)
+@pytest.mark.parametrize("dtype", (torch.float32, torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("n,hq", [(1, 2), (8, 4), (40, 8)])
+def test_rows_never_written_ahead_of_the_others(fmt, dtype, n, hq):
+    """Keys whose codes and scales are 0 score 0, have that weight, and add nothing: 700 of them first, so that
+    they alone set a maximum and a sum before any other key does, alone in a sequence, and all of it."""
+    sizes, contexts = [n, 2, 1], [1500, 0, 520]
+    q, k, v, ks, vs, bt, mask = _case(sizes, contexts, hq, 2, 128, 16, dtype, fmt, 12)
+    for blocks in (bt[0, :44].long(), bt[2, :20].long()):
+        for t in (k.view(torch.uint8), v.view(torch.uint8), ks, vs):
+            t[blocks] = 0
+    out, bound = ref.attention(q, k, v, bt, 16, contexts, sizes, mask, ks, vs,
+                               p_type=torch.float16 if dtype != torch.float32 else None)
+    for split in (True, False):
+        ref.assert_within(_run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes, split=split), out, bound, f"split={split}")
+
+
 @pytest.mark.parametrize("dtype", (torch.float32, torch.float16, torch.bfloat16))
 @pytest.mark.parametrize("scale", [-0.2, 0.0])
 def test_negative_and_zero_softmax_scale(dtype, scale):

@@ -307,8 +307,9 @@ struct Join {
         for (int p = sub; p < n; p += WPR) {
             const float* wp = partial(p);
             const float2 ml = *reinterpret_cast<const float2*>(wp + D);
-            const float f = exp2f(ml.x - base);
-            Ls += ml.y * f;
+            // (a factor in two halves: a sum may be 2^100 and more, see kLeastScale)
+            const float h = exp2f(0.5f * (ml.x - base)), f = h * h;
+            Ls += ml.y * h * h;
 #pragma unroll
             for (int e = 0; e < PER; e += 2) {
                 const float2 v = *reinterpret_cast<const float2*>(wp + e * 32 + lane * 2);
@@ -332,8 +333,9 @@ struct Join {
         float f[WPR], total = 0.f;
 #pragma unroll
         for (int k = 0; k < WPR; ++k) {
-            f[k] = top == -INFINITY ? 0.f : exp2f(tops[w0 + k] - top);
-            total += sums[w0 + k] * f[k];
+            const float h = top == -INFINITY ? 0.f : exp2f(0.5f * (tops[w0 + k] - top));
+            f[k] = h * h;
+            total += sums[w0 + k] * h * h;
         }
         for (int d = sub * 32 + lane; d < D; d += WPR * 32) {
             float A = 0.f;
@@ -439,7 +441,6 @@ struct TreePlan {
     int tiles;      // row tiles per CTA of the tcgen05 kernel; 0: another kernel
     int rows;       // rows per work item
     int ctas;       // persistent CTAs: as many as fit, or one per unit of work if that is fewer
-    int min_units;  // least stretch of a CTA
     bool split;     // whether sequences may be cut
     bool spread;    // whether joining an item's rows is for a CTA each (see tree_merge_kernel)
     bool fits;      // whether the work has fewer than 2^31 units
@@ -447,18 +448,17 @@ struct TreePlan {
 
 // The kernel and its grid, by sizes alone (lengths are on the device; the block
 // tables bound them).  A cut costs a partial of (D + 2) floats a row, written and
-// read back, so a CTA's stretch is at least two blocks of 128 keys, or four of 64;
-// and a second launch, so sequences of up to 768 keys (256 of the mma.sync kernel's)
+// read back, so a CTA's stretch is at least two blocks of keys; and a second launch, so
+// sequences of up to 768 keys (256 of the mma.sync kernel's)
 // stay whole.  Whole | cut: a tree of 16 nodes x 4 heads, 8 kv heads, at 500 keys 15.3 |
 // 16.9 us, at 1000 18.3 | 17.1, at 2000 26.7 | 18.7; 8 of them at 500 keys 16.4 | 22.9;
-// decode of 4 sequences over e4m3 at 200 keys 9.0 | 10.1 us, at 500 13.6 | 11.4, at 1000
-// 23.7 | 13.6.
+// decode of 4 sequences over e4m3 at 200 keys 8.6 | 9.2 us, at 500 13.1 | 10.6, at 1000
+// 23.7 | 11.9.
 TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     TreePlan p{};
     const int64_t G = g.num_q_heads / g.num_kv_heads, rows = (g.cu_seqlens_q ? g.max_tree : 1) * G;
     int64_t per_sm, keys = 64;
     const bool plain = g.cache_format == QF_CACHE_PLAIN;
-    p.min_units = 4;
     if (g.dtype == QF_F32) {
         p.rows = rows <= 4 ? 4 : 16;
         per_sm = g.head_dim == 256 ? 2 : 4;
@@ -467,7 +467,6 @@ TreePlan make_plan(const qf_paged_tree_attention_args& g) {
         p.rows = 128 * p.tiles;
         per_sm = 1;
         keys = 128;
-        p.min_units = 2;
     } else {
         p.rows = g.head_dim == 256 || rows <= 8 ? 8 : 16;
         per_sm = tree_mma_ctas_per_sm(plain, (int)g.head_dim);
@@ -597,7 +596,6 @@ extern "C" int qf_paged_tree_attention(const qf_paged_tree_attention_args* p, cu
     a.ot = g.out_stride_token;
     a.oh = g.out_stride_head;
     a.ws = need > 0 ? static_cast<float*>(g.workspace) : nullptr;
-    a.min_units = plan.min_units;
     a.status = g.status;
     const int D = (int)g.head_dim;
     if (g.dtype == QF_F32)

@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
                         const float2 k2 = *reinterpret_cast<const float2*>(sp + 8 * n + 2 * tig);
                         const float2 v2 = *reinterpret_cast<const float2*>(sp + 16 + 8 * n + 2 * tig);
                         ksv[n][0] = k2.x, ksv[n][1] = k2.y;
-                        // a scale of 0 (a row never written) stands for zeros, as good as at 2^-120
+                        // a scale of 0 (a row never written) stands for zeros, as good as at 2^-100
                         lvv[n][0] = log2_of(v2.x < kLeastScale ? kLeastScale : v2.x);
                         lvv[n][1] = log2_of(v2.y < kLeastScale ? kLeastScale : v2.y);
                     }
@@ -333,7 +333,10 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
                     mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 2));
                     const float mn = fmaxf(m[nt], mx), base = mn == -INFINITY ? 0.f : mn;
-                    corr[nt] = pow2(m[nt] - base);
+                    // (in two steps: l may be 2^100 and more, see kLeastScale, and what is left
+                    // of it count, where the factor alone is too small for a float)
+                    const float half = pow2(0.5f * (m[nt] - base));
+                    corr[nt] = half * half;
                     m[nt] = mn;
                     float sum = 0.f;
 #pragma unroll
@@ -343,7 +346,7 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
                             pw[nt][n][e] = pow2(u[n][e] - base);
                             sum += Q8 ? pow2(t[n][e] - base) : pw[nt][n][e];
                         }
-                    l[nt] = l[nt] * corr[nt] + sum;
+                    l[nt] = l[nt] * half * half + sum;
                     moved |= corr[nt] != 1.f;
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
@@ -493,9 +496,9 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
             for (int k = 0; k < kWarps; ++k) M = fmaxf(M, wm[k * NR + ri]);
 #pragma unroll
             for (int k = 0; k < kWarps; ++k) {
-                const float f = M == -INFINITY ? 0.f : exp2f(wm[k * NR + ri] - M);
-                Ls += wl[k * NR + ri] * f;
-                A += wacc[(k * NR + ri) * D + d] * f;
+                const float f = M == -INFINITY ? 0.f : exp2f(0.5f * (wm[k * NR + ri] - M));  // its half
+                Ls += wl[k * NR + ri] * f * f;
+                A += wacc[(k * NR + ri) * D + d] * f * f;
             }
             if (sg.slot < 0) {
                 const int tok = r / a.G;

@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
         auto inform = [&](int slot, bool first) {
             if (lane == 0) *reinterpret_cast<uint4*>(valid[slot]) = make_uint4(ok[0], ok[1], ok[2], ok[3]);
             if constexpr (Q8) {
-                // a scale of 0 (a row never written) stands for zeros, as good as at 2^-120
+                // a scale of 0 (a row never written) stands for zeros, as good as at 2^-100
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
                     if (vs[x] < kLeastScale) vs[x] = kLeastScale;
@@ -820,7 +820,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
             const uint32_t see2[2] = {h ? see[2] : see[0], h ? see[3] : see[1]};
             // The reference moves: O and l with it.
             auto follow = [&](bool move, float mx) {
-                const float corr = move ? ex2(m - mx) : 1.f;
+                const float half = move ? ex2(0.5f * (m - mx)) : 1.f, corr = half * half;
                 if (!first || h > 0) {
                     // O is between two products: those of the block before were done before this
                     // block's S, the first half's are waited for, this half's wait for P
@@ -839,7 +839,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
                         tmem_st32(sO + 32 * q, o);
                     }
                 }
-                l *= corr;
+                l = l * half * half;  // (it may be 2^100 and more where a scale is part of m)
                 if (move) m = mx;
             };
             if (!Q8 || near) {
@@ -964,11 +964,12 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
             stat[0][tid] = m, stat[1][tid] = l, stat[2][tid] = unscale;
             got = soft_all(got);
             const float m2 = stat[0][tid ^ kRows], top = fmaxf(m, m2);
-            const float f = m == -INFINITY ? 0.f : ex2(m - top), f2 = m2 == -INFINITY ? 0.f : ex2(m2 - top);
+            const float h = m == -INFINITY ? 0.f : ex2(0.5f * (m - top));
+            const float h2 = m2 == -INFINITY ? 0.f : ex2(0.5f * (m2 - top)), f = h * h, f2 = h2 * h2;
             both = nblk > 1;
             own *= f;
             other = stat[2][tid ^ kRows] * f2;
-            l = l * f + stat[1][tid ^ kRows] * f2;
+            l = l * h * h + stat[1][tid ^ kRows] * h2 * h2;
             m = top;
         }
         if (whole) {
