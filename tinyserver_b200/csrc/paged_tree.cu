@@ -449,11 +449,10 @@ struct TreePlan {
 // The kernel and its grid, by sizes alone (lengths are on the device; the block
 // tables bound them).  A cut costs a partial of (D + 2) floats a row, written and
 // read back, so a CTA's stretch is at least two blocks of keys; and a second launch, so
-// sequences of up to 768 keys (256 of the mma.sync kernel's)
-// stay whole.  Whole | cut: a tree of 16 nodes x 4 heads, 8 kv heads, at 500 keys 15.3 |
-// 16.9 us, at 1000 18.3 | 17.1, at 2000 26.7 | 18.7; 8 of them at 500 keys 16.4 | 22.9;
-// decode of 4 sequences over e4m3 at 200 keys 8.6 | 9.2 us, at 500 13.1 | 10.6, at 1000
-// 23.7 | 11.9.
+// sequences of up to 768 keys (256 of the mma.sync kernel's) stay whole.  Whole | cut: a
+// tree of 16 nodes x 4 heads, 8 kv heads, at 500 keys 15.3 | 16.9 us, at 1000 18.3 |
+// 17.1, at 2000 26.7 | 18.7; 8 of them at 500 keys 16.4 | 22.9; decode of 4 sequences
+// over e4m3 at 200 keys 8.6 | 9.2 us, at 500 13.1 | 10.6, at 1000 23.7 | 11.9.
 TreePlan make_plan(const qf_paged_tree_attention_args& g) {
     TreePlan p{};
     const int64_t G = g.num_q_heads / g.num_kv_heads, rows = (g.cu_seqlens_q ? g.max_tree : 1) * G;

@@ -120,7 +120,8 @@ def paged_attention_quantized(query: torch.Tensor, k_cache: torch.Tensor, v_cach
     """:func:`~tinyserver_b200.paged_attention_forward` over a quantised cache:
     one query token per sequence, ``query`` (num_seqs, Hq, D), against the
     first ``seq_lens[s]`` cached tokens of sequence s, their rows dequantised as
-    they are read.  Any Hq / Hkv; a sequence of no tokens gives zeros."""
+    they are read.  Any Hq / Hkv; a sequence of no tokens gives zeros.  Scales are
+    what the store writes, not negative; one below 2**-100 reads as that."""
     what = "paged_attention_quantized"
     if query.dim() == 3 and (seq_lens.dim() != 1 or seq_lens.numel() != query.shape[0]):
         raise ValueError(f"{what}: seq_lens must be (num_seqs,) for {query.shape[0]} queries, got "
