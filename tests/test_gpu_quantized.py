@@ -327,3 +327,23 @@ def test_a_prefix_cached_quantised_then_prefilled_and_decoded():
     # the prefill's K and V are rounded to bf16 on loading: u in the scores (times E ~ 20) and in V
     u = 2.0 ** -8
     assert ((full.double() - out).abs() <= bound + (2 * 20 * u + u) * 1.0).all()
+
+
+@pytest.mark.parametrize("fmt", ref.FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq", [8, 64])
+def test_keys_of_nan_scales_alone_give_nan(fmt, dtype, hq):
+    """Every V row that a head sees was stored from an infinity or a NaN: its output is NaN, not the zeros of a
+    sequence of no keys; one key, several tiles, and partials none of which has a weight."""
+    lens = [1, 70, 4000, 0]
+    k, v, ks, vs, bt = paged(lens, 2, 128, 16, fmt, dtype, seed=14)
+    vs[:, 1] = float("nan")
+    _bits(v)[:, 1] = 0
+    q = torch.randn(4, hq, 128, generator=torch.Generator().manual_seed(6)).to(dtype).to(DEV)
+    want = torch.zeros(4, hq, dtype=torch.bool, device=DEV)
+    want[:3, hq // 2:] = True
+    for split in (True, False):
+        got = tsb.paged_attention_quantized(q, k, v, ks, vs, bt, 16, torch.tensor(lens, device=DEV), split=split)
+        tsb.check_errors()
+        assert torch.equal(torch.isnan(got).all(-1), want) and torch.isfinite(got[~want]).all(), split
+        assert not got[3].any()

@@ -341,7 +341,8 @@ struct Join {
             float A = 0.f;
 #pragma unroll
             for (int k = 0; k < WPR; ++k) A += part[w0 + k][d] * f[k];
-            o[d] = Dt<T>::from_f(total == 0.f ? 0.f : A / total);
+            // (no weight at all: 0, or NaN where every key the row sees has a NaN for a scale)
+            o[d] = Dt<T>::from_f(total == 0.f ? A * 0.f : A / total);
         }
     }
 };

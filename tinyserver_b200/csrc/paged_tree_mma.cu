@@ -501,9 +501,10 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
                 A += wacc[(k * NR + ri) * D + d] * f * f;
             }
             if (sg.slot < 0) {
+                // (no weight at all: 0, or NaN where every key the row sees has a NaN for a scale)
                 const int tok = r / a.G;
                 reinterpret_cast<T*>(a.out)[(int64_t)(w.q0 + tok) * a.ot + (int64_t)(g * a.G + r - tok * a.G) * a.oh + d] =
-                    Dt<T>::from_f(Ls == 0.f ? 0.f : A / Ls);
+                    Dt<T>::from_f(Ls == 0.f ? A * 0.f : A / Ls);
             } else {
                 float* o = tree_partial(a, gridDim.x, blockIdx.x, sg.slot, NR, ri, D);
                 o[d] = A;
