@@ -456,3 +456,41 @@ def test_registered_ops_match_their_fakes_and_run_in_a_graph():
     assert torch.equal(got, want)
     for a, b in zip(*caches):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("fmt", [None, *ref.FORMATS])
+@pytest.mark.parametrize("n,hq,D,parts", [(1, 2, 128, 4), (12, 1, 64, 4), (5, 1, 256, 4), (40, 1, 128, 2),
+                                          (150, 1, 128, 1)])
+def test_small_weights_beside_keys_without_a_value(fmt, n, hq, D, parts):
+    """A key of a large score and a V of zeros outweighs each of 2^18 others 2^25.5 times, and those make the whole
+    output: they count in the product as they do in the sum, whatever 16-bit type the probabilities are held in.
+    As many such keys as a row has partial sums in a CTA (the mma.sync kernel's warps, which take 16 keys in turn;
+    the tcgen05 kernel's warpgroups, 128 in turn), one for each of them."""
+    block, pages = 64, parts << 12
+    L = pages * block
+    k, v = torch.zeros(5, 1, block, D), -torch.ones(5, 1, block, D)
+    for j in [i * (16 if parts == 4 else 128) for i in range(parts)]:
+        k[j // block, 0, j % block, 0] = 4.42
+        v[j // block, 0, j % block] = 0
+
+    def cache(c):  # four pages, and the fifth again and again
+        return None if c is None else torch.cat([c.to(DEV)[:4], c.to(DEV)[4:].expand(pages - 4, *c.shape[1:])])
+
+    (k, ks), (v, vs) = (map(cache, ref.quantise(c, fmt) if fmt else (c.half(), None)) for c in (k, v))
+    if vs is not None:  # codes of 0 at the scale of the others, so that it is no part of the weight's range
+        vs[:] = vs[4, 0, 0]
+    q = torch.zeros(n, hq, D, dtype=torch.float16, device=DEV)
+    q[..., 0] = 4
+    bt = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    mask = ref.mask_of([-1] * n, [n], n)[0].to(DEV)
+    out, _ = ref.attention(q, k, v, bt, block, [L - n], [n], mask, ks, vs, scale=1.0)
+    # Counted as in tree_reference, A being |out|; the sums' part by what is added up, 2^18 / 16 steps of an
+    # accumulator that may cut off what it cannot hold, 2^-23 of it.  And half a probability's least step, 2^-25
+    # where a row's largest is 2^4 (the tcgen05 kernel over codes), |v| being 1, for each of 2^18 keys.
+    u = 2.0 ** -11
+    c = 2 * ((D + 8) * 2.0 ** -24 * 17.7 + 2.0 ** -16) + 2.0 ** 14 * 2.0 ** -23
+    bound = (u + (u + c) * (1 + u)) * out.abs() + 2.0 ** 18 * 2.0 ** -29
+    for split in (True, False):
+        got = _run(q, k, v, ks, vs, bt, mask, block, [L - n], [n], split=split, softmax_scale=1.0)
+        tsb.check_errors()
+        ref.assert_within(got, out, bound, f"split={split}")

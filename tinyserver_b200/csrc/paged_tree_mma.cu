@@ -27,7 +27,9 @@
 // P goes in as a 16-bit high part and the rounded remainder, so the product
 // keeps 16 significant bits or more of p; over codes and for bf16 outputs fp16's 11
 // bits, an eighth of the output's own rounding, are enough and the remainder is left
-// out.  Sums and maxima are fp32.
+// out.  fp16 ends at 2^-24, so there p is held times 2^15: full precision down to 2^-29
+// of a row's largest, and something down to 2^-39.  (Without it 2^18 keys at 2^-25.5, all
+// of a row's output beside a key whose V is 0, gave 0.)  Sums and maxima are fp32.
 //
 // Decode, 4 heads a kv head, 8 kv heads of 128: 256 sequences of up to 8191 keys over
 // e4m3 in 413 us (5.6 TB/s); 32 of 2000 keys in 38 us, of 8000 in 105 us: ~15 us besides
@@ -44,6 +46,7 @@ namespace qf {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr float kRoomLog2 = 15.f;  // P in fp16 is held times 2^15
 constexpr unsigned kAll = 0xffffffffu;
 
 __device__ __forceinline__ float pow2(float x) {
@@ -114,6 +117,7 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
     constexpr bool LO = !Q8 || std::is_same<T, __half>::value;  // P's remainder goes in too
     using MT = typename std::conditional<Q8, __half, T>::type;  // the products' operand type
     using MP = Packed<MT>;
+    constexpr float ROOM = std::is_same<MT, __half>::value ? kRoomLog2 : 0.f;
     using R = MmaRing<FMT, D>;
     constexpr int EB = R::EB, ST = R::STAGES;
     constexpr int KS = D / 16;                    // k-steps of Q K^T
@@ -338,12 +342,13 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
                     const float half = pow2(0.5f * (m[nt] - base));
                     corr[nt] = half * half;
                     m[nt] = mn;
-                    float sum = 0.f;
+                    const float pbase = base - ROOM;
+                    float sum = 0.f;  // (over codes of p itself, else of p times 2^ROOM)
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            pw[nt][n][e] = pow2(u[n][e] - base);
+                            pw[nt][n][e] = pow2(u[n][e] - pbase);
                             sum += Q8 ? pow2(t[n][e] - base) : pw[nt][n][e];
                         }
                     l[nt] = l[nt] * half * half + sum;
@@ -500,6 +505,7 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
                 Ls += wl[k * NR + ri] * f * f;
                 A += wacc[(k * NR + ri) * D + d] * f * f;
             }
+            if constexpr (Q8) A *= 1.f / (1 << (int)kRoomLog2);
             if (sg.slot < 0) {
                 // (no weight at all: 0, or NaN where every key the row sees has a NaN for a scale)
                 const int tok = r / a.G;

@@ -42,7 +42,7 @@
 // Quantised rows: the codes go into the products as they are.  K's scale multiplies
 // the score, V's (times 2^x, x of the segment's first block) the probability before
 // its one rounding; the sum takes the probability alone.  A block with a scale
-// that 2^x does not bring into [2^-6, 2^6] has V's scale in the exponent instead,
+// that 2^x does not bring into [2^-6, 2^3] has V's scale in the exponent instead,
 // p' = 2^(t + log2 vs + x - m), m being the maximum of that, so that p' fits fp16
 // whatever the scales' range.
 // P is rounded to the operand type (fp16 over quantised rows, else the query's):
@@ -67,9 +67,20 @@ constexpr unsigned kFull = 0xffffffffu;
 // What beginning and ending an item costs, in blocks.  64 trees of 64, 16 of 16 over
 // 16-bit rows, 32 of 32 over e4m3: 347, 48.7, 214 us; with 2: 370, 53.5, 234; 8: 357, 51.9, 213.
 constexpr int kItemBlocks = 4;
-constexpr float kKeepLog2 = 8.f;    // the reference maximum moves when the row's has grown by 2^8
-constexpr float kScaleLog2 = 6.f;   // log2 of the v-scales (times 2^x) that a probability is multiplied by
-
+// The probabilities' range.  When a row's reference moves, its largest p becomes 2^ROOM; it
+// moves again once p would pass 2^TOP, 2^8 more (2^6 more, over codes: 212 -> 239 us).  fp16
+// ends at 2^-24 and 2^16, so over fp16 rows TOP is 15, and over codes 12, since V's scales
+// (times 2^x), 2^-6 to 2^3 of them, go into P before its rounding.  So p keeps fp16's
+// precision down to 2^-21 of a row's largest, over codes 2^-18, and something down to 2^-31
+// and 2^-28.  (With ROOM 0, 2^18 keys at 2^-25.5, all of a row's output beside a key whose V
+// is 0, gave 0.)
+template <bool Q8, typename MT>
+struct PRange {
+    static constexpr bool H = std::is_same<MT, __half>::value;
+    static constexpr float TOP = Q8 ? 12.f : H ? 15.f : 8.f;
+    static constexpr float ROOM = Q8 ? 4.f : H ? 7.f : 0.f;
+};
+constexpr float kScaleLow = -6.f, kScaleTop = 3.f;  // log2 of those scales
 
 template <int NT>
 struct TreeTc {
@@ -304,6 +315,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
     constexpr bool Q8 = FMT != QF_CACHE_PLAIN;
     using MT = typename std::conditional<Q8, __half, T>::type;
     using MP = Packed<MT>;
+    using PR = PRange<Q8, MT>;
     constexpr int ST = C::ST, LW = C::LW;
     constexpr bool TURNS = NT == 1;  // the warpgroups take turns at one tile's blocks
     constexpr int STEP = TURNS ? 2 : 1;  // between a warpgroup's blocks
@@ -456,7 +468,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const float v = vs[x] * f, lv = log2f(vs[x]) + (float)vexp;
-                    if ((ok[x] >> lane) & 1) near = near && fabsf(lv) <= kScaleLog2;  // (a NaN is not near)
+                    if ((ok[x] >> lane) & 1) near = near && lv >= kScaleLow && lv <= kScaleTop;  // (a NaN is not near)
                     sk[slot][x * 32 + lane] = ks[x];
                     sv[slot][x * 32 + lane] = v;
                     sl[slot][x * 32 + lane] = lv;
@@ -819,8 +831,8 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
             const uint32_t sh = sS + (uint32_t)c0;
             const uint32_t see2[2] = {h ? see[2] : see[0], h ? see[3] : see[1]};
             // The reference moves: O and l with it.
-            auto follow = [&](bool move, float mx) {
-                const float half = move ? ex2(0.5f * (m - mx)) : 1.f, corr = half * half;
+            auto follow = [&](bool move, float to) {
+                const float half = move ? ex2(0.5f * (m - to)) : 1.f, corr = half * half;
                 if (!first || h > 0) {
                     // O is between two products: those of the block before were done before this
                     // block's S, the first half's are waited for, this half's wait for P
@@ -840,11 +852,11 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
                     }
                 }
                 l = l * half * half;  // (it may be 2^100 and more where a scale is part of m)
-                if (move) m = mx;
+                if (move) m = to;
             };
             if (!Q8 || near) {
             // One pass over S against the reference m, P in registers, the half block's maximum
-            // on the side.  While no row's maximum has grown past 2^8 (but for the first blocks,
+            // on the side.  While no row's p has grown past 2^TOP (but for the first blocks,
             // nearly always) P stands; else the reference moves, and the pass is made again over
             // S, which P has not touched yet.
             uint32_t pk[32];
@@ -902,9 +914,9 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
                 }
                 sum = (s0 + s1) + (s2 + s3);
                 const float mx = fmaxf(mx0, mx1) * rs;
-                const bool move = turn == 0 && (mx > m + kKeepLog2 || (m == -INFINITY && mx > -INFINITY));
+                const bool move = turn == 0 && (mx > m + PR::TOP || (m == -INFINITY && mx > -INFINITY));
                 if (!__any_sync(kFull, move)) break;
-                follow(move, mx);
+                follow(move, mx - PR::ROOM);
                 if (!got) break;
             }
             if (!got) break;
@@ -937,8 +949,8 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
             uint32_t pk[8];
 #pragma unroll 1
             for (int c = 0; c < 64; c += 16) quarter(c, 0.f, &mx, &sum, pk);
-            const bool move = mx > m + kKeepLog2 || (m == -INFINITY && mx > -INFINITY);
-            if (__any_sync(kFull, move)) follow(move, mx);
+            const bool move = mx > m + PR::TOP || (m == -INFINITY && mx > -INFINITY);
+            if (__any_sync(kFull, move)) follow(move, mx - PR::ROOM);
             if (!got) break;
             sum = 0.f;
 #pragma unroll 1
