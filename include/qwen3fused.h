@@ -330,7 +330,7 @@ size_t qf_kv_quantized_args_size(void);
  * q, out: (T, Hq, D), token and head strides, head_dim contiguous, rows
  * 16-byte aligned; caches (N, Hkv, B, D) with equal strides, head_dim
  * contiguous, rows 16-byte aligned (`cache_format` says what they hold); scales
- * (N, Hkv, B), equal strides, not negative, below 2^-100 read as that, for the
+ * (N, Hkv, B), equal strides, not negative (one of V below 2^-126 reads as 0), for the
  * quantised formats; block_tables int32 rows; context_lens, cu_seqlens_q int32; tree_mask (T, mask_words) int64.
  * head_dim 64, 128 or 256; any Hq / Hkv; block tables of at most 2^30 keys a row, and
  * sequences x kv heads x the longest table's blocks of 64 keys below 2^31.

@@ -494,3 +494,22 @@ def test_small_weights_beside_keys_without_a_value(fmt, n, hq, D, parts):
         got = _run(q, k, v, ks, vs, bt, mask, block, [L - n], [n], split=split, softmax_scale=1.0)
         tsb.check_errors()
         ref.assert_within(got, out, bound, f"split={split}")
+
+
+@pytest.mark.parametrize("fmt", ref.FORMATS)
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("n,hq", [(1, 2), (8, 4), (40, 8), (80, 8)])
+def test_the_least_scales_that_the_store_writes(fmt, dtype, n, hq):
+    """V rows of 2^-108 to 2^-90, whose scales go down to 2^-100 / Q: attention reads them as the load does."""
+    sizes, contexts = [n, 1], [1100, 40]
+    q, k, v, ks, vs, bt, mask = _case(sizes, contexts, hq, 2, 128, 16, dtype, fmt, 13)
+    g = torch.Generator().manual_seed(2)
+    rows = torch.randn(v.shape, generator=g) * 2.0 ** torch.randint(-108, -90, (*v.shape[:3], 1), generator=g)
+    rows[bt[0, 20:40].cpu().long()] *= 2.0 ** -10  # pages of the least of them alone
+    rows[bt[1].cpu().long()] *= 2.0 ** -10
+    v, vs = (x.to(DEV) for x in ref.quantise(rows, fmt))
+    out, bound = ref.attention(q, k, v, bt, 16, contexts, sizes, mask, ks, vs, p_type=torch.float16)
+    for split in (True, False):
+        got = _run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes, split=split)
+        tsb.check_errors()
+        ref.assert_within(got, out, bound, f"split={split}")

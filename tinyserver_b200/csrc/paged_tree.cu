@@ -307,7 +307,8 @@ struct Join {
         for (int p = sub; p < n; p += WPR) {
             const float* wp = partial(p);
             const float2 ml = *reinterpret_cast<const float2*>(wp + D);
-            // (a factor in two halves: a sum may be 2^100 and more, see kLeastScale)
+            // (a factor in two halves: a sum may be 2^100 and more where V's scales are in
+            // the reference)
             const float h = exp2f(0.5f * (ml.x - base)), f = h * h;
             Ls += ml.y * h * h;
 #pragma unroll

@@ -20,7 +20,7 @@
 //    as the 8-wide index, 8 rows cost half of what they would as the 16-wide.
 // Codes become fp16 in registers (both formats are exact there).  Their row
 // scales never touch the codes: K's multiplies the score t, V's enters the
-// exponent, p' = 2^(t + log2 vs - m) with m the maximum of that sum, so that p' is
+// exponent, p' = 2^(t + log2 vs - m) with m the maximum of that sum (see kLeastLog2), so that p' is
 // in [0, 1] however the scales vary; the row's sum takes 2^(t - m), and O / l is the
 // definition.  Queries become fp16 after a power-of-two row factor that puts
 // their largest element in [2^14, 2^15): exact for every element within 2^-28 of it.
@@ -47,6 +47,10 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr float kRoomLog2 = 15.f;  // P in fp16 is held times 2^15
+// In the reference a V scale counts as 2^-100 at least (a row never written has 0): the sum,
+// which has no scale in it, grows by 2^100 a key at most, and 2^27 of them stay finite.  Such
+// keys' p is below 1 for it: the least scale that the store writes, 2^-108.8, leaves 2^6.2.
+constexpr float kLeastLog2 = -100.f;
 constexpr unsigned kAll = 0xffffffffu;
 
 __device__ __forceinline__ float pow2(float x) {
@@ -300,7 +304,7 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
 
                 // online softmax; this lane: rows gid (+ 8), keys 8 n + 2 tig + e
                 const bool draft = a.cu && j0 + 16 > w.ctx;
-                float ksv[2][2], lvv[2][2];
+                float ksv[2][2], lvv[2][2];  // K's scales, log2 of V's (-inf: a scale of 0, values of 0)
                 if constexpr (Q8) {
                     const float* sp = reinterpret_cast<const float*>(kt + 2 * R::MAT);
 #pragma unroll
@@ -308,9 +312,8 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
                         const float2 k2 = *reinterpret_cast<const float2*>(sp + 8 * n + 2 * tig);
                         const float2 v2 = *reinterpret_cast<const float2*>(sp + 16 + 8 * n + 2 * tig);
                         ksv[n][0] = k2.x, ksv[n][1] = k2.y;
-                        // a scale of 0 (a row never written) stands for zeros, as good as at 2^-100
-                        lvv[n][0] = log2_of(v2.x < kLeastScale ? kLeastScale : v2.x);
-                        lvv[n][1] = log2_of(v2.y < kLeastScale ? kLeastScale : v2.y);
+                        lvv[n][0] = log2_of(v2.x);
+                        lvv[n][1] = log2_of(v2.y);
                     }
                 }
                 float pw[NRT][2][2];
@@ -332,12 +335,12 @@ __global__ void __launch_bounds__(32 * kWarps, mma_ctas(FMT == QF_CACHE_PLAIN, D
                             if constexpr (Q8) x *= ksv[n][e];
                             t[n][e] = ok ? x : -INFINITY;
                             u[n][e] = Q8 ? (ok ? x + lvv[n][e] : -INFINITY) : t[n][e];
-                            mx = fmaxf(mx, u[n][e]);
+                            mx = fmaxf(mx, Q8 ? t[n][e] + fmaxf(lvv[n][e], kLeastLog2) : t[n][e]);
                         }
                     mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 2));
                     const float mn = fmaxf(m[nt], mx), base = mn == -INFINITY ? 0.f : mn;
-                    // (in two steps: l may be 2^100 and more, see kLeastScale, and what is left
+                    // (in two steps: l may be 2^100 and more, see kLeastLog2, and what is left
                     // of it count, where the factor alone is too small for a float)
                     const float half = pow2(0.5f * (m[nt] - base));
                     corr[nt] = half * half;

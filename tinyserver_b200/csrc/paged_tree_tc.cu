@@ -43,7 +43,7 @@
 // the score, V's (times 2^x, x of the segment's first block) the probability before
 // its one rounding; the sum takes the probability alone.  A block with a scale
 // that 2^x does not bring into [2^-6, 2^3] has V's scale in the exponent instead,
-// p' = 2^(t + log2 vs + x - m), m being the maximum of that, so that p' fits fp16
+// p' = 2^(t + log2 vs + x - m), m being the maximum of that (see kLeastLog2), so that p' fits fp16
 // whatever the scales' range.
 // P is rounded to the operand type (fp16 over quantised rows, else the query's):
 // half a step of the same size as the output's own.  Sums, maxima and O are fp32.
@@ -81,6 +81,9 @@ struct PRange {
     static constexpr float ROOM = Q8 ? 4.f : H ? 7.f : 0.f;
 };
 constexpr float kScaleLow = -6.f, kScaleTop = 3.f;  // log2 of those scales
+// In the reference a V scale (times 2^x) counts as 2^-85 at least (a row never written has 0):
+// the sum, which has no scale in it, grows by 2^(85 + TOP) a key at most.
+constexpr float kLeastLog2 = -85.f;
 
 template <int NT>
 struct TreeTc {
@@ -451,10 +454,6 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
         auto inform = [&](int slot, bool first) {
             if (lane == 0) *reinterpret_cast<uint4*>(valid[slot]) = make_uint4(ok[0], ok[1], ok[2], ok[3]);
             if constexpr (Q8) {
-                // a scale of 0 (a row never written) stands for zeros, as good as at 2^-100
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    if (vs[x] < kLeastScale) vs[x] = kLeastScale;
                 if (first) {
                     float top = 0.f;
 #pragma unroll
@@ -938,7 +937,7 @@ __global__ void __launch_bounds__(TreeTc<NT>::THREADS, 1)
                         const bool ok = ((c & 32 ? see2[1] : see2[0]) >> ((c & 31) + e + y)) & 1;
                         const float tt = ok ? __uint_as_float(x[e + y]) * sk[slot][c0 + cc] * rs : -INFINITY;
                         u[y] = ok ? tt + sl[slot][c0 + cc] : -INFINITY;
-                        *mx = fmaxf(*mx, u[y]);
+                        *mx = fmaxf(*mx, tt + fmaxf(sl[slot][c0 + cc], kLeastLog2));
                         *sum += ex2(tt - mref);
                         p[y] = ex2(u[y] - mref);
                     }

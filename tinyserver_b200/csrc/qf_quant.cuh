@@ -18,11 +18,6 @@
 
 namespace qf {
 
-// The kernels that take log2 of a row's scale read a smaller one (0: a row never
-// written) as this: a sum against a reference that such a scale is part of grows by
-// 2^100 a key, and a sequence of up to 2^27 of them stays finite.
-constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100
-
 template <int FMT>
 __device__ __forceinline__ float code_top() {
     return FMT == QF_CACHE_E4M3 ? 448.f : 127.f;

@@ -121,7 +121,7 @@ def paged_attention_quantized(query: torch.Tensor, k_cache: torch.Tensor, v_cach
     one query token per sequence, ``query`` (num_seqs, Hq, D), against the
     first ``seq_lens[s]`` cached tokens of sequence s, their rows dequantised as
     they are read.  Any Hq / Hkv; a sequence of no tokens gives zeros.  Scales are
-    what the store writes, not negative; one below 2**-100 reads as that."""
+    what the store writes, not negative; one of V below 2**-126 reads as 0."""
     what = "paged_attention_quantized"
     if query.dim() == 3 and (seq_lens.dim() != 1 or seq_lens.numel() != query.shape[0]):
         raise ValueError(f"{what}: seq_lens must be (num_seqs,) for {query.shape[0]} queries, got "
