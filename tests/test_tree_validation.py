@@ -267,3 +267,12 @@ def test_reference_attention_against_a_softmax():
         for h in range(4):
             p = torch.softmax(q[t, h].double() @ kk[:, h // 2].T / 4, -1)
             assert torch.allclose(out[t, h], p @ vv[:, h // 2])
+
+
+@pytest.mark.parametrize("kw,decode", [(dict(lens=torch.zeros(2)), True), (dict(lens=torch.zeros(2)), False),
+                                       (dict(block_tables=torch.zeros(2, 3)), True),
+                                       (dict(block_tables=torch.zeros(2, 3, dtype=torch.int16)), False),
+                                       (dict(cu=torch.tensor([0., 2., 5.])), False)])
+def test_attention_refuses_lengths_and_tables_of_other_types(kw, decode):
+    with pytest.raises(ValueError, match="index dtype"):
+        _attend(decode, **kw)

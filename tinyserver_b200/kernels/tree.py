@@ -173,6 +173,9 @@ def attend(what: str, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         raise ValueError(f"{what}: block_tables must be (num_seqs, max_blocks) and the lengths "
                          f"(num_seqs,), got {tuple(block_tables.shape)} and {tuple(lens.shape)}")
     tag = dtype_tag(query, what)
+    for index in (block_tables, lens, cu_seqlens):
+        if index is not None:
+            index_tag(index, what)
     dev = device_index(what, query, k_cache, v_cache, block_tables, lens, k_scale, v_scale,
                        cu_seqlens, tree_mask, workspace)
     q = query
