@@ -347,3 +347,24 @@ def test_keys_of_nan_scales_alone_give_nan(fmt, dtype, hq):
         tsb.check_errors()
         assert torch.equal(torch.isnan(got).all(-1), want) and torch.isfinite(got[~want]).all(), split
         assert not got[3].any()
+
+
+def test_int64_lengths_and_blocks_past_32_bits_are_cut_and_flagged():
+    """2^32 + 5 keys are more than the table describes, not 5; block 2^32 + 1 is no block of the cache, not 1."""
+    lens = [40, 30]
+    k, v, ks, vs, bt = paged(lens, 2, 128, 16, torch.int8, torch.bfloat16, seed=12)
+    q = torch.randn(2, 8, 128, device=DEV).to(torch.bfloat16)
+    run = lambda b, n: tsb.paged_attention_quantized(q, k, v, ks, vs, b, 16, torch.tensor(n, device=DEV))  # noqa: E731
+    cap = bt.shape[1] * 16
+    want = run(bt, [cap, 30])
+    tsb.check_errors()
+    got = run(bt, [(1 << 32) + 5, 30])
+    with pytest.raises(IndexError, match="block table"):
+        tsb.check_errors()
+    assert torch.equal(got, want)
+    far = bt.long()
+    far[1, :2] += 1 << 32
+    got = run(far, lens)
+    with pytest.raises(IndexError, match="block index"):
+        tsb.check_errors()
+    assert not got[1].any()

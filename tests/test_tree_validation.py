@@ -276,3 +276,15 @@ def test_reference_attention_against_a_softmax():
 def test_attention_refuses_lengths_and_tables_of_other_types(kw, decode):
     with pytest.raises(ValueError, match="index dtype"):
         _attend(decode, **kw)
+
+
+def test_int64_lengths_stay_out_of_range_as_int32():
+    """What is beyond int32 is the least or the largest of it, which the kernels cut and report: never a small
+    number that it happens to equal modulo 2^32."""
+    from tinyserver_b200.kernels.tree import _int32
+
+    got = _int32(torch.tensor([(1 << 32) + 5, -(1 << 32) + 5, 1 << 31, 7, -3, (1 << 31) - 1]))
+    assert got.dtype == torch.int32
+    assert got.tolist() == [(1 << 31) - 1, -(1 << 31), (1 << 31) - 1, 7, -3, (1 << 31) - 1]
+    for t in (torch.tensor([3, 4], dtype=torch.int32), torch.tensor([[1, 2], [3, 4]], dtype=torch.int32)):
+        assert _int32(t) is t

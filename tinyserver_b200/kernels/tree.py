@@ -31,10 +31,15 @@ __all__ = ["build_tree_mask", "paged_tree_attention", "paged_tree_attention_work
 CACHE_FORMATS = {torch.float8_e4m3fn: _capi.QF_CACHE_E4M3, torch.int8: _capi.QF_CACHE_INT8}
 
 
+def _narrow(t: torch.Tensor) -> torch.Tensor:
+    """``t`` (int32 or int64) as int32.  What int32 does not hold becomes its least or
+    largest number, which the kernels cut and report, not another one in range."""
+    return t if t.dtype == torch.int32 else t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+
+
 def _int32(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as contiguous int32, itself where it is that already."""
-    if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+    """:func:`_narrow`, contiguous."""
+    t = _narrow(t)
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -184,7 +189,7 @@ def attend(what: str, query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     if sq[2] != 1 or (sq[0] * es) % 16 or (sq[1] * es) % 16 or q.data_ptr() % 16:
         q = torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q)  # the kernels' alignment
         sq = q.stride()
-    bt = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
+    bt = _narrow(block_tables)
     max_blocks = bt.shape[1]
     if max_blocks > 1 and bt.stride(1) != 1:
         bt = bt.contiguous()
