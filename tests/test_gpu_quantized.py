@@ -368,3 +368,16 @@ def test_int64_lengths_and_blocks_past_32_bits_are_cut_and_flagged():
     with pytest.raises(IndexError, match="block index"):
         tsb.check_errors()
     assert not got[1].any()
+
+
+def test_int64_slots_beside_int32_blocks_keep_their_values():
+    """Slot 2^32 + 3 is no slot of the page, whatever the type of the block mapping."""
+    k = torch.ones(2, 2, 128, dtype=torch.bfloat16, device=DEV)
+    codes, scales = _empty_cache((4, 2, 8, 128), torch.int8)
+    before = codes.clone(), scales.clone()
+    bm = torch.tensor([1, 2], dtype=torch.int32, device=DEV)
+    sm = torch.tensor([(1 << 32) + 3, -(1 << 32)], device=DEV)
+    tsb.store_kv_cache_quantized(k, k, codes, codes, scales, scales, bm, sm)
+    with pytest.raises(IndexError, match="slot"):
+        tsb.check_errors()
+    assert torch.equal(codes, before[0]) and torch.equal(scales, before[1])

@@ -288,3 +288,15 @@ def test_int64_lengths_stay_out_of_range_as_int32():
     assert got.tolist() == [(1 << 31) - 1, -(1 << 31), (1 << 31) - 1, 7, -3, (1 << 31) - 1]
     for t in (torch.tensor([3, 4], dtype=torch.int32), torch.tensor([[1, 2], [3, 4]], dtype=torch.int32)):
         assert _int32(t) is t
+
+
+def test_mappings_of_two_types_keep_their_values():
+    from tinyserver_b200.kernels.quantized import _mappings
+
+    small, large = torch.tensor([1, 2], dtype=torch.int32), torch.tensor([3, (1 << 32) + 4])
+    for pair in ((small, large), (large, small)):
+        bm, sm, tag = _mappings("test", *pair)
+        assert bm.tolist() == pair[0].tolist() and sm.tolist() == pair[1].tolist()
+        assert bm.dtype == sm.dtype == torch.int64 and tag == _capi.QF_I64
+    bm, sm, tag = _mappings("test", small, small)
+    assert bm is small and sm is small and tag == _capi.QF_I32

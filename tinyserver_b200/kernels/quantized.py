@@ -32,9 +32,9 @@ def _mappings(what: str, block_mapping: torch.Tensor, slot_mapping: torch.Tensor
         raise ValueError(f"{what}: block_mapping and slot_mapping must be 1D of one length, got "
                          f"{tuple(block_mapping.shape)} and {tuple(slot_mapping.shape)}")
     itag = index_tag(block_mapping, f"{what} block_mapping")
-    index_tag(slot_mapping, f"{what} slot_mapping")
-    if slot_mapping.dtype != block_mapping.dtype:
-        slot_mapping = slot_mapping.to(block_mapping.dtype)
+    if index_tag(slot_mapping, f"{what} slot_mapping") != itag:  # both as the wider
+        itag = _capi.QF_I64
+        block_mapping, slot_mapping = block_mapping.long(), slot_mapping.long()
     if not block_mapping.is_contiguous():
         block_mapping = block_mapping.contiguous()
     if not slot_mapping.is_contiguous():
