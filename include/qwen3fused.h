@@ -361,7 +361,9 @@ typedef struct {
 int qf_paged_tree_attention(const qf_paged_tree_attention_args* args, cudaStream_t stream);
 
 /* Workspace bytes that let qf_paged_tree_attention split long sequences over
- * several CTAs (0: nothing to split).  Reads sizes, dtype and cache_format only. */
+ * several CTAs (0: nothing to split).  Reads sizes, dtype and cache_format, and
+ * whether cu_seqlens_q is NULL: then enough for a decode call, and for one of trees
+ * of max_tree whose arrays are not there yet; else for the tree call alone. */
 size_t qf_paged_tree_attention_workspace_bytes(const qf_paged_tree_attention_args* args);
 
 /* sizeof(qf_paged_tree_attention_args) as compiled into the library. */

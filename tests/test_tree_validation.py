@@ -300,3 +300,15 @@ def test_mappings_of_two_types_keep_their_values():
         assert bm.dtype == sm.dtype == torch.int64 and tag == _capi.QF_I64
     bm, sm, tag = _mappings("test", small, small)
     assert bm is small and sm is small and tag == _capi.QF_I32
+
+
+def test_workspace_sizes_before_the_arrays_exist():
+    """cu_seqlens_q NULL: enough for the trees' call, and for a decode call of the same sizes."""
+    size = lambda **kw: _capi.lib().qf_paged_tree_attention_workspace_bytes(_tree_args(**kw))  # noqa: E731
+    for fmt in (_capi.QF_CACHE_PLAIN, _capi.QF_CACHE_E4M3):
+        for dtype in (_capi.QF_F32, _capi.QF_BF16):
+            for max_tree in (1, 3, 64):
+                kw = dict(cache_format=fmt, dtype=dtype, max_tree=max_tree)
+                trees, decode = size(**kw), size(**kw, cu_seqlens_q=0)
+                assert 0 < trees <= decode
+                assert size(**{**kw, "max_tree": 1}, cu_seqlens_q=0) <= decode

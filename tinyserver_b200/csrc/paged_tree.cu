@@ -545,7 +545,14 @@ int launch_tree_f32(const TreeDev& a, int format, int D, int rows, int ctas, cud
 
 extern "C" size_t qf_paged_tree_attention_workspace_bytes(const qf_paged_tree_attention_args* p) {
     if (!p || !qf::known_sizes(*p)) return 0;
-    return qf::plan_bytes(*p, qf::make_plan(*p));
+    qf_paged_tree_attention_args g = *p;
+    size_t bytes = qf::plan_bytes(g, qf::make_plan(g));
+    if (!g.cu_seqlens_q) {
+        static const int32_t some = 0;
+        g.cu_seqlens_q = &some;  // (whether there is one is all that is read)
+        bytes = std::max(bytes, qf::plan_bytes(g, qf::make_plan(g)));
+    }
+    return bytes;
 }
 
 extern "C" size_t qf_paged_tree_attention_args_size(void) {
