@@ -381,3 +381,20 @@ def test_int64_slots_beside_int32_blocks_keep_their_values():
     with pytest.raises(IndexError, match="slot"):
         tsb.check_errors()
     assert torch.equal(codes, before[0]) and torch.equal(scales, before[1])
+
+
+@pytest.mark.parametrize("fmt", ref.FORMATS)
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("hq,hkv,block", [(32, 1, 16), (71, 1, 24), (160, 1, 16), (100, 2, 4), (60, 2, 5)])
+def test_decode_of_many_heads_per_kv_head(fmt, dtype, hq, hkv, block):
+    """More than 24 query heads a kv head: one node a sequence and no mask in the tcgen05 kernel."""
+    lens = [0, 1, 127, 128, 129, 1029, 5000]
+    k, v, ks, vs, bt = paged(lens, hkv, 128, block, fmt, dtype, seed=hq + block)
+    q = torch.randn(len(lens), hq, 128, generator=torch.Generator().manual_seed(5)).to(dtype).to(DEV)
+    out, bound = ref.attention(q, k, v, bt, block, lens, k_scale=ks, v_scale=vs, p_type=torch.float16)
+    sl = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    for split in (True, False):
+        got = tsb.paged_attention_quantized(q, k, v, ks, vs, bt, block, sl, split=split)
+        tsb.check_errors()
+        assert not got[0].any()
+        ref.assert_within(got, out, bound, f"split={split}")

@@ -513,3 +513,11 @@ def test_the_least_scales_that_the_store_writes(fmt, dtype, n, hq):
         got = _run(q, k, v, ks, vs, bt, mask, 16, contexts, sizes, split=split)
         tsb.check_errors()
         ref.assert_within(got, out, bound, f"split={split}")
+
+
+@pytest.mark.parametrize("fmt,block", [(None, 8), (None, 24), (None, 32), (None, 64)] +
+                         [(f, b) for f in ref.FORMATS for b in (4, 8, 12, 32, 64)])
+def test_pages_of_every_power_of_two(fmt, block):
+    """Boxes of 4 to 64 slots, a page in one or several, with ends inside them; one tile of rows and two."""
+    for hq in (4, 8):
+        _check([9, 40, 1], [333, 127, 1029], hq, 2, 128, block, torch.bfloat16, fmt, seed=block + hq)
