@@ -398,3 +398,24 @@ def test_decode_of_many_heads_per_kv_head(fmt, dtype, hq, hkv, block):
         tsb.check_errors()
         assert not got[0].any()
         ref.assert_within(got, out, bound, f"split={split}")
+
+
+@pytest.mark.parametrize("fmt", ref.FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128, 256, 80, 1])
+def test_rows_come_back_within_half_a_step(fmt, dtype, D):
+    """What the kernels stored and loaded, K and V: half a step of the code from the source, 1 / 127 of the row's
+    largest value for int8; 2^-3 of the value, or 2^-9 codes below 2^-6 of them, for e4m3.  Two roundings of 2^-24
+    on the way to the code, and two on the way back."""
+    g = torch.Generator().manual_seed(D + 1)
+    for T in (1, 33, 130):
+        k, v = (torch.randn(3, T, D, generator=g).mul_(10.0 ** torch.randint(-3, 4, (3, T, 1), generator=g))
+                .to(dtype) for _ in range(2))
+        pools, bm, sm = _check_store(k, v, fmt, 16, 12, g)
+        got = tsb.load_kv_cache_quantized(pools[0][0], pools[1][0], pools[0][1], pools[1][1], bm.to(DEV),
+                                          sm.to(DEV), torch.float32)
+        for x, src in zip(got, (k.double(), v.double())):
+            top = src.abs().amax(-1, keepdim=True)
+            half = (0.5 / 127 * top).expand_as(src) if fmt == torch.int8 else \
+                torch.maximum(2.0 ** -4 * src.abs(), 2.0 ** -10 * top / 448)
+            assert ((x.double().cpu() - src).abs() <= half + 4 * 2.0 ** -24 * top).all()
