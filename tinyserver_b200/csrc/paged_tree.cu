@@ -25,10 +25,11 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 // Rows per kv head that the mma.sync kernel takes at head_dim 128, over 16-bit and over
 // 8-bit rows (it reads the cache once per 16 of them, the tcgen05 kernel once per 256).
-// 32 trees at 4096 context keys, 8 kv heads, mma.sync | tcgen05: bf16, 8 rows 105 | 109
-// us, 16 rows 101 | 110, 24 rows 182 | 111; e4m3, 16 rows 84 | 171, 24 rows 146 | 171, 32
-// rows 151 | 155 (int8 166 | 144), 48 rows 217 | 176; 2 trees at 700 keys, bf16, 16 rows
-// 15.9 | 17.2, 24 rows 18.7 | 17.2.
+// 32 trees at 4096 context keys, 8 kv heads, pages of 16, mma.sync | tcgen05: bf16, 8 rows
+// 101 | 106 us, 16 rows 101 | 106, 24 rows 182 | 107; e4m3, 16 rows 85 | 171, 24 rows 148 |
+// 170, 32 rows 154 | 156 (int8 167 | 144), 48 rows 220 | 176; 2 trees at 700 keys, bf16, 16
+// rows 13.9 | 16.4, 24 rows 16.9 | 16.4.  The same with 2 kv heads and pages of 64: bf16, 16
+// rows 40.8 | 41.9, 24 rows 57.0 | 42.2; e4m3, 24 rows 48.1 | 58.0, 32 rows 49.5 | 56.8.
 constexpr int kMmaRows = 16, kMmaRows8 = 24;
 constexpr int kF32Keys = 64;  // keys of a work unit of the fp32 kernel
 

@@ -1,7 +1,10 @@
 // Paged attention for few query rows per kv head (a decode step's G heads, a
 // small tree's tokens x G), 16-bit queries, over a 16-bit or a quantised
 // cache.  Bound by HBM: every K and V row is read once and meets at most 16
-// rows.
+// rows (8 at head_dim 256).  More rows, at head_dim 64 and 256, where the tcgen05
+// kernel has no form, and up to 24 over codes at 128, go in groups of that many, each
+// of which reads the keys again, bound by its instructions: 32 trees of 16 and of 64 nodes x 4 heads at 4096 keys, 8 kv heads, over bf16 204 and
+// 777 us at head_dim 64, 1495 and 6229 at 256; over e4m3 212 and 749, 775 and 3528.
 //
 // Warps take tiles of 16 keys in turn, each through a ring of its own in shared
 // memory that cp.async fills three or four tiles deep: 40 KB and more per SM in
@@ -32,10 +35,10 @@
 // of a row's output beside a key whose V is 0, gave 0.)  Sums and maxima are fp32.
 //
 // Decode, 4 heads a kv head, 8 kv heads of 128: 256 sequences of up to 8191 keys over
-// e4m3 in 413 us (5.6 TB/s); 32 of 2000 keys in 38 us, of 8000 in 105 us: ~15 us besides
+// e4m3 in 416 us (5.5 TB/s); 32 of 2000 keys in 38 us, of 8000 in 106 us: ~15 us besides
 // the bytes, a launch each of this kernel and the join's, and per item Q's load, the
-// rings' filling and the warps' join.  Issue slots are 59% used over e4m3 (~500
-// instructions per 16 keys and warp); over bf16 32 of 4096 keys take 102 us (5.3 TB/s).
+// rings' filling and the warps' join.  Issue slots are 54% used over e4m3 (470
+// instructions per 16 keys and warp); over bf16 32 of 4096 keys take 101 us (5.3 TB/s).
 #include <math.h>
 
 #include "qf_mma.cuh"
@@ -98,12 +101,12 @@ struct MmaRing {
 constexpr int kMmaKeys = 16 * kWarps;  // keys of a work unit
 
 // CTAs per SM: by the registers that a kernel needs (wide heads and 16-bit fragments take
-// more) and the rings' shared memory.  Each measured with a slower join than today's:
-// decode over e4m3 as above with two, three, four CTAs 494, 425, 433 us; 32 trees of 4
-// nodes x 4 heads at 4096 keys over e4m3, one, two, three: 150, 114, 111; over bf16, one,
-// two: 158, 125; at head_dim 64 over e4m3, three, four, five: 76.4, 76.2, 87.1, of one
-// node over bf16, two, three, four: 59.1, 58.7, 60.3; at head_dim 256 over e4m3, of one
-// node, one, two: 147, 109.
+// more) and the rings' shared memory.  Decode over e4m3 as above with two, three, four CTAs
+// 496, 417, 421 us; of 32 sequences of 8000 keys, 2 kv heads of 8 heads, pages of 64: 41.4,
+// 38.8, 41.0; 32 trees of 4 nodes x 4 heads at 4096 keys over e4m3: 92, 85, 137; over bf16,
+// one, two: 146, 101; at head_dim 64 over e4m3, three, four, five: 60.4, 59.2, 68.9, of one
+// node 46.8, 44.9, 46.1, and over bf16, two, three, four: 55.8, 54.8, 55.3; at head_dim 256
+// over e4m3, of one node, one, two: 148, 104.
 constexpr int mma_ctas(bool plain, int D) {
     return D == 256 ? (plain ? 1 : 2) : D == 128 ? (plain ? 2 : 3) : plain ? 3 : 4;
 }

@@ -31,11 +31,13 @@
 //    TB/s (two CTAs per SM with one stage each and halves of a block in turn: 127 us).
 //  * 8-bit rows: by the softmax warps' dependent instructions (two warps per scheduler;
 //    36% of the issue slots used): a half block takes 2300 cycles, against 1100 over
-//    16-bit rows, for the scales' loads and products.  The same trees over e4m3: 154 us
-//    (182 us); 32 trees of 32 nodes at up to 8191 context keys: 213 us.
+//    16-bit rows, for the scales' loads and products.  The same trees over e4m3: 158 us
+//    (182 us then); 32 trees of 32 nodes at up to 8191 context keys: 208 to 238 us, from
+//    process to process.
 //  * More than 128 rows: by the chain of products and softmax, ~4100 cycles a block of
-//    two tiles; 64 trees of 64 nodes x 4 heads at up to 8191 context keys: 329 us, 925
-//    TFLOP/s (as single tiles, which read K and V twice, 445 us against 350 then).
+//    two tiles; 64 trees of 64 nodes x 4 heads at up to 8191 context keys: 332 to 345
+//    us, 880 to 920 TFLOP/s (as single tiles, which read K and V twice, 445 us against 350
+//    then).
 // Registers moved from the loaders to the softmax (88 and 168 a thread instead of 128)
 // cost more in the loaders than they gained: 154 -> 206 us.
 //
